@@ -22,7 +22,7 @@ _lib = None
 
 __all__ = [
     "lib", "gemm_fp8", "gemm_i8", "gmm", "gmm_fp8", "GroupedFP8Weights", "gemm_fp8_rowcol", "gemm_fp8_swiglu", "gemm_w4a16", "gemm_nvfp4", "nvfp4_swizzle_sf",
-    "gemm_mxfp8", "mxfp8_swizzle_sf", "quant_rows_nvfp4",
+    "gemm_mxfp8", "mxfp8_swizzle_sf", "quant_rows_nvfp4", "gemm_mxfp4", "quant_rows_mxfp4",
     "gemm_sparse_fp8", "quant_rows_e4m3", "status", "check_status", "set_wait_limit_ms", "WaitTimeout", "LIB_PATH",
 ]
 
@@ -32,6 +32,7 @@ _SIZE_T_FUNCS = {
     "b200q_nvfp4_sf_bytes": [C.c_int, C.c_int],
     "b200q_mxfp8_sf_bytes": [C.c_int, C.c_int],
     "b200q_gemm_mxfp8_workspace_bytes": [C.c_int, C.c_int, C.c_int],
+    "b200q_gemm_mxfp4_workspace_bytes": [C.c_int, C.c_int, C.c_int],
     "b200q_gemm_nvfp4_static_max_bytes": [],
     "b200q_allreduce_signal_bytes": [],
     "b200q_rank_barrier_signal_bytes": [],
@@ -52,6 +53,8 @@ _SIGNATURES = {
     "b200q_gemm_mxfp8": [_VP, _VP, _VP, _VP, _VP, _I, _I, _I, _VP, _VP],
     "b200q_gemm_mxfp8_blocked": [_VP, _VP, _VP, _VP, _VP, _I, _I, _I, _VP],
     "b200q_mxfp8_swizzle_sf": [_VP, _VP, _I, _I, _VP],
+    "b200q_gemm_mxfp4": [_VP, _VP, _VP, _VP, _VP, _I, _I, _I, _VP, _VP],
+    "b200q_gemm_mxfp4_blocked": [_VP, _VP, _VP, _VP, _VP, _I, _I, _I, _VP],
     "b200q_mxfp8_set_tile_n": [_I],
     "b200q_nvfp4_set_tile_n": [_I],
     "b200q_nvfp4_set_2cta": [_I],
@@ -66,6 +69,7 @@ _SIGNATURES = {
     "b200q_gemm_sp24_fp8": [_VP, _VP, _VP, _VP, _I, _I, _I, _F, _F, _VP],
     "b200q_quant_rows_e4m3": [_VP, _VP, _VP, _I, _I, _VP],
     "b200q_quant_rows_nvfp4": [_VP, _VP, _VP, _I, _I, _F, _VP],
+    "b200q_quant_rows_mxfp4": [_VP, _VP, _VP, _I, _I, _VP],
     "b200q_status": [_VP, _I],
     "b200q_set_wait_limit_ms": [_I, _I],
     "b200q_rank_barrier": [_VP, _I, _I, C.c_uint, C.c_uint, _VP],
@@ -132,7 +136,8 @@ def _check(t: torch.Tensor, name: str, dtypes, ndim: int) -> None:
 # signatures with defaults, as op/grouped_gemm/cudaop_grouped_gemm/ops.py does for its _C module.
 
 EXTENSION_OPS = ("gemm_fp8", "gemm_fp8_rowcol", "gemm_fp8_swiglu", "gemm_w4a16", "nvfp4_swizzle_sf", "gemm_nvfp4",
-                 "mxfp8_swizzle_sf", "gemm_mxfp8", "gemm_sparse_fp8", "quant_rows_e4m3", "quant_rows_nvfp4", "gemm_i8", "gmm_fp8")
+                 "mxfp8_swizzle_sf", "gemm_mxfp8", "gemm_sparse_fp8", "quant_rows_e4m3", "quant_rows_nvfp4", "gemm_i8", "gmm_fp8",
+                 "gemm_mxfp4", "quant_rows_mxfp4")
 try:
     from . import _C                                    # noqa: F401
     _C_ERROR = None
@@ -233,6 +238,13 @@ def gemm_mxfp8(a, sfa, b, sfb, blocked: bool = False) -> torch.Tensor:
     return _ext().gemm_mxfp8(a, sfa, b, sfb, bool(blocked))
 
 
+def gemm_mxfp4(aq, sfa, bq, sfb, blocked: bool = False) -> torch.Tensor:
+    """C[M,N] (bf16) for MXFP4 operands: packed E2M1 [rows, K/2] with one UE8M0 scale per 32 K ([rows, K/32], or with
+    ``blocked=True`` the blocked layout that :func:`quant_rows_mxfp4` writes and :func:`mxfp8_swizzle_sf` makes of row-major
+    scales: the MX formats share it)."""
+    return _ext().gemm_mxfp4(aq, sfa, bq, sfb, bool(blocked))
+
+
 def gemm_sparse_fp8(a_comp, a_meta, b, scale_a: float, scale_b: float) -> torch.Tensor:
     """C[M,N] (bf16) = (expand_2:4(a_comp[M,K/2], a_meta[M,K/8]) @ B[N,K].T) * (scale_a * scale_b)."""
     return _ext().gemm_sparse_fp8(a_comp, a_meta, b, float(scale_a), float(scale_b))
@@ -247,6 +259,13 @@ def quant_rows_nvfp4(x: torch.Tensor, global_scale: float):
     """bf16 [rows, cols] -> (packed E2M1 [rows, cols/2] uint8, UE4M3 scales in the blocked layout, 1-D uint8):
     operands for :func:`gemm_nvfp4` with ``blocked=True``."""
     return _ext().quant_rows_nvfp4(x, float(global_scale))
+
+
+def quant_rows_mxfp4(x: torch.Tensor):
+    """bf16 [rows, cols] -> (packed E2M1 [rows, cols/2] uint8, UE8M0 scales per 32 columns in the blocked layout, 1-D
+    uint8): operands for :func:`gemm_mxfp4` with ``blocked=True``; also how weights are quantised, once.  A block of 32
+    that holds NaN or an infinity gets the NaN scale, so its products are NaN."""
+    return _ext().quant_rows_mxfp4(x)
 
 
 def status(clear: bool = True) -> int:

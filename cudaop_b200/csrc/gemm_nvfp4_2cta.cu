@@ -3,9 +3,11 @@
 //   FMT 1  MXFP8: E4M3 data, one UE8M0 scale per 32 K, kind::mxf8f6f4.block_scale           (256 x BN x 32)
 //          (the reference's other block-scaled format: op/test/arch_primitives/ptx_mma_fp8.cu:126-178,
 //          scale decoder op/test/arch_primitives/ptx_mma_fp6.cu:344-351)
-// Both keep a 128-byte K slab per row and stage and the same blocked scale layout (512-byte blocks of 128
-// rows x 4 scales); a block covers 64 K for NVFP4 (one MMA) and 128 K for MXFP8 (four MMAs, which pick their
-// scale byte with the scale-factor id of the instruction descriptor).  The text below describes NVFP4.
+//   FMT 2  MXFP4: E2M1 data, one UE8M0 scale per 32 K, kind::mxf4.block_scale.scale_vec::2X (256 x BN x 64)
+// All keep a 128-byte K slab per row and stage and the same blocked scale layout (512-byte blocks of 128
+// rows x 4 scales); a block covers 64 K for NVFP4 (one MMA), 128 K for MXFP8 (four MMAs, which pick their
+// scale byte with the scale-factor id of the instruction descriptor) and 128 K for MXFP4 (two MMAs, a byte pair
+// each).  The text below describes NVFP4.
 //
 // Same arithmetic and operand formats as gemm_nvfp4.cu (E2M1 data, one UE4M3 scale per 16 K in the
 // blocked layout, fp32 accumulate, global scales in the epilogue; formats:
@@ -32,8 +34,9 @@ using ptx::tma_load_3d_pair;
 using ptx::tmem_cp_32x128b_warpx4_pair;
 using ptx::umma_mxf4nvf4_pair;
 using ptx::umma_mxf8f6f4_pair;
+using ptx::umma_mxf4_pair;
 
-constexpr int kFmtNvfp4 = 0, kFmtMxfp8 = 1;
+constexpr int kFmtNvfp4 = 0, kFmtMxfp8 = 1, kFmtMxfp4 = 2;
 
 constexpr int kBM = 128;                 // rows per CTA (256 per pair)
 constexpr int kBKBytes = 128;            // per row and stage: 256 E2M1 or 128 E4M3
@@ -45,7 +48,7 @@ template <int BN, int FMT>
 struct Cfg {
     static_assert(BN % 64 == 0 && BN <= 256, "B tile width");
     static constexpr int kBKElems = (FMT == kFmtMxfp8) ? 128 : 256;  // K elements per stage
-    static constexpr int kSfBlocks = (FMT == kFmtMxfp8) ? 1 : 4;     // 512-byte scale blocks per row block and stage
+    static constexpr int kSfBlocks = (FMT == kFmtMxfp8) ? 1 : (FMT == kFmtMxfp4) ? 2 : 4;   // 512-byte scale blocks per row block and stage
     static constexpr int kMaxOff = (BN % 128 == 0) ? 0 : 64;
     static constexpr int kNB = (kMaxOff + BN + 127) / 128;           // scale row-blocks of the whole B tile
     static constexpr int kABytes = kBM * kBKBytes;
@@ -61,7 +64,7 @@ struct Cfg {
     static constexpr int kAccBufs = (2 * BN + kSfCols + kSfCols * kNB <= 512) ? 2 : 1;
     static constexpr int kSfaCol = kAccBufs * BN;
     static constexpr int kSfbCol = kSfaCol + kSfCols;
-    static_assert(FMT == kFmtMxfp8 || kLoadBytes % 1024 == 0, "stage alignment");
+    static_assert(FMT != kFmtNvfp4 || kLoadBytes % 1024 == 0, "stage alignment");
 };
 
 struct Params {
@@ -109,7 +112,9 @@ gemm_nvfp4_2cta_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_con
     const uint32_t cta_rank = ptx::cluster_ctarank();
     const int pair = blockIdx.x >> 1, pairs = gridDim.x >> 1;
     const int num_kb = (p.K + kBKElems - 1) / kBKElems;
-    const int ksteps_total = p.K / (FMT == kFmtMxfp8 ? 32 : 64);     // MMAs along K
+    // MMAs along K; MXFP4 takes K % 64 == 32: the loads zero-fill the data of the last MMA's second half, and its scale
+    // bytes are the layout's zero padding
+    const int ksteps_total = FMT == kFmtMxfp8 ? p.K / 32 : (p.K + 63) / 64;
     const int num_tiles = p.tiles_m * p.tiles_n;
 
     if (threadIdx.x == 0) {
@@ -157,9 +162,10 @@ gemm_nvfp4_2cta_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_con
         // ---------------------------------------------------------- MMA issuer (leader only)
         if (cta_rank == 0 && ptx::elect_one()) {
             // NVFP4: E2M1 (format 1 of kind::mxf4nvf4) with UE4M3 scales; MXFP8: E4M3 (format 0 of kind::mxf8f6f4) with
-            // UE8M0 scales, scale-factor ids filled in per MMA
-            constexpr uint32_t idesc = (FMT == kFmtMxfp8) ? ptx::umma_idesc_block_scaled(0, 0, 2 * kBM, BN, 0, 0, 1)
-                                                          : ptx::umma_idesc_block_scaled(1, 1, 2 * kBM, BN, 0, 0, 0);
+            // UE8M0 scales, scale-factor ids filled in per MMA; MXFP4: E2M1 with UE8M0 scales, ids 0 and 2
+            constexpr uint32_t idesc = (FMT == kFmtMxfp8)   ? ptx::umma_idesc_block_scaled(0, 0, 2 * kBM, BN, 0, 0, 1)
+                                       : (FMT == kFmtMxfp4) ? ptx::umma_idesc_block_scaled(1, 1, 2 * kBM, BN, 0, 0, 1)
+                                                            : ptx::umma_idesc_block_scaled(1, 1, 2 * kBM, BN, 0, 0, 0);
             int stage = 0; uint32_t phase = 0; bool ok = true;
             int t = 0;
             for (int tile = pair; tile < num_tiles && ok; tile += pairs, ++t) {
@@ -188,6 +194,26 @@ gemm_nvfp4_2cta_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_con
                         auto kstep = [&](int ks) {
                             const uint32_t id = idesc | (static_cast<uint32_t>(ks) << 4) | (static_cast<uint32_t>(ks) << 29);
                             umma_mxf8f6f4_pair(d_tmem, da + 2u * ks, db + 2u * ks, id, tsfa, tsfb + sfb_col_off, (kb | ks) != 0);
+                        };
+                        if (ksteps == 4) {
+#pragma unroll
+                            for (int ks = 0; ks < 4; ++ks) kstep(ks);
+                        } else {
+                            for (int ks = 0; ks < ksteps; ++ks) kstep(ks);
+                        }
+                    } else if constexpr (FMT == kFmtMxfp4) {
+                        // two scale blocks per row block and slab, each for two MMAs
+                        auto kstep = [&](int ks) {
+                            const int h = ks >> 1;
+                            if ((ks & 1) == 0) {
+                                tmem_cp_32x128b_warpx4_pair(tsfa + 4 * h, dsfa + 32u * h);
+#pragma unroll
+                                for (int i = 0; i < C::kNB; ++i)
+                                    tmem_cp_32x128b_warpx4_pair(tsfb + 4 * C::kNB * h + 4 * i, dsfb + 32u * (i * 2 + h));
+                            }
+                            const uint32_t id = idesc | (static_cast<uint32_t>(2 * (ks & 1)) << 4) | (static_cast<uint32_t>(2 * (ks & 1)) << 29);
+                            umma_mxf4_pair(d_tmem, da + 2u * ks, db + 2u * ks, id, tsfa + 4 * h,
+                                           tsfb + 4 * C::kNB * h + sfb_col_off, (kb | ks) != 0);
                         };
                         if (ksteps == 4) {
 #pragma unroll
@@ -346,9 +372,9 @@ extern "C" int b200q_nvfp4_set_group(int g)
     b200q::nvfp4p::g_group = g;
     return 0;
 }
-// Called by b200q_gemm_nvfp4_blocked (fmt 0, when the CTA-pair kernel is selected with b200q_nvfp4_set_2cta) and by
-// b200q_gemm_mxfp8_blocked (fmt 1).  Operand rows hold K/2 bytes (NVFP4) or K bytes (MXFP8); the blocked scale arrays
-// hold one 512-byte block per 128 rows and per 64 K (NVFP4) / 128 K (MXFP8).
+// Called by b200q_gemm_nvfp4_blocked (fmt 0, when the CTA-pair kernel is selected with b200q_nvfp4_set_2cta), by
+// b200q_gemm_mxfp8_blocked (fmt 1) and by b200q_gemm_mxfp4_blocked (fmt 2).  Operand rows hold K/2 bytes (E2M1) or K
+// bytes (MXFP8); the blocked scale arrays hold one 512-byte block per 128 rows and per 64 K (NVFP4) / 128 K (MX formats).
 namespace b200q {
 
 int gemm_block_scaled_pair(int fmt, const void* Aq, const void* SFA_blocked, const void* Bq, const void* SFB_blocked,
@@ -357,8 +383,8 @@ int gemm_block_scaled_pair(int fmt, const void* Aq, const void* SFA_blocked, con
     using namespace nvfp4p;
     if (Aq == nullptr || SFA_blocked == nullptr || Bq == nullptr || SFB_blocked == nullptr || C == nullptr)
         return cudaErrorInvalidValue;
-    if (fmt != kFmtNvfp4 && fmt != kFmtMxfp8) return cudaErrorInvalidValue;
-    if (M <= 0 || N <= 0 || K <= 0 || K % (fmt == kFmtMxfp8 ? 32 : 64) != 0) return cudaErrorInvalidValue;
+    if (fmt != kFmtNvfp4 && fmt != kFmtMxfp8 && fmt != kFmtMxfp4) return cudaErrorInvalidValue;
+    if (M <= 0 || N <= 0 || K <= 0 || K % (fmt == kFmtNvfp4 ? 64 : 32) != 0) return cudaErrorInvalidValue;
     if (!aligned16(Aq) || !aligned16(Bq) || !aligned16(SFA_blocked) || !aligned16(SFB_blocked)) return cudaErrorInvalidValue;
     if (bn != 192 && bn != 256) return cudaErrorInvalidValue;
     const size_t row_bytes = fmt == kFmtMxfp8 ? static_cast<size_t>(K) : static_cast<size_t>(K) / 2;
@@ -374,8 +400,8 @@ int gemm_block_scaled_pair(int fmt, const void* Aq, const void* SFA_blocked, con
     {
         // the blocked scale arrays as [row block][2 * blocks along K][256 bytes]; one box takes the blocks of a
         // K slab for all row blocks of the B tile at once
-        const uint64_t blocks_k = fmt == kFmtMxfp8 ? static_cast<uint64_t>((K + 127) / 128) : static_cast<uint64_t>(K / 64);
-        const uint32_t slab_rows = fmt == kFmtMxfp8 ? 2u : 8u;
+        const uint64_t blocks_k = fmt == kFmtNvfp4 ? static_cast<uint64_t>(K / 64) : static_cast<uint64_t>((K + 127) / 128);
+        const uint32_t slab_rows = fmt == kFmtMxfp8 ? 2u : fmt == kFmtMxfp4 ? 4u : 8u;
         const uint64_t k_rows = blocks_k * 2;
         const uint64_t strides[2] = {256, k_rows * 256};
         const uint64_t dims_a[3] = {256, k_rows, static_cast<uint64_t>((M + 127) / 128)};
@@ -401,6 +427,8 @@ int gemm_block_scaled_pair(int fmt, const void* Aq, const void* SFA_blocked, con
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     if (fmt == kFmtMxfp8)
         return bn == 192 ? launch<192, kFmtMxfp8>(tmA, tmB, tmSFA, tmSFB, tmC, p, s) : launch<256, kFmtMxfp8>(tmA, tmB, tmSFA, tmSFB, tmC, p, s);
+    if (fmt == kFmtMxfp4)
+        return bn == 192 ? launch<192, kFmtMxfp4>(tmA, tmB, tmSFA, tmSFB, tmC, p, s) : launch<256, kFmtMxfp4>(tmA, tmB, tmSFA, tmSFB, tmC, p, s);
     return bn == 192 ? launch<192, kFmtNvfp4>(tmA, tmB, tmSFA, tmSFB, tmC, p, s) : launch<256, kFmtNvfp4>(tmA, tmB, tmSFA, tmSFB, tmC, p, s);
 }
 

@@ -172,6 +172,79 @@ quant_rows_nvfp4_kernel(const __nv_bfloat16* __restrict__ X, uint32_t* __restric
     }
 }
 
+// ------------------------------------------------------------------------------------------------------
+// bf16 rows -> MXFP4: packed E2M1 [rows, cols/2] + one UE8M0 scale byte per 32 K in the blocked layout of the MX GEMMs.
+// Rule: with a = max|blk| the scale is 2^(floor(log2 a) - 2) (2 = exponent of the largest E2M1 value), at least 2^-127;
+// q = e2m1_rn(x / scale), saturating at 6.  A block holding NaN or an infinity gets the NaN scale (byte 255) and zero codes.
+// Everything is exact up to the one rounding to E2M1: the maximum is taken on the magnitude bits (NaN > infinity > finite),
+// the scale byte is the maximum's exponent field minus 2, and x / scale is a product with a power of two.
+// Bandwidth-bound (2 bytes read, 0.53125 written per element); the walk is the NVFP4 quantiser's: a warp takes
+// kVecs * 32 consecutive 16-byte vectors, a 32-element block lies in four neighbouring lanes.
+template <int kVecs>
+__global__ void __launch_bounds__(256)
+quant_rows_mxfp4_kernel(const __nv_bfloat16* __restrict__ X, uint32_t* __restrict__ Q, uint8_t* __restrict__ SF, int rows, int k32)
+{
+    const int lane = threadIdx.x & 31;
+    const int k128 = (k32 + 3) / 4;
+    const bool words = (k32 & 3) == 0;                                // four scales of a 128-K slab lie in sixteen neighbouring lanes
+    const long long vecs = static_cast<long long>(rows) * k32 * 4;    // 16-byte input vectors
+    const long long warps = (static_cast<long long>(gridDim.x) * blockDim.x) >> 5;
+    const long long spans = (vecs + 32 * kVecs - 1) / (32 * kVecs);
+    const uint4* x = reinterpret_cast<const uint4*>(X);
+    for (long long sp = (static_cast<long long>(blockIdx.x) * blockDim.x + threadIdx.x) >> 5; sp < spans; sp += warps) {
+        uint4 v[kVecs];
+#pragma unroll
+        for (int i = 0; i < kVecs; ++i) {
+            const long long vi = (sp * kVecs + i) * 32 + lane;
+            v[i] = vi < vecs ? __ldg(x + vi) : make_uint4(0, 0, 0, 0);
+        }
+#pragma unroll
+        for (int i = 0; i < kVecs; ++i) {
+            const long long vi = (sp * kVecs + i) * 32 + lane;
+            const uint32_t w[4] = {v[i].x, v[i].y, v[i].z, v[i].w};
+            uint32_t m2 = 0;
+#pragma unroll
+            for (int k = 0; k < 4; ++k) m2 = __vmaxu2(m2, w[k] & 0x7FFF7FFFu);
+            uint32_t mx = max(m2 & 0xFFFFu, m2 >> 16);
+            mx = max(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
+            mx = max(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
+            const uint32_t ex = mx >> 7;                              // biased exponent of the maximum
+            const bool finite = ex < 255u;
+            const uint32_t s8 = !finite ? 255u : ex > 2u ? ex - 2u : 0u;
+            const float inv = __uint_as_float((254u - s8) << 23);     // 2^(127 - s8); unused when not finite
+            float y[8];
+#pragma unroll
+            for (int k = 0; k < 4; ++k) { y[2 * k] = bf16_lo(w[k]) * inv; y[2 * k + 1] = bf16_hi(w[k]) * inv; }
+            if (vi < vecs) Q[vi] = finite ? cvt8_e2m1(y) : 0u;
+            uint32_t word = s8;
+            if (words) {
+                word |= __shfl_down_sync(0xffffffffu, s8, 4) << 8;
+                word |= __shfl_down_sync(0xffffffffu, s8, 8) << 16;
+                word |= __shfl_down_sync(0xffffffffu, s8, 12) << 24;
+            }
+            if ((lane & (words ? 15 : 3)) == 0 && vi < vecs) {
+                const long long blk = vi >> 2;
+                const int r = static_cast<int>(blk / k32), j = static_cast<int>(blk - static_cast<long long>(r) * k32);
+                uint8_t* to = SF + (static_cast<size_t>(r >> 7) * k128 + (j >> 2)) * 512 + (r & 31) * 16 + ((r >> 5) & 3) * 4 + (j & 3);
+                if (words) *reinterpret_cast<uint32_t*>(to) = word;
+                else *to = static_cast<uint8_t>(s8);
+            }
+        }
+    }
+    // the layout's padding is zero: rows up to the next 128, and the slab bytes behind the last 32 K of a row
+    const int rows_up = (rows + 127) / 128 * 128, tail = k128 * 4 - k32;
+    const long long pad_rows = static_cast<long long>(rows_up - rows) * k128, pads = pad_rows + (tail ? rows : 0);
+    for (long long i = static_cast<long long>(blockIdx.x) * blockDim.x + threadIdx.x; i < pads;
+         i += static_cast<long long>(gridDim.x) * blockDim.x) {
+        const bool whole = i < pad_rows;
+        const int r = whole ? rows + static_cast<int>(i / k128) : static_cast<int>(i - pad_rows);
+        const int kb = whole ? static_cast<int>(i % k128) : k128 - 1;
+        uint8_t* to = SF + (static_cast<size_t>(r >> 7) * k128 + kb) * 512 + (r & 31) * 16 + ((r >> 5) & 3) * 4;
+        if (whole) *reinterpret_cast<uint32_t*>(to) = 0u;
+        else for (int j = 4 - tail; j < 4; ++j) to[j] = 0;
+    }
+}
+
 }  // namespace quant
 }  // namespace b200q
 
@@ -209,5 +282,29 @@ extern "C" int b200q_quant_rows_nvfp4(const void* X, void* Q, void* SF_blocked, 
     if (blocks < 1) blocks = 1;
     quant::quant_rows_nvfp4_kernel<<<static_cast<int>(blocks), 256, 0, static_cast<cudaStream_t>(stream)>>>(
         static_cast<const __nv_bfloat16*>(X), static_cast<uint32_t*>(Q), static_cast<uint32_t*>(SF_blocked), rows, cols, global_scale);
+    return cudaGetLastError();
+}
+
+extern "C" int b200q_quant_rows_mxfp4(const void* X, void* Q, void* SF_blocked, int rows, int cols, void* stream)
+{
+    using namespace b200q;
+    if (X == nullptr || Q == nullptr || SF_blocked == nullptr) return cudaErrorInvalidValue;
+    if (rows <= 0 || cols <= 0 || cols % 32 != 0) return cudaErrorInvalidValue;
+    if (!aligned16(X) || (reinterpret_cast<uintptr_t>(Q) & 3u) != 0 || !aligned16(SF_blocked)) return cudaErrorInvalidValue;
+    const int sms = num_sms();
+    if (sms <= 0) return cudaErrorInvalidDevice;
+    const __nv_bfloat16* x = static_cast<const __nv_bfloat16*>(X);
+    uint32_t* q = static_cast<uint32_t*>(Q);
+    uint8_t* sf = static_cast<uint8_t*>(SF_blocked);
+    cudaStream_t st = static_cast<cudaStream_t>(stream);
+    const long long vecs = static_cast<long long>(rows) * cols / 8;
+    // few vectors: one per thread, so that a decode batch is one pass of the machine; many: eight loads in flight a thread
+    if (vecs <= 256LL * sms) {
+        quant::quant_rows_mxfp4_kernel<1><<<static_cast<int>((vecs + 255) / 256), 256, 0, st>>>(x, q, sf, rows, cols / 32);
+    } else {
+        long long blocks = (vecs + 2047) / 2048;
+        if (blocks > sms * 8LL) blocks = sms * 8LL;
+        quant::quant_rows_mxfp4_kernel<8><<<static_cast<int>(blocks), 256, 0, st>>>(x, q, sf, rows, cols / 32);
+    }
     return cudaGetLastError();
 }

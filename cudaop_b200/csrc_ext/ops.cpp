@@ -230,6 +230,31 @@ torch::Tensor gemm_mxfp8(torch::Tensor a, torch::Tensor sfa, torch::Tensor b, to
     return c;
 }
 
+torch::Tensor gemm_mxfp4(torch::Tensor aq, torch::Tensor sfa, torch::Tensor bq, torch::Tensor sfb, bool blocked)
+{
+    check_cuda_2d(aq, "aq", {kU8}); check_cuda_2d(bq, "bq", {kU8});
+    const int64_t M = aq.size(0), N = bq.size(0), K = 2 * aq.size(1);
+    TORCH_CHECK_VALUE(aq.size(1) == bq.size(1) && K % 32 == 0, "shape mismatch (K must match and be a multiple of 32)");
+    const c10::cuda::CUDAGuard guard(aq.device());
+    auto c = out_like(aq, {M, N}, kBF16);
+    if (blocked) {
+        check_cuda_2d(sfa, "sfa", {kU8}, 1); check_cuda_2d(sfb, "sfb", {kU8}, 1);
+        same_device({&aq, &sfa, &bq, &sfb});
+        TORCH_CHECK_VALUE(sfa.numel() == (int64_t)b200q_mxfp8_sf_bytes((int)M, (int)K) && sfb.numel() == (int64_t)b200q_mxfp8_sf_bytes((int)N, (int)K),
+                          "blocked scale arrays have the wrong size");
+        raise_on(b200q_gemm_mxfp4_blocked(aq.data_ptr(), sfa.data_ptr(), bq.data_ptr(), sfb.data_ptr(), c.data_ptr(), (int)M, (int)N, (int)K,
+                                          stream_of(aq)), "b200q_gemm_mxfp4_blocked");
+        return c;
+    }
+    check_cuda_2d(sfa, "sfa", {kU8}); check_cuda_2d(sfb, "sfb", {kU8});
+    same_device({&aq, &sfa, &bq, &sfb});
+    TORCH_CHECK_VALUE(sfa.size(0) == M && sfa.size(1) == K / 32 && sfb.size(0) == N && sfb.size(1) == K / 32, "shape mismatch");
+    auto ws = out_like(aq, {(int64_t)b200q_gemm_mxfp4_workspace_bytes((int)M, (int)N, (int)K)}, kU8);
+    raise_on(b200q_gemm_mxfp4(aq.data_ptr(), sfa.data_ptr(), bq.data_ptr(), sfb.data_ptr(), c.data_ptr(), (int)M, (int)N, (int)K,
+                              ws.data_ptr(), stream_of(aq)), "b200q_gemm_mxfp4");
+    return c;
+}
+
 torch::Tensor gemm_sparse_fp8(torch::Tensor a_comp, torch::Tensor a_meta, torch::Tensor b, double scale_a, double scale_b)
 {
     check_cuda_2d(a_comp, "a_comp", {kU8, kE4M3}); check_cuda_2d(a_meta, "a_meta", {kU8}); check_cuda_2d(b, "b", {kU8, kE4M3});
@@ -267,6 +292,18 @@ std::tuple<torch::Tensor, torch::Tensor> quant_rows_nvfp4(torch::Tensor x, doubl
     return {q, sf};
 }
 
+std::tuple<torch::Tensor, torch::Tensor> quant_rows_mxfp4(torch::Tensor x)
+{
+    check_cuda_2d(x, "x", {kBF16});
+    TORCH_CHECK_VALUE(x.size(1) % 32 == 0, "the row length must be a multiple of 32");
+    const c10::cuda::CUDAGuard guard(x.device());
+    auto q = out_like(x, {x.size(0), x.size(1) / 2}, kU8);
+    auto sf = out_like(x, {(int64_t)b200q_mxfp8_sf_bytes((int)x.size(0), (int)x.size(1))}, kU8);
+    raise_on(b200q_quant_rows_mxfp4(x.data_ptr(), q.data_ptr(), sf.data_ptr(), (int)x.size(0), (int)x.size(1), stream_of(x)),
+             "b200q_quant_rows_mxfp4");
+    return {q, sf};
+}
+
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m)
 {
     m.def("gemm_fp8", &gemm_fp8, "FP8 E4M3 GEMM, per-tensor scales, bf16 out");
@@ -279,9 +316,11 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m)
     m.def("gemm_nvfp4", &gemm_nvfp4, "NVFP4 block-scaled GEMM");
     m.def("mxfp8_swizzle_sf", &mxfp8_swizzle_sf, "row-major UE8M0 scales -> blocked layout");
     m.def("gemm_mxfp8", &gemm_mxfp8, "MXFP8 block-scaled GEMM");
+    m.def("gemm_mxfp4", &gemm_mxfp4, "MXFP4 block-scaled GEMM");
     m.def("gemm_sparse_fp8", &gemm_sparse_fp8, "2:4-sparse FP8 GEMM");
     m.def("quant_rows_e4m3", &quant_rows_e4m3, "bf16 rows -> E4M3 + per-row fp32 scale");
     m.def("quant_rows_nvfp4", &quant_rows_nvfp4, "bf16 rows -> packed E2M1 + blocked UE4M3 scales");
+    m.def("quant_rows_mxfp4", &quant_rows_mxfp4, "bf16 rows -> packed E2M1 + blocked UE8M0 scales");
 }
 
 }  // namespace cudaop_b200

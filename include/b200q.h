@@ -125,6 +125,17 @@ int b200q_mxfp8_swizzle_sf(const void* sf_rowmajor, void* sf_blocked, int rows, 
 size_t b200q_mxfp8_sf_bytes(int rows, int K);
 int b200q_mxfp8_set_tile_n(int bn);     /* width of the B tile of the MXFP8 GEMM: 256 (default) or 192 */
 
+/* MXFP4 block-scaled GEMM: C(bf16) = ((A . 2^(sfa-127)) * (B . 2^(sfb-127))^T).  A[M,K/2], B[N,K/2]: two E2M1 per byte,
+ * low nibble = lower K (op/test/arch_primitives/ptx_mma_fp4.cu:49-53,120-130); scales as for MXFP8: one UE8M0 byte per 32
+ * consecutive K, row-major SFA[M,K/32], SFB[N,K/32], or blocked (b200q_mxfp8_swizzle_sf and b200q_mxfp8_sf_bytes serve both
+ * formats).  Requires K % 32 == 0 and 16-byte aligned pointers; any M, N >= 1.  `workspace`: caller-owned scratch of
+ * b200q_gemm_mxfp4_workspace_bytes(M,N,K) bytes for the blocked copies of both scale arrays. */
+int b200q_gemm_mxfp4(const void* A, const void* SFA, const void* B, const void* SFB, void* C, int M, int N, int K,
+                     void* workspace, void* stream);
+size_t b200q_gemm_mxfp4_workspace_bytes(int M, int N, int K);
+int b200q_gemm_mxfp4_blocked(const void* A, const void* SFA_blocked, const void* B, const void* SFB_blocked, void* C,
+                             int M, int N, int K, void* stream);
+
 /* 2:4 structured-sparse FP8 GEMM: C(bf16) = (expand(Acomp, Ameta) * B^T) * (scale_a * scale_b).
  * Acomp[M,K/2] E4M3 keeps the two retained values of every four in order; Ameta[M,K/8]: one
  * nibble per group of four = two ascending 2-bit positions, lower position in bits [1:0],
@@ -180,6 +191,13 @@ int b200q_quant_rows_e4m3(const void* X, void* Q, float* S, int rows, int cols, 
  * op/test/arch_primitives/ptx_mma_fp4.cu:55-65,120-144,293-309; the reference has no quantiser.  cols % 64 == 0,
  * global_scale > 0 (normally max|X| / (6 * 448)); X, SF 16-byte aligned, Q 4-byte aligned. */
 int b200q_quant_rows_nvfp4(const void* X, void* Q, void* SF_blocked, int rows, int cols, float global_scale, void* stream);
+
+/* bf16 rows -> MXFP4 operands of b200q_gemm_mxfp4_blocked: packed E2M1 Q[rows,cols/2] and one UE8M0 scale per 32 K in the
+ * blocked layout, SF_blocked of b200q_mxfp8_sf_bytes(rows, cols) bytes (padding written as zero).
+ * scale = 2^(floor(log2 max|blk|) - 2), at least 2^-127; q = e2m1_rn(x / scale), saturating at 6; a block that holds NaN or
+ * an infinity gets scale byte 255 (NaN) and zero codes.  Requires cols % 32 == 0, 16-byte aligned X and SF_blocked, 4-byte
+ * aligned Q. */
+int b200q_quant_rows_mxfp4(const void* X, void* Q, void* SF_blocked, int rows, int cols, void* stream);
 
 /* Sum all-reduce of the MLP's fp32 partial outputs over NVLink / NVSwitch, one call per rank, all
  * ranks at the same time: Y(bf16, on every rank) = sum_r P_r, P_r fp32 or (partial_is_bf16) bf16.  Replaces the in-place
