@@ -23,6 +23,7 @@ _lib = None
 __all__ = [
     "lib", "gemm_fp8", "gemm_i8", "gmm", "gmm_fp8", "GroupedFP8Weights", "gemm_fp8_rowcol", "gemm_fp8_swiglu", "gemm_w4a16", "gemm_nvfp4", "nvfp4_swizzle_sf",
     "gemm_mxfp8", "mxfp8_swizzle_sf", "quant_rows_nvfp4", "gemm_mxfp4", "quant_rows_mxfp4",
+    "paged_cache_write", "paged_cache_read", "paged_attention",
     "gemm_sparse_fp8", "quant_rows_e4m3", "status", "check_status", "set_wait_limit_ms", "WaitTimeout", "LIB_PATH",
 ]
 
@@ -34,6 +35,7 @@ _SIZE_T_FUNCS = {
     "b200q_gemm_mxfp8_workspace_bytes": [C.c_int, C.c_int, C.c_int],
     "b200q_gemm_mxfp4_workspace_bytes": [C.c_int, C.c_int, C.c_int],
     "b200q_gemm_nvfp4_static_max_bytes": [],
+    "b200q_paged_attention_workspace_bytes": [C.c_int],
     "b200q_allreduce_signal_bytes": [],
     "b200q_rank_barrier_signal_bytes": [],
     "b200q_fused_allreduce_flag_bytes": [],
@@ -70,6 +72,9 @@ _SIGNATURES = {
     "b200q_quant_rows_e4m3": [_VP, _VP, _VP, _I, _I, _VP],
     "b200q_quant_rows_nvfp4": [_VP, _VP, _VP, _I, _I, _F, _VP],
     "b200q_quant_rows_mxfp4": [_VP, _VP, _VP, _I, _I, _VP],
+    "b200q_paged_cache_write": [_VP] * 7 + [_I] * 3 + [C.c_longlong] * 4 + [_I] * 3 + [_VP],
+    "b200q_paged_cache_read": [_VP] * 8 + [_I] * 9 + [_VP],
+    "b200q_paged_attention": [_VP] * 10 + [_I] * 5 + [C.c_longlong] * 2 + [_I] * 5 + [_F] + [_I] * 3 + [_VP] * 2,
     "b200q_status": [_VP, _I],
     "b200q_set_wait_limit_ms": [_I, _I],
     "b200q_rank_barrier": [_VP, _I, _I, C.c_uint, C.c_uint, _VP],
@@ -137,7 +142,7 @@ def _check(t: torch.Tensor, name: str, dtypes, ndim: int) -> None:
 
 EXTENSION_OPS = ("gemm_fp8", "gemm_fp8_rowcol", "gemm_fp8_swiglu", "gemm_w4a16", "nvfp4_swizzle_sf", "gemm_nvfp4",
                  "mxfp8_swizzle_sf", "gemm_mxfp8", "gemm_sparse_fp8", "quant_rows_e4m3", "quant_rows_nvfp4", "gemm_i8", "gmm_fp8",
-                 "gemm_mxfp4", "quant_rows_mxfp4")
+                 "gemm_mxfp4", "quant_rows_mxfp4", "paged_cache_write", "paged_cache_read", "paged_attention")
 try:
     from . import _C                                    # noqa: F401
     _C_ERROR = None
@@ -266,6 +271,46 @@ def quant_rows_mxfp4(x: torch.Tensor):
     uint8): operands for :func:`gemm_mxfp4` with ``blocked=True``; also how weights are quantised, once.  A block of 32
     that holds NaN or an infinity gets the NaN scale, so its products are NaN."""
     return _ext().quant_rows_mxfp4(x)
+
+
+def paged_cache_write(k, v, slots, k_cache, v_cache, k_scale=None, v_scale=None) -> None:
+    """Writes the keys and values of new tokens into a paged cache, in place, quantising them if it is an E4M3 cache.
+
+    ``k``, ``v``: bf16 [tokens, kv_heads, head_dim]; slices of a fused projection's output are taken as they are (last
+    dimension contiguous, rows on 16-byte boundaries).  ``slots``: int64 [tokens], page * page_size + offset for each token;
+    a negative slot or one behind the cache is not written (padding).  The slots that are written must differ: of a slot
+    named twice, what stays is some mixture of the two tokens.
+    ``k_cache``, ``v_cache``: [pages, kv_heads, page_size, head_dim], bf16, or E4M3 (uint8 or float8_e4m3fn) with
+    ``k_scale``, ``v_scale`` fp32 [pages, kv_heads, page_size]: one scale per token and head, max|row| / 448, the rule of
+    :func:`quant_rows_e4m3` (a row with NaN or infinity gets the scale NaN).  page_size 16, 32, 64 or 128; head_dim 64 or 128."""
+    _ext().paged_cache_write(k, v, slots, k_cache, v_cache, k_scale, v_scale)
+
+
+def paged_cache_read(k_cache, v_cache, page_table, cu_kv, total: int, k_scale=None, v_scale=None, k_out=None, v_out=None):
+    """Sequences of a paged cache back to bf16: (k, v), each [total, kv_heads, head_dim], row ``cu_kv[b] + j`` being token j
+    of sequence b.  ``page_table``: int32 [seqs, max_pages]; ``cu_kv``: int32 [seqs + 1]; ``total``: rows of the output
+    (normally ``cu_kv[-1]``).  A token whose page number is not in the cache (say -1) reads as zero.  Rows of no sequence
+    are zero, or left as they are where ``k_out`` and ``v_out`` are given."""
+    return _ext().paged_cache_read(k_cache, v_cache, page_table, cu_kv, int(total), k_scale, v_scale, k_out, v_out)
+
+
+def paged_attention(q, k_cache, v_cache, page_table, cu_q, kv_lens, max_q: int, k_scale=None, v_scale=None, scale=None,
+                    causal: bool = True, window: int = 0, return_lse: bool = False, out=None):
+    """Attention of a chunk of new tokens per sequence over a paged cache that holds them already; bf16 like ``q``.
+
+    ``q``: bf16 [tokens, heads, head_dim] (slices of a fused projection's output are taken as they are), the chunks of the
+    sequences one after the other: rows ``cu_q[b]`` to ``cu_q[b + 1]`` (int32 [seqs + 1], from 0; lengths may differ, and be
+    zero).  They are the last tokens of the ``kv_lens[b]`` (int32 [seqs]) cached ones.  ``max_q``: a bound of the chunk
+    lengths (it chooses the kernel; a wrong one costs time only).  ``heads`` is a multiple of the cache's kv_heads; query
+    head h reads kv head h // (heads // kv_heads).  ``page_table``: int32 [seqs, max_pages]; a token whose page number is not in
+    the cache is left out.
+    A token at position p sees keys j <= p (``causal``; else all), and with a ``window`` only j > p - window.  A row
+    that sees nothing is zero.  ``scale``: of the scores, 1 / sqrt(head_dim) by default.
+    ``return_lse``: returns (out, lse), lse fp32 [tokens, heads] the natural log of the sum of exponentials (-inf for a row that
+    sees nothing).  Rows of no sequence are zero, or left as they are where ``out`` is given."""
+    o, lse = _ext().paged_attention(q, k_cache, v_cache, page_table, cu_q, kv_lens, int(max_q), k_scale, v_scale,
+                                    float(q.shape[-1] ** -0.5 if scale is None else scale), bool(causal), int(window), bool(return_lse), out)
+    return (o, lse) if return_lse else o
 
 
 def status(clear: bool = True) -> int:

@@ -1,0 +1,61 @@
+// Entry point of the attention over a paged cache: argument checks and the choice of kernel.
+#include "paged_attn.cuh"
+#include "../../include/b200q.h"
+
+namespace b200q {
+namespace paged {
+int page_shift_of(int page_size);        // paged_cache.cu
+}
+}
+
+extern "C" {
+
+size_t b200q_paged_attention_workspace_bytes(int head_dim)
+{
+    if (head_dim != 64 && head_dim != 128) return 0;
+    return b200q::paged::attn_split_workspace(head_dim);
+}
+
+int b200q_paged_attention(const void* q, const void* k_cache, const void* v_cache, const float* k_scale, const float* v_scale,
+                          const int* page_table, const int* cu_q, const int* kv_lens, void* out, float* lse, int seqs, int tokens,
+                          int heads, int kv_heads, int head_dim, long long q_stride, long long q_head_stride, int max_q, int max_pages,
+                          int num_pages, int page_size, int fp8, float softmax_scale, int causal, int window, int zero_rest,
+                          void* workspace, void* stream)
+{
+    using namespace b200q;
+    using namespace b200q::paged;
+    if (q == nullptr || k_cache == nullptr || v_cache == nullptr || page_table == nullptr || cu_q == nullptr || kv_lens == nullptr ||
+        out == nullptr || workspace == nullptr) return cudaErrorInvalidValue;
+    if (fp8 && (k_scale == nullptr || v_scale == nullptr)) return cudaErrorInvalidValue;
+    const int shift = page_shift_of(page_size);
+    if (seqs <= 0 || tokens <= 0 || heads <= 0 || kv_heads <= 0 || heads % kv_heads != 0 || max_q <= 0 || max_pages <= 0 ||
+        num_pages <= 0 || shift < 0 || (head_dim != 64 && head_dim != 128)) return cudaErrorInvalidValue;
+    if (window < 0 || (window > 0 && !causal) || !(softmax_scale == softmax_scale)) return cudaErrorInvalidValue;
+    if (q_stride % 8 || q_head_stride % 8 || !aligned16(q) || !aligned16(k_cache) || !aligned16(v_cache) || !aligned16(out) ||
+        !aligned16(workspace) || (fp8 && (!aligned16(k_scale) || !aligned16(v_scale)))) return cudaErrorInvalidValue;
+    // positions, rows of a chunk and rows of the cache are 32-bit numbers
+    const long long most = 0x7FFFFFFFll - 4096;
+    if ((static_cast<long long>(max_pages) << shift) > most || static_cast<long long>(tokens) * heads > most ||
+        ((static_cast<long long>(num_pages) * kv_heads) << shift) > most) return cudaErrorInvalidValue;
+    if (num_sms() <= 0) return cudaErrorInvalidDevice;
+
+    Args a{};
+    a.s.cu_q = cu_q; a.s.kv_lens = kv_lens; a.s.table = page_table;
+    a.s.seqs = seqs; a.s.tokens = tokens; a.s.heads = heads; a.s.kv_heads = kv_heads; a.s.group = heads / kv_heads;
+    a.s.max_pages = max_pages; a.s.page_shift = shift; a.s.num_pages = num_pages;
+    a.s.causal = causal != 0; a.s.window = window;
+    a.q = static_cast<const __nv_bfloat16*>(q); a.q_stride = q_stride; a.q_head = q_head_stride;
+    a.k_cache = k_cache; a.v_cache = v_cache; a.k_scale = k_scale; a.v_scale = v_scale;
+    a.out = static_cast<__nv_bfloat16*>(out); a.lse = lse;
+    a.scale_log2 = softmax_scale * 1.44269504088896341f;
+    a.max_q = max_q < tokens ? max_q : tokens;
+    a.zero_rest = zero_rest != 0;
+    a.status = status_ptr();
+    if (a.status == nullptr) return cudaErrorInvalidDevice;
+    const size_t open_bytes = static_cast<size_t>(2 * num_sms()) * sizeof(Open) / 16 * 16 + 16;
+    a.open = static_cast<Open*>(workspace);
+    a.part = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + open_bytes);
+    return attn_split(a, head_dim, fp8 != 0, static_cast<cudaStream_t>(stream));
+}
+
+}  // extern "C"

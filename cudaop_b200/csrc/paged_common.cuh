@@ -1,0 +1,161 @@
+// What the paged-cache operators share: the shape of a call, which keys a block of query rows sees, and how a persistent
+// grid divides the work of a ragged batch.
+//
+// Cache layout: [pages, kv_heads, page_size, head_dim] for keys and for values (bf16, or E4M3 bytes with one fp32 scale per
+// row in [pages, kv_heads, page_size]): the tokens of one page and head are one contiguous run, so a tile of keys is a few
+// boxes of a 2-D tensor map over rows, and a row is (page * kv_heads + head) * page_size + offset.
+#pragma once
+#include "common.cuh"
+
+namespace b200q {
+namespace paged {
+
+// One call of the attention.  The rows of a sequence's chunk of n tokens are ordered (token, head of the group), row
+// r = token * group + g, for each kv head: query heads that share keys share a tile.
+struct Shape {
+    const int* cu_q;          // [seqs + 1] first row of each sequence's chunk in q
+    const int* kv_lens;       // [seqs] cached tokens, the chunk included
+    const int* table;         // [seqs, max_pages]
+    int seqs, tokens, heads, kv_heads, group;
+    int max_pages, page_shift, num_pages;
+    int causal, window;       // window 0 = none; a window implies causal
+};
+
+// Lengths as the caller gave them, made safe: whatever the arrays hold, rows stay inside q and keys inside the table.
+struct Seq {
+    int q0, n, kv, cap;
+};
+__device__ __forceinline__ Seq load_seq(const Shape& s, int b)
+{
+    Seq q;
+    q.q0 = min(max(__ldg(s.cu_q + b), 0), s.tokens);
+    q.n = min(max(__ldg(s.cu_q + b + 1), q.q0), s.tokens) - q.q0;
+    q.kv = max(__ldg(s.kv_lens + b), 0);
+    q.cap = min(q.kv, s.max_pages << s.page_shift);
+    return q;
+}
+
+// Keys [lo, hi) that some row of block i (rows i * rm .. of the chunk) sees, and the tiles of kt keys that hold them.  A block
+// that sees nothing gets one empty tile: its rows are written (as zero) like any others.
+struct Range {
+    int lo, hi, tile0, tiles;
+};
+__device__ __forceinline__ Range block_range(const Shape& s, const Seq& q, int i, int rm, int kt)
+{
+    const int r0 = i * rm, r1 = min(q.n * s.group, r0 + rm);
+    const int first = q.kv - q.n + r0 / s.group, last = q.kv - q.n + (r1 - 1) / s.group;   // positions of the block's tokens
+    Range r;
+    r.hi = s.causal ? min(q.cap, last + 1) : q.cap;
+    r.lo = s.window > 0 ? max(0, first - s.window + 1) : 0;
+    if (r.lo >= r.hi) { r.lo = 0; r.hi = 0; }
+    r.tile0 = r.lo / kt;
+    r.tiles = max(1, (r.hi + kt - 1) / kt - r.tile0);
+    return r;
+}
+
+// The work of a call is the list of all tiles: sequence by sequence, kv head by kv head, row block by row block, tile by
+// tile.  CTA c of g (g at most W) takes the tiles [c * W / g, (c + 1) * W / g), whatever the lengths are: every CTA gets the same number, and a
+// long sequence is split over as many CTAs as it takes.  A block whose tiles lie in several CTAs leaves partial results
+// (running maximum, sum, unnormalised output), joined by the combine kernel in CTA order.
+struct Cursor {
+    int b, h, i;              // sequence, kv head, row block
+    int tile;                 // first tile (counted from the block's tile0) this CTA takes of the block
+    long long at, end;        // this CTA's tiles, as indices of the list; at == end: nothing left
+    long long total;          // length of the list
+    int ctas;                 // CTAs that have work: no more than there are tiles
+};
+
+// Whole CTA; `prefix` holds seqs 64-bit words in shared memory (free again after the call, which ends in a barrier).
+// `block_limit`: an upper bound of the row blocks of one sequence.
+__device__ __forceinline__ Cursor find_work(const Shape& s, int rm, int kt, long long* prefix, int block_limit, int cta, int ctas)
+{
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
+    if (block_limit <= 8) {                        // a thread per sequence
+        for (int b = threadIdx.x; b < s.seqs; b += blockDim.x) {
+            const Seq q = load_seq(s, b);
+            const int blocks = (q.n * s.group + rm - 1) / rm;
+            long long w = 0;
+            for (int i = 0; i < blocks; ++i) w += block_range(s, q, i, rm, kt).tiles;
+            prefix[b] = w * s.kv_heads;
+        }
+    } else {                                       // a warp per sequence
+        for (int b = warp; b < s.seqs; b += warps) {
+            const Seq q = load_seq(s, b);
+            const int blocks = (q.n * s.group + rm - 1) / rm;
+            long long w = 0;
+            for (int i = lane; i < blocks; i += 32) w += block_range(s, q, i, rm, kt).tiles;
+#pragma unroll
+            for (int o = 16; o > 0; o >>= 1) w += __shfl_xor_sync(0xffffffffu, w, o);
+            if (lane == 0) prefix[b] = w * s.kv_heads;
+        }
+    }
+    __syncthreads();
+    if (warp == 0) {                               // inclusive prefix sums
+        long long run = 0;
+        for (int b0 = 0; b0 < s.seqs; b0 += 32) {
+            long long v = b0 + lane < s.seqs ? prefix[b0 + lane] : 0;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const long long u = __shfl_up_sync(0xffffffffu, v, o);
+                if (lane >= o) v += u;
+            }
+            v += run;
+            if (b0 + lane < s.seqs) prefix[b0 + lane] = v;
+            run = __shfl_sync(0xffffffffu, v, 31);
+        }
+    }
+    __syncthreads();
+    const long long total = s.seqs > 0 ? prefix[s.seqs - 1] : 0;
+    Cursor c{};
+    c.total = total;
+    c.ctas = static_cast<int>(min(static_cast<long long>(ctas), total));
+    if (cta < c.ctas) {
+        const long long first = total * cta / c.ctas;
+        c.at = first;
+        c.end = total * (cta + 1) / c.ctas;
+        int lo = 0, hi = s.seqs - 1;               // first sequence whose inclusive prefix exceeds `first`
+        while (lo < hi) {
+            const int mid = (lo + hi) / 2;
+            if (prefix[mid] > first) hi = mid; else lo = mid + 1;
+        }
+        c.b = lo;
+        const long long before = lo > 0 ? prefix[lo - 1] : 0;
+        const long long per_head = (prefix[lo] - before) / s.kv_heads;
+        long long rem = first - before;
+        c.h = static_cast<int>(rem / per_head);
+        rem -= c.h * per_head;
+        const Seq q = load_seq(s, lo);
+        for (c.i = 0;; ++c.i) {
+            const int t = block_range(s, q, c.i, rm, kt).tiles;
+            if (rem < t) break;
+            rem -= t;
+        }
+        c.tile = static_cast<int>(rem);
+    }
+    __syncthreads();
+    return c;
+}
+
+// The next block after (b, h, i), called while tiles are left; sequences without rows are passed over.
+__device__ __forceinline__ void next_block(const Shape& s, Cursor& c, Seq& q, int rm)
+{
+    c.tile = 0;
+    if ((c.i + 1) * rm < q.n * s.group) { ++c.i; return; }
+    c.i = 0;
+    if (++c.h < s.kv_heads) return;
+    c.h = 0;
+    do { q = load_seq(s, ++c.b); } while (q.n == 0);
+}
+
+// The CTA that does tile t of the list.
+__device__ __forceinline__ int owner(const Cursor& c, long long t) { return static_cast<int>(((t + 1) * c.ctas - 1) / c.total); }
+
+// What a CTA leaves for the combine kernel: the block whose first tiles it did and whose last it did not.
+struct Open {
+    int token0;               // first row of the sequence's chunk in q
+    int r0, rows, h;          // the block
+    int last;                 // CTA that does the block's last tile; -1: nothing open
+};
+
+}  // namespace paged
+}  // namespace b200q

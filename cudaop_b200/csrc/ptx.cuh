@@ -709,6 +709,40 @@ __device__ __forceinline__ float ld_dsmem_f32(uint32_t cluster_addr)
     return v;
 }
 
+// ex2.approx.ftz.f32: 2^x (relative error about 2^-22; 2^-inf = 0)
+__device__ __forceinline__ float ex2(float x)
+{
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
+// ld.shared.v4 / v2: 16 / 8 bytes from a shared-window offset
+__device__ __forceinline__ uint4 ld_shared_v4(uint32_t smem_addr)
+{
+    uint4 v;
+    asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(smem_addr) : "memory");
+    return v;
+}
+__device__ __forceinline__ uint2 ld_shared_v2(uint32_t smem_addr)
+{
+    uint2 v;
+    asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(smem_addr) : "memory");
+    return v;
+}
+__device__ __forceinline__ float ld_shared_f32(uint32_t smem_addr)
+{
+    float v;
+    asm volatile("ld.shared.f32 %0, [%1];" : "=f"(v) : "r"(smem_addr) : "memory");
+    return v;
+}
+
+// bar.sync on a named barrier for `threads` threads
+__device__ __forceinline__ void named_barrier(int id, int threads)
+{
+    asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(threads) : "memory");
+}
+
 __device__ __forceinline__ void st_release_sys(uint32_t* p, uint32_t v)
 {
     asm volatile("st.release.sys.global.u32 [%0], %1;" ::"l"(p), "r"(v) : "memory");

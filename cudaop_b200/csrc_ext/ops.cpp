@@ -12,6 +12,8 @@
 #include <c10/cuda/CUDAException.h>
 #include <c10/cuda/CUDAGuard.h>
 
+#include <algorithm>
+#include <cmath>
 #include <tuple>
 #include <vector>
 
@@ -304,6 +306,159 @@ std::tuple<torch::Tensor, torch::Tensor> quant_rows_mxfp4(torch::Tensor x)
     return {q, sf};
 }
 
+// ---------------------------------------------------------------------------------------------- paged cache
+
+struct CacheArgs {
+    int pages, kv_heads, page, dim, fp8;
+    const float *ks, *vs;
+};
+
+void same_place(const torch::Tensor& ref, const torch::Tensor& t, const char* name)
+{
+    TORCH_CHECK_VALUE(t.device() == ref.device(), name, " must be on the same device as the cache");
+}
+
+// [pages, kv_heads, page_size, head_dim] in bf16, or in E4M3 with fp32 scales [pages, kv_heads, page_size]
+CacheArgs check_cache(const torch::Tensor& kc, const torch::Tensor& vc, const c10::optional<torch::Tensor>& ks,
+                      const c10::optional<torch::Tensor>& vs)
+{
+    check_cuda_2d(kc, "k_cache", {kBF16, kU8, kE4M3}, 4); check_cuda_2d(vc, "v_cache", {kBF16, kU8, kE4M3}, 4);
+    same_place(kc, vc, "v_cache");
+    TORCH_CHECK_VALUE(kc.scalar_type() == vc.scalar_type() && kc.sizes() == vc.sizes(), "k_cache and v_cache must have the same dtype and shape");
+    CacheArgs c{};
+    const int64_t page = kc.size(2), dim = kc.size(3);
+    TORCH_CHECK_VALUE(kc.size(0) > 0 && kc.size(1) > 0, "the cache is empty");
+    TORCH_CHECK_VALUE(page == 16 || page == 32 || page == 64 || page == 128, "page_size must be 16, 32, 64 or 128, got ", num(page));
+    TORCH_CHECK_VALUE(dim == 64 || dim == 128, "head_dim must be 64 or 128, got ", num(dim));
+    TORCH_CHECK_VALUE(kc.size(0) <= (INT32_MAX - 4096) / (kc.size(1) * page), "the cache has too many rows for 32-bit row numbers");
+    c.pages = (int)kc.size(0); c.kv_heads = (int)kc.size(1); c.page = (int)page; c.dim = (int)dim;
+    c.fp8 = kc.scalar_type() != kBF16;
+    TORCH_CHECK_VALUE(ks.has_value() == (bool)c.fp8 && vs.has_value() == (bool)c.fp8,
+                      "k_scale and v_scale belong to an E4M3 cache, and to no other");
+    if (c.fp8) {
+        check_cuda_2d(*ks, "k_scale", {kF32}, 3); check_cuda_2d(*vs, "v_scale", {kF32}, 3);
+        same_place(kc, *ks, "k_scale"); same_place(kc, *vs, "v_scale");
+        TORCH_CHECK_VALUE(ks->sizes() == kc.sizes().slice(0, 3) && vs->sizes() == kc.sizes().slice(0, 3),
+                          "the scales must be [pages, kv_heads, page_size]");
+        c.ks = ks->data_ptr<float>(); c.vs = vs->data_ptr<float>();
+    }
+    return c;
+}
+
+// rows [tokens, heads, dim] in bf16 that may be slices of a wider tensor: the last dimension contiguous, the others any
+// multiple of 16 bytes apart
+void check_rows(const torch::Tensor& t, const char* name, const torch::Tensor& kc)
+{
+    TORCH_CHECK_VALUE(t.dim() == 3, name, " must have 3 dimensions, got ", num(t.dim()));
+    TORCH_CHECK_VALUE(t.is_cuda(), name, " must be a CUDA tensor");
+    same_place(kc, t, name);
+    TORCH_CHECK_VALUE(t.scalar_type() == kBF16, name, " has dtype ", c10::toString(t.scalar_type()), ", which this operator does not take");
+    TORCH_CHECK_VALUE(t.size(2) == kc.size(3), name, " must have the cache's head_dim");
+    TORCH_CHECK_VALUE(t.size(2) == 1 || t.stride(2) == 1, "the last dimension of ", name, " must be contiguous");
+    TORCH_CHECK_VALUE(t.stride(0) % 8 == 0 && t.stride(1) % 8 == 0 && reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0,
+                      "the rows of ", name, " must start on 16-byte boundaries");
+}
+
+void check_index(const torch::Tensor& t, const char* name, c10::ScalarType dt, int64_t dim, const torch::Tensor& kc)
+{
+    check_cuda_2d(t, name, {dt}, dim);
+    same_place(kc, t, name);
+}
+
+void paged_cache_write(torch::Tensor k, torch::Tensor v, torch::Tensor slots, torch::Tensor k_cache, torch::Tensor v_cache,
+                       c10::optional<torch::Tensor> k_scale, c10::optional<torch::Tensor> v_scale)
+{
+    const CacheArgs c = check_cache(k_cache, v_cache, k_scale, v_scale);
+    check_rows(k, "k", k_cache); check_rows(v, "v", k_cache);
+    TORCH_CHECK_VALUE(k.size(1) == c.kv_heads && v.sizes() == k.sizes(), "k and v must be [tokens, kv_heads, head_dim]");
+    check_index(slots, "slots", c10::ScalarType::Long, 1, k_cache);
+    TORCH_CHECK_VALUE(slots.numel() == k.size(0), "slots must have one entry per token");
+    TORCH_CHECK_VALUE(k.size(0) <= INT32_MAX - 4096, "too many tokens");
+    if (k.size(0) == 0) return;
+    const c10::cuda::CUDAGuard guard(k_cache.device());
+    raise_on(b200q_paged_cache_write(k.data_ptr(), v.data_ptr(), reinterpret_cast<const long long*>(slots.data_ptr<int64_t>()), k_cache.data_ptr(),
+                                     v_cache.data_ptr(), const_cast<float*>(c.ks), const_cast<float*>(c.vs), (int)k.size(0), c.kv_heads, c.dim,
+                                     k.stride(0), v.stride(0), k.stride(1), v.stride(1), c.pages, c.page, c.fp8, stream_of(k_cache)),
+             "b200q_paged_cache_write");
+}
+
+std::tuple<torch::Tensor, torch::Tensor> paged_cache_read(torch::Tensor k_cache, torch::Tensor v_cache, torch::Tensor page_table,
+                                                          torch::Tensor cu_kv, int64_t total, c10::optional<torch::Tensor> k_scale,
+                                                          c10::optional<torch::Tensor> v_scale, c10::optional<torch::Tensor> k_out,
+                                                          c10::optional<torch::Tensor> v_out)
+{
+    const CacheArgs c = check_cache(k_cache, v_cache, k_scale, v_scale);
+    check_index(page_table, "page_table", kI32, 2, k_cache); check_index(cu_kv, "cu_kv", kI32, 1, k_cache);
+    const int64_t seqs = page_table.size(0);
+    TORCH_CHECK_VALUE(cu_kv.numel() == seqs + 1, "cu_kv must have one entry per sequence and one more");
+    TORCH_CHECK_VALUE(seqs <= INT32_MAX - 4096 && page_table.size(1) <= INT32_MAX - 4096, "page_table is too large");
+    TORCH_CHECK_VALUE(total >= 0 && total <= INT32_MAX - 4096, "total must not be negative, nor pass 32 bits");
+    TORCH_CHECK_VALUE(k_out.has_value() == v_out.has_value(), "k_out and v_out go together");
+    const c10::cuda::CUDAGuard guard(k_cache.device());
+    torch::Tensor k, v;
+    if (k_out.has_value()) {
+        check_cuda_2d(*k_out, "k_out", {kBF16}, 3); check_cuda_2d(*v_out, "v_out", {kBF16}, 3);
+        same_place(k_cache, *k_out, "k_out"); same_place(k_cache, *v_out, "v_out");
+        TORCH_CHECK_VALUE(k_out->size(0) == total && k_out->size(1) == c.kv_heads && k_out->size(2) == c.dim && v_out->sizes() == k_out->sizes(),
+                          "k_out and v_out must be [total, kv_heads, head_dim]");
+        k = *k_out; v = *v_out;
+    } else {
+        k = out_like(k_cache, {total, c.kv_heads, c.dim}, kBF16);
+        v = out_like(k_cache, {total, c.kv_heads, c.dim}, kBF16);
+    }
+    if (total == 0) return {k, v};
+    if (seqs == 0 || page_table.size(1) == 0) {                    // no token has a page
+        if (!k_out.has_value() || seqs > 0) { k.zero_(); v.zero_(); }
+        return {k, v};
+    }
+    raise_on(b200q_paged_cache_read(k_cache.data_ptr(), v_cache.data_ptr(), c.ks, c.vs, page_table.data_ptr<int>(), cu_kv.data_ptr<int>(),
+                                    k.data_ptr(), v.data_ptr(), (int)seqs, (int)total, c.kv_heads, c.dim, (int)page_table.size(1), c.pages, c.page,
+                                    c.fp8, !k_out.has_value(), stream_of(k_cache)), "b200q_paged_cache_read");
+    return {k, v};
+}
+
+std::tuple<torch::Tensor, c10::optional<torch::Tensor>> paged_attention(
+    torch::Tensor q, torch::Tensor k_cache, torch::Tensor v_cache, torch::Tensor page_table, torch::Tensor cu_q, torch::Tensor kv_lens,
+    int64_t max_q, c10::optional<torch::Tensor> k_scale, c10::optional<torch::Tensor> v_scale, double scale, bool causal, int64_t window,
+    bool return_lse, c10::optional<torch::Tensor> out)
+{
+    const CacheArgs c = check_cache(k_cache, v_cache, k_scale, v_scale);
+    check_rows(q, "q", k_cache);
+    const int64_t tokens = q.size(0), heads = q.size(1), seqs = kv_lens.numel();
+    TORCH_CHECK_VALUE(heads > 0 && heads % c.kv_heads == 0, "the heads of q must be a multiple of the cache's kv_heads");
+    check_index(page_table, "page_table", kI32, 2, k_cache); check_index(cu_q, "cu_q", kI32, 1, k_cache);
+    check_index(kv_lens, "kv_lens", kI32, 1, k_cache);
+    TORCH_CHECK_VALUE(page_table.size(0) == seqs && cu_q.numel() == seqs + 1, "page_table, cu_q and kv_lens must agree on the number of sequences");
+    TORCH_CHECK_VALUE(seqs > 0 && page_table.size(1) > 0, "there must be a sequence and a page");
+    TORCH_CHECK_VALUE(max_q > 0, "max_q must be positive");
+    TORCH_CHECK_VALUE(window >= 0 && (window == 0 || causal), "window must not be negative, and needs causal");
+    TORCH_CHECK_VALUE(std::isfinite(scale), "scale must be finite");
+    TORCH_CHECK_VALUE(tokens * heads <= INT32_MAX - 4096 && page_table.size(1) <= (INT32_MAX - 4096) / c.page && seqs <= INT32_MAX - 4096,
+                      "sizes pass 32 bits");
+    const c10::cuda::CUDAGuard guard(k_cache.device());
+    const bool given = out.has_value();
+    torch::Tensor o;
+    if (given) {
+        check_cuda_2d(*out, "out", {kBF16}, 3);
+        same_place(k_cache, *out, "out");
+        TORCH_CHECK_VALUE(out->sizes() == q.sizes(), "out must have the shape of q");
+        o = *out;
+    } else {
+        o = out_like(k_cache, {tokens, heads, c.dim}, kBF16);
+    }
+    c10::optional<torch::Tensor> lse;
+    if (return_lse) lse = given ? torch::full({tokens, heads}, -INFINITY, k_cache.options().dtype(kF32)) : out_like(k_cache, {tokens, heads}, kF32);
+    if (tokens == 0) return {o, lse};
+    auto ws = out_like(k_cache, {(int64_t)b200q_paged_attention_workspace_bytes(c.dim)}, kU8);
+    raise_on(b200q_paged_attention(q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), c.ks, c.vs, page_table.data_ptr<int>(),
+                                   cu_q.data_ptr<int>(), kv_lens.data_ptr<int>(), o.data_ptr(), lse.has_value() ? lse->data_ptr<float>() : nullptr,
+                                   (int)seqs, (int)tokens, (int)heads, c.kv_heads, c.dim, q.stride(0), q.stride(1),
+                                   (int)std::min<int64_t>(max_q, tokens), (int)page_table.size(1), c.pages, c.page, c.fp8, (float)scale, causal,
+                                   (int)std::min<int64_t>(window, INT32_MAX / 2), !given, ws.data_ptr(), stream_of(k_cache)),
+             "b200q_paged_attention");
+    return {o, lse};
+}
+
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m)
 {
     m.def("gemm_fp8", &gemm_fp8, "FP8 E4M3 GEMM, per-tensor scales, bf16 out");
@@ -321,6 +476,9 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m)
     m.def("quant_rows_e4m3", &quant_rows_e4m3, "bf16 rows -> E4M3 + per-row fp32 scale");
     m.def("quant_rows_nvfp4", &quant_rows_nvfp4, "bf16 rows -> packed E2M1 + blocked UE4M3 scales");
     m.def("quant_rows_mxfp4", &quant_rows_mxfp4, "bf16 rows -> packed E2M1 + blocked UE8M0 scales");
+    m.def("paged_cache_write", &paged_cache_write, "new tokens' keys and values into a paged cache");
+    m.def("paged_cache_read", &paged_cache_read, "sequences of a paged cache back to bf16");
+    m.def("paged_attention", &paged_attention, "attention of a chunk of new tokens over a paged cache");
 }
 
 }  // namespace cudaop_b200

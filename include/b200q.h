@@ -145,6 +145,40 @@ int b200q_gemm_mxfp4_blocked(const void* A, const void* SFA_blocked, const void*
 int b200q_gemm_sp24_fp8(const void* Acomp, const void* Ameta, const void* B, void* C, int M, int N, int K,
                         float scale_a, float scale_b, void* stream);
 
+/* A paged cache of keys and values.  k_cache, v_cache: [num_pages, kv_heads, page_size, head_dim], bf16 (fp8 == 0) or E4M3
+ * bytes (fp8 != 0) with k_scale, v_scale fp32 [num_pages, kv_heads, page_size]; page_size 16, 32, 64 or 128, head_dim 64 or 128,
+ * num_pages * kv_heads * page_size below 2^31.  (The reference has no cache; its scale rule for rows is that of
+ * b200q_quant_rows_e4m3.)  Strides are in elements, multiples of 8; pointers to rows and caches are 16-byte aligned.
+ *
+ * Write: row (token, head) of k at token * k_stride + head * k_head_stride goes to slot slots[token] = page * page_size +
+ * offset (DEVICE int64; slots outside the cache are skipped, those written must differ).  E4M3: s = max|row| / 448 (1 for a
+ * zero row), byte = e4m3_rn(x * (1 / s)); a row with NaN or infinity gets the scale NaN and zero bytes. */
+int b200q_paged_cache_write(const void* k, const void* v, const long long* slots, void* k_cache, void* v_cache, float* k_scale,
+                            float* v_scale, int tokens, int kv_heads, int head_dim, long long k_stride, long long v_stride,
+                            long long k_head_stride, long long v_head_stride, int num_pages, int page_size, int fp8, void* stream);
+
+/* Read back: k, v [total, kv_heads, head_dim] bf16, row cu_kv[b] + j = token j of sequence b (page_table: DEVICE int32
+ * [seqs, max_pages], cu_kv: DEVICE int32 [seqs + 1]).  Tokens on pages outside the cache read as zero; rows of no
+ * sequence are zeroed (zero_rest != 0) or left. */
+int b200q_paged_cache_read(const void* k_cache, const void* v_cache, const float* k_scale, const float* v_scale,
+                           const int* page_table, const int* cu_kv, void* k, void* v, int seqs, int total, int kv_heads, int head_dim,
+                           int max_pages, int num_pages, int page_size, int fp8, int zero_rest, void* stream);
+
+/* Attention of a chunk of new tokens per sequence over the cache: out[tokens, heads, head_dim] (bf16) = softmax(scale q k^T) v, and
+ * optionally lse[tokens, heads] (fp32, natural log; NULL for none).  The rows cu_q[b] .. cu_q[b + 1] of q (DEVICE int32
+ * [seqs + 1]) are the last tokens of the kv_lens[b] (DEVICE int32 [seqs]) cached ones; the token at position p sees keys
+ * j <= p (causal != 0), and j > p - window (window > 0, needs causal); rows that see nothing are zero, lse -inf.  max_q: a
+ * bound of the chunk lengths (speed only).  Tokens on pages outside the cache are left out.  Rows of no sequence are zeroed
+ * (zero_rest != 0) or left.  Row (token, head) of q is at token * q_stride + head * q_head_stride elements.  `workspace`:
+ * caller-owned scratch of b200q_paged_attention_workspace_bytes(head_dim) bytes, 16-byte aligned, no contents needed, not to be
+ * shared by calls that may overlap. */
+int b200q_paged_attention(const void* q, const void* k_cache, const void* v_cache, const float* k_scale, const float* v_scale,
+                          const int* page_table, const int* cu_q, const int* kv_lens, void* out, float* lse, int seqs, int tokens,
+                          int heads, int kv_heads, int head_dim, long long q_stride, long long q_head_stride, int max_q, int max_pages,
+                          int num_pages, int page_size, int fp8, float softmax_scale, int causal, int window, int zero_rest,
+                          void* workspace, void* stream);
+size_t b200q_paged_attention_workspace_bytes(int head_dim);
+
 /* Tuning knobs.  Every b200q_*_set_* function changes a PROCESS-WIDE setting read by later calls on any
  * device; they are not synchronised with calls in flight on other host threads — set them once at
  * start-up, before the threads that issue work are started.  All of them default to the measured best. */
