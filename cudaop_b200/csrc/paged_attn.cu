@@ -5,6 +5,7 @@
 namespace b200q {
 namespace paged {
 int page_shift_of(int page_size);        // paged_cache.cu
+size_t open_bytes() { return (static_cast<size_t>(attn_split_ctas()) * sizeof(Open) + 15) / 16 * 16; }
 }
 }
 
@@ -13,7 +14,7 @@ extern "C" {
 size_t b200q_paged_attention_workspace_bytes(int head_dim)
 {
     if (head_dim != 64 && head_dim != 128) return 0;
-    return b200q::paged::attn_split_workspace(head_dim);
+    return b200q::paged::open_bytes() + b200q::paged::attn_split_part_bytes(head_dim);
 }
 
 int b200q_paged_attention(const void* q, const void* k_cache, const void* v_cache, const float* k_scale, const float* v_scale,
@@ -52,9 +53,8 @@ int b200q_paged_attention(const void* q, const void* k_cache, const void* v_cach
     a.zero_rest = zero_rest != 0;
     a.status = status_ptr();
     if (a.status == nullptr) return cudaErrorInvalidDevice;
-    const size_t open_bytes = static_cast<size_t>(2 * num_sms()) * sizeof(Open) / 16 * 16 + 16;
     a.open = static_cast<Open*>(workspace);
-    a.part = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + open_bytes);
+    a.part = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + open_bytes());
     return attn_split(a, head_dim, fp8 != 0, static_cast<cudaStream_t>(stream));
 }
 

@@ -25,12 +25,8 @@ struct Args {
 };
 
 int attn_split(const Args& a, int head_dim, bool fp8, cudaStream_t stream);
-size_t attn_split_workspace(int head_dim);
-
-__device__ __forceinline__ float max_nan4(float a, float b, float c, float d)
-{
-    return ptx::max_nan(ptx::max_nan(a, b), ptx::max_nan(c, d));
-}
+int attn_split_ctas();                       // the most CTAs a launch uses
+size_t attn_split_part_bytes(int head_dim);  // the most its parts take
 
 // natural log of sum_j e^(scale * q.k_j), from the maximum in units of log2 and the sum of 2^(x - max); -inf for no keys
 __device__ __forceinline__ float lse_of(float m, float l)

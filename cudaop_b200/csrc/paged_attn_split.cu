@@ -1,18 +1,25 @@
 // Attention of a chunk of new tokens over a paged cache, for few rows per kv head (decode, drafted tokens): the split-KV
-// kernel and the kernel that joins its parts.
+// kernel.
 //
 //   o[r,:] = sum_j p_j v_j / sum_j p_j,  p_j = 2^(x_j - m),  x_j = scale * log2(e) * (q_r . k_j),  m = max_j x_j
-// over the keys j that row r sees.  An E4M3 cache is never dequantised as such: the bytes become bf16 exactly (see e4m3x2 below),
-// a key's scale multiplies the 32-bit product q.k and a value's scale multiplies p before it is rounded to bf16 for the second
-// product.  That rounding of p (half a step, 2^-9 of a value's share) is the only one besides the output's; sums, maxima and
-// accumulators are 32-bit.
+// over the keys j that row r sees.
 //
-// Bound by the bytes of the cache: with 16 rows the tensor work per byte is small, so the design is one pass over the keys at
-// HBM rate.  A CTA is a producer warp that fills a ring of 64-key tiles by TMA (one box per page and tensor; the
-// page table is read a tile ahead) and four consumer warps of 16 keys each: their softmax states are independent, so a tile needs no
-// barrier but the ring's, and they meet once per block of rows.  m16n8k16 products with the rows as the 16 side; the contraction
-// order over head_dim (and the order of output columns) is permuted so that every shared-memory read is a conflict-free
-// 16 (or 8) byte load of consecutive elements.  The work is divided over the persistent grid by tiles (paged_common.cuh).
+// Bound by the bytes of the cache: one pass over the keys, meant to run at HBM rate.  A CTA is a producer warp that fills a ring of
+// 64-key tiles by TMA (one box per page and tensor; the page table is read a tile ahead) and four consumer warps of 16
+// keys each: their softmax states are independent, so a tile needs no barrier but the ring's, and they meet once per block of rows.
+// The products are computed transposed, keys (then head_dim) on the 16 side of m16n8k16 and 8 rows on its narrow side: with 8
+// query heads per kv head a decode step fills it exactly (rows on the 16 side left half of the products, of the softmax
+// and of the accumulator registers to rows that do not exist: 571 instructions per 16 keys of 128 against about 200, and
+// 247 us against 149 us for 48 sequences of 1 to 16 thousand tokens, 8 kv heads, E4M3).  Between the two products the 8x8 blocks of p are
+// transposed in registers (movmatrix).  The order of the contraction over head_dim, and of the output columns, is permuted so that
+// every shared-memory read is a conflict-free 16 (or 8) byte load of consecutive elements.
+//
+// Precision.  An E4M3 cache is never rounded again: the bytes become fp16 exactly, a key's scale multiplies the 32-bit
+// product q.k, and a value's scale multiplies p.  The fp16 operands are kept in range by powers of two: a row of q is divided
+// by that of its largest element (an element 2^15 below it starts to lose bits that are below those of the 32-bit sum), and p * scale by that of the largest
+// scale seen so far, which is a running maximum like m.  So p keeps 11 bits.  A bf16 cache needs bf16 operands, which would leave p 8
+// bits; it is split in two (its rounding and the rest) and the second product runs twice, which costs nothing here.
+// Sums, maxima and accumulators are 32-bit.  The work is divided over the persistent grid by tiles (paged_common.cuh).
 #include "paged_common.cuh"
 #include "paged_attn.cuh"
 #include "ptx.cuh"
@@ -21,10 +28,13 @@ namespace b200q {
 namespace paged {
 namespace split {
 
-constexpr int kRows = 16, kTile = 64, kConsumers = 4, kThreads = 32 * (kConsumers + 1);
+constexpr int kTile = 64, kConsumers = 4, kThreads = 32 * (kConsumers + 1);
 
-template <int D, bool FP8>
+// NT: groups of 8 rows per block
+template <int D, bool FP8, int NT>
 struct Cfg {
+    static constexpr int kRows = 8 * NT;
+    static constexpr int kCtasPerSm = NT == 1 ? 3 : 2;
     static constexpr int kRowBytes = FP8 ? D : 2 * D;
     static constexpr int kBoxBytes = kRowBytes < 128 ? kRowBytes : 128;       // inner extent of a box = swizzle span
     static constexpr int kHalves = kRowBytes / kBoxBytes;
@@ -33,28 +43,16 @@ struct Cfg {
     static constexpr int kScaleBytes = FP8 ? kTile * 4 : 0;
     static constexpr int kStageBytes = (2 * kTensorBytes + 2 * kScaleBytes + 1023) / 1024 * 1024;
     static constexpr int kJoinBytes = kRows * D * 4;                          // one warp's accumulators
-    static constexpr int kStages = (112 * 1024 - 2048 - kJoinBytes) / kStageBytes < 8 ? (112 * 1024 - 2048 - kJoinBytes) / kStageBytes : 8;
+    static constexpr int kBudget = 227 * 1024 / kCtasPerSm - 1024 - 3 * 1024 - kJoinBytes;
+    static constexpr int kStages = kBudget / kStageBytes < 8 ? kBudget / kStageBytes : 8;
+    static_assert(kStages >= 2, "ring");
     static constexpr int kStateBytes = kConsumers * kRows * 8;                // running maximum and sum per warp and row
     static constexpr int kSmemBytes = 1024 + kStages * kStageBytes + kJoinBytes + kStateBytes + kStages * (8 + 16);
-    static constexpr int kSteps = D / 16;                                     // k-steps of q.k
-    static constexpr int kCols = D / 8;                                       // 8-column groups of the output
+    static constexpr int kSteps = D / 16;                                     // k-steps of q.k, and 16-column groups of the output
 };
 
-// Two E4M3 bytes, in bits 8..15 and 24..31 of x, as two bf16, exactly: sign and the seven exponent and mantissa bits go where
-// bf16 has them, which reads as the value times 2^-120 (the exponent biases are 7 and 127; subnormals included), and one
-// exact product puts that right.  NaN bytes do not occur (the write kernel stores none).
-__device__ __forceinline__ uint32_t e4m3x2(uint32_t x)
-{
-    const uint32_t t = (x & 0x80008000u) | ((x >> 4) & 0x07F007F0u);
-    __nv_bfloat162 v, c;
-    *reinterpret_cast<uint32_t*>(&v) = t;
-    *reinterpret_cast<uint32_t*>(&c) = 0x7B807B80u;                            // 2^120
-    v = __hmul2(v, c);
-    return *reinterpret_cast<uint32_t*>(&v);
-}
-
-// The row r of the block as its 16-bit elements in the order the products take them: k-step s gives thread c = lane % 4 the
-// four consecutive elements that follow d0(s, c).
+// The row of q as 16-bit elements in the order the products take them: k-step s gives thread c = lane % 4 the four
+// consecutive elements that follow q_element(s, c).
 template <int D, bool FP8>
 __device__ __forceinline__ int q_element(int s, int c)
 {
@@ -62,7 +60,7 @@ __device__ __forceinline__ int q_element(int s, int c)
     return (s >> 2) * 64 + (2 * c + ((s >> 1) & 1)) * 8 + 4 * (s & 1);
 }
 
-// bytes [16 * chunk, +16) of row `row` of a tile half whose rows are kBox bytes, 128- (64-) byte swizzle
+// byte `byte` of row `row` of a tile half whose rows are kBox bytes, 128- (64-) byte swizzle
 template <int kBox>
 __device__ __forceinline__ uint32_t swizzled(uint32_t base, int row, int byte)
 {
@@ -70,11 +68,26 @@ __device__ __forceinline__ uint32_t swizzled(uint32_t base, int row, int byte)
     return base + (a ^ (kBox == 128 ? (a >> 3) & 0x70u : (a >> 3) & 0x30u));
 }
 
-template <int D, bool FP8>
-__global__ void __launch_bounds__(kThreads, 2)
+template <bool FP8>
+__device__ __forceinline__ void mma(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1)
+{
+    if (FP8) ptx::mma_f16_16816(d, a0, a1, a2, a3, b0, b1);
+    else ptx::mma_bf16_16816(d, a0, a1, a2, a3, b0, b1);
+}
+
+__device__ __forceinline__ uint32_t pack_f16x2(float lo, float hi)
+{
+    const __half2 v = __floats2half2_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t*>(&v);
+}
+__device__ __forceinline__ float pow2_of_field(uint32_t e) { return __uint_as_float(e << 23); }      // 2^(e - 127), 1 <= e <= 254
+
+template <int D, bool FP8, int NT>
+__global__ void __launch_bounds__(kThreads, NT == 1 ? 3 : 2)
 attn_split_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV, const Args a)
 {
-    using C = Cfg<D, FP8>;
+    using C = Cfg<D, FP8, NT>;
+    constexpr int kRows = C::kRows;
     extern __shared__ uint8_t smem_raw[];
     const uint32_t raw = ptx::smem_u32(smem_raw);
     const uint32_t ring = (raw + 1023u) & ~1023u;
@@ -166,6 +179,7 @@ attn_split_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
     }
 
     // ---------------------------------------------------------------------------------------------- consumers
+    // lane 4g + cc: keys g and g + 8 of the warp's 16, rows 8 * nt + 2cc + {0, 1} (and, of the output, columns of chunk g)
     const int g = lane >> 2, cc = lane & 3;
     int stage = 0;
     uint32_t phase = 0;
@@ -174,31 +188,59 @@ attn_split_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
         const Range r = block_range(s, q, c.i, kRows, kTile);
         const int todo = static_cast<int>(min(static_cast<long long>(r.tiles - c.tile), c.end - c.at));
         const int r0 = c.i * kRows, rows = min(kRows, q.n * s.group - r0);
-        // this thread's two rows: where they stand in q, and their positions
-        int pos[2];
-        const __nv_bfloat16* qp[2];
+        // q: this thread holds row 8 * nt + g; what belongs to rows 2cc + {0, 1} comes from the lanes that hold them
+        uint32_t qb[NT][C::kSteps][2];
+        int pos[NT][2];
+        float row_scale[NT][2];                                      // softmax scale (and, for fp16 rows, their power of two)
+        int pos_lo = 0, pos_hi = 0;
 #pragma unroll
-        for (int u = 0; u < 2; ++u) {
-            const int row = min(g + 8 * u, rows - 1);
+        for (int nt = 0; nt < NT; ++nt) {
+            const int row = min(8 * nt + g, rows - 1);               // rows behind the block repeat its last one
             const int t = (r0 + row) / s.group;
-            pos[u] = q.kv - q.n + t;
-            qp[u] = a.q + (q.q0 + t) * a.q_stride + (c.h * s.group + (r0 + row) - t * s.group) * a.q_head;
-        }
-        const int pos_lo = __shfl_sync(0xffffffffu, pos[0], 0), pos_hi = __shfl_sync(0xffffffffu, pos[1], 31);
-        uint32_t qa[C::kSteps][4];
+            const __nv_bfloat16* qp = a.q + (q.q0 + t) * a.q_stride + (c.h * s.group + (r0 + row) - t * s.group) * a.q_head;
 #pragma unroll
-        for (int ks = 0; ks < C::kSteps; ++ks)
+            for (int ks = 0; ks < C::kSteps; ++ks) {
+                const uint2 w = __ldg(reinterpret_cast<const uint2*>(qp + q_element<D, FP8>(ks, cc)));
+                qb[nt][ks][0] = w.x;
+                qb[nt][ks][1] = w.y;
+            }
+            float factor = a.scale_log2;
+            if (FP8) {
+                uint32_t m2 = 0;
+#pragma unroll
+                for (int ks = 0; ks < C::kSteps; ++ks) m2 = __vmaxu2(m2, __vmaxu2(qb[nt][ks][0] & 0x7FFF7FFFu, qb[nt][ks][1] & 0x7FFF7FFFu));
+                uint32_t mx = max(m2 & 0xFFFFu, m2 >> 16);
+                mx = max(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
+                mx = max(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
+                const uint32_t e = min(max(mx >> 7, 1u), 253u);      // exponent field of the largest element
+                const float down = pow2_of_field(254u - e);          // 2^(127 - e): the row's largest element becomes 1 to 4
+                factor *= pow2_of_field(e);
+#pragma unroll
+                for (int ks = 0; ks < C::kSteps; ++ks)
+#pragma unroll
+                    for (int i = 0; i < 2; ++i) {
+                        const uint32_t w = qb[nt][ks][i];
+                        qb[nt][ks][i] = pack_f16x2(__uint_as_float(w << 16) * down, __uint_as_float(w & 0xFFFF0000u) * down);
+                    }
+            }
+            const int p = q.kv - q.n + t;
 #pragma unroll
             for (int u = 0; u < 2; ++u) {
-                uint2 w = __ldg(reinterpret_cast<const uint2*>(qp[u] + q_element<D, FP8>(ks, cc)));
-                if (FP8) w = make_uint2(__byte_perm(w.x, w.y, 0x5410), __byte_perm(w.x, w.y, 0x7632));     // even and odd elements
-                qa[ks][u] = w.x;
-                qa[ks][2 + u] = w.y;
+                pos[nt][u] = __shfl_sync(0xffffffffu, p, 4 * (2 * cc + u));
+                row_scale[nt][u] = __shfl_sync(0xffffffffu, factor, 4 * (2 * cc + u));
             }
-        float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.0f, 0.0f};
-        float o[C::kCols][4];
+            if (nt == 0) pos_lo = __shfl_sync(0xffffffffu, p, 0);
+            pos_hi = __shfl_sync(0xffffffffu, p, 31);
+        }
+        float m[NT][2], l[NT][2], o[NT][C::kSteps][4];
 #pragma unroll
-        for (int i = 0; i < C::kCols; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.0f;
+        for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+            for (int u = 0; u < 2; ++u) { m[nt][u] = -INFINITY; l[nt][u] = 0.0f; }
+#pragma unroll
+            for (int i = 0; i < C::kSteps; ++i) o[nt][i][0] = o[nt][i][1] = o[nt][i][2] = o[nt][i][3] = 0.0f;
+        }
+        uint32_t v_field = 1;                                        // exponent field of the power of two that p * scale is divided by
 
         for (int t = 0; t < todo; ++t) {
             if (ok) ok = ptx::mbar_wait(full_bar(stage), phase, a.status, 2);
@@ -206,97 +248,113 @@ attn_split_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
             const uint32_t valid = static_cast<uint32_t>(mask_p[stage] >> (16 * warp)) & 0xFFFFu;
             if (ok && valid != 0) {
                 const uint32_t kb = ring + stage * C::kStageBytes, vb = kb + C::kTensorBytes;
-                float x[2][4] = {};                                  // products with keys 8 * nt + 2 * cc + {0, 1}
+                const int kr = warp * 16 + g;
+                float x[NT][4];                                      // keys g (0, 1) and g + 8 (2, 3) with rows 2cc + {0, 1}
 #pragma unroll
-                for (int nt = 0; nt < 2; ++nt) {
-                    const int row = warp * 16 + nt * 8 + g;
-                    if constexpr (FP8) {
+                for (int nt = 0; nt < NT; ++nt) x[nt][0] = x[nt][1] = x[nt][2] = x[nt][3] = 0.0f;
+                if constexpr (FP8) {
 #pragma unroll
-                        for (int v = 0; v < D / 64; ++v) {
-                            const uint4 w = ptx::ld_shared_v4(swizzled<C::kBoxBytes>(kb, row, D == 128 ? (2 * cc + v) * 16 : cc * 16));
-                            const uint32_t ws[4] = {w.x, w.y, w.z, w.w};
+                    for (int v = 0; v < D / 64; ++v) {
+                        const int byte = D == 128 ? (2 * cc + v) * 16 : cc * 16;
+                        const uint4 w = ptx::ld_shared_v4(swizzled<C::kBoxBytes>(kb, kr, byte)), y = ptx::ld_shared_v4(swizzled<C::kBoxBytes>(kb, kr + 8, byte));
+                        const uint32_t ws[4] = {w.x, w.y, w.z, w.w}, ys[4] = {y.x, y.y, y.z, y.w};
 #pragma unroll
-                            for (int i = 0; i < 4; ++i) {
-                                const uint32_t (&qf)[4] = qa[4 * v + i];
-                                ptx::mma_bf16_16816(x[nt], qf[0], qf[1], qf[2], qf[3], e4m3x2(ws[i] << 8), e4m3x2(ws[i]));
-                            }
+                        for (int i = 0; i < 4; ++i) {
+                            const uint32_t a0 = ptx::e4m3x2_lo(ws[i]), a1 = ptx::e4m3x2_lo(ys[i]), a2 = ptx::e4m3x2_hi(ws[i]), a3 = ptx::e4m3x2_hi(ys[i]);
+#pragma unroll
+                            for (int nt = 0; nt < NT; ++nt) mma<FP8>(x[nt], a0, a1, a2, a3, qb[nt][4 * v + i][0], qb[nt][4 * v + i][1]);
                         }
-                    } else {
+                    }
+                } else {
 #pragma unroll
-                        for (int hv = 0; hv < D / 32; ++hv) {
-                            const uint4 w = ptx::ld_shared_v4(swizzled<128>(kb + (hv >> 1) * C::kHalfBytes, row, (2 * cc + (hv & 1)) * 16));
-                            const uint32_t (&q0)[4] = qa[2 * hv];
-                            const uint32_t (&q1)[4] = qa[2 * hv + 1];
-                            ptx::mma_bf16_16816(x[nt], q0[0], q0[1], q0[2], q0[3], w.x, w.y);
-                            ptx::mma_bf16_16816(x[nt], q1[0], q1[1], q1[2], q1[3], w.z, w.w);
+                    for (int hv = 0; hv < D / 32; ++hv) {
+                        const uint32_t half = kb + (hv >> 1) * C::kHalfBytes;
+                        const int byte = (2 * cc + (hv & 1)) * 16;
+                        const uint4 w = ptx::ld_shared_v4(swizzled<128>(half, kr, byte)), y = ptx::ld_shared_v4(swizzled<128>(half, kr + 8, byte));
+#pragma unroll
+                        for (int nt = 0; nt < NT; ++nt) {
+                            mma<FP8>(x[nt], w.x, y.x, w.y, y.y, qb[nt][2 * hv][0], qb[nt][2 * hv][1]);
+                            mma<FP8>(x[nt], w.z, y.z, w.w, y.w, qb[nt][2 * hv + 1][0], qb[nt][2 * hv + 1][1]);
                         }
                     }
                 }
-                // scores in units of log2; a key's scale first
-                float vs[2][2];
+                float ks[2] = {1.0f, 1.0f}, vs[2] = {1.0f, 1.0f};    // of keys g and g + 8
+                const bool there[2] = {((valid >> g) & 1u) != 0, ((valid >> (g + 8)) & 1u) != 0};
+                float v_down = 1.0f, v_move = 1.0f;
+                if (FP8) {
+                    const uint32_t at = kb + 2 * C::kTensorBytes + kr * 4;
+                    ks[0] = ptx::ld_shared_f32(at); ks[1] = ptx::ld_shared_f32(at + 32);
+                    vs[0] = ptx::ld_shared_f32(at + C::kScaleBytes); vs[1] = ptx::ld_shared_f32(at + C::kScaleBytes + 32);
+                    // field of the smallest power of two above the largest finite scale (scales are not negative)
+                    uint32_t f = 0;
 #pragma unroll
-                for (int nt = 0; nt < 2; ++nt) {
-                    float2 ks = make_float2(1.0f, 1.0f), v2 = ks;
-                    if (FP8) {
-                        const uint32_t at = kb + 2 * C::kTensorBytes + (warp * 16 + nt * 8 + 2 * cc) * 4;
-                        const uint2 w = ptx::ld_shared_v2(at), y = ptx::ld_shared_v2(at + C::kScaleBytes);
-                        ks = make_float2(__uint_as_float(w.x), __uint_as_float(w.y));
-                        v2 = make_float2(__uint_as_float(y.x), __uint_as_float(y.y));
+                    for (int k = 0; k < 2; ++k) {
+                        const uint32_t bits = __float_as_uint(vs[k]) & 0x7FFFFFFFu;
+                        if (there[k] && bits < 0x7F800000u) f = max(f, bits);
                     }
-                    vs[nt][0] = v2.x; vs[nt][1] = v2.y;
-                    const float f0 = ks.x * a.scale_log2, f1 = ks.y * a.scale_log2;
-                    x[nt][0] *= f0; x[nt][1] *= f1; x[nt][2] *= f0; x[nt][3] *= f1;
+                    f = min((__reduce_max_sync(0xffffffffu, f) >> 23) + 1, 253u);
+                    if (f > v_field) { v_move = f - v_field < 127u ? pow2_of_field(127u - (f - v_field)) : 0.0f; v_field = f; }
+                    v_down = pow2_of_field(254u - v_field);
                 }
-                // keys that are not there for the whole block (their values are zeroed too: what lies in their place may
-                // be anything), that come after a row, or that have left its window
+                // keys that are not there for the whole block, that come after a row, or that have left its window
                 const bool whole = valid == 0xFFFFu && (!s.causal || key0 + 15 <= pos_lo) && (s.window == 0 || key0 > pos_hi - s.window);
-                if (!whole) {
+                uint32_t pb[NT][2], pl[NT][2];
+                bool moved = FP8 && v_move != 1.0f;
+                float f[NT][2];
 #pragma unroll
-                    for (int nt = 0; nt < 2; ++nt)
-#pragma unroll
-                        for (int e = 0; e < 2; ++e) {
-                            const int j = nt * 8 + 2 * cc + e;
-                            const bool there = (valid >> j) & 1u;
-#pragma unroll
-                            for (int u = 0; u < 2; ++u) {
-                                const int key = key0 + j;
-                                const bool seen = there && (!s.causal || key <= pos[u]) && (s.window == 0 || key > pos[u] - s.window);
-                                if (!seen) x[nt][2 * u + e] = -INFINITY;
-                            }
-                        }
-                }
-                uint32_t pa[4];
-                float f[2];
-                bool moved = false;
-#pragma unroll
-                for (int u = 0; u < 2; ++u) {
-                    float t4 = max_nan4(x[0][2 * u], x[0][2 * u + 1], x[1][2 * u], x[1][2 * u + 1]);
-                    t4 = ptx::max_nan(t4, __shfl_xor_sync(0xffffffffu, t4, 1));
-                    t4 = ptx::max_nan(t4, __shfl_xor_sync(0xffffffffu, t4, 2));
-                    const float mn = ptx::max_nan(m[u], t4);
-                    const float base = mn == -INFINITY ? 0.0f : mn;          // a row that has seen nothing yet
-                    f[u] = ptx::ex2(m[u] - base);
-                    moved |= mn != m[u];
-                    m[u] = mn;
+                for (int nt = 0; nt < NT; ++nt) {
                     float p[4];
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) p[i] = ptx::ex2(x[i >> 1][2 * u + (i & 1)] - base);
-                    l[u] = l[u] * f[u] + ((p[0] + p[1]) + (p[2] + p[3]));
+                    for (int i = 0; i < 4; ++i) {
+                        const int k = i >> 1, u = i & 1;
+                        x[nt][i] *= FP8 ? ks[k] * row_scale[nt][u] : row_scale[nt][u];
+                        if (!whole) {
+                            const int key = key0 + g + 8 * k;
+                            const bool seen = there[k] && (!s.causal || key <= pos[nt][u]) && (s.window == 0 || key > pos[nt][u] - s.window);
+                            if (!seen) x[nt][i] = -INFINITY;
+                        }
+                    }
+#pragma unroll
+                    for (int u = 0; u < 2; ++u) {
+                        float mn = ptx::max_nan(x[nt][u], x[nt][2 + u]);
+#pragma unroll
+                        for (int w = 4; w <= 16; w <<= 1) mn = ptx::max_nan(mn, __shfl_xor_sync(0xffffffffu, mn, w));
+                        mn = ptx::max_nan(mn, m[nt][u]);
+                        const float base = mn == -INFINITY ? 0.0f : mn;      // a row that has seen nothing yet
+                        const float fm = ptx::ex2(m[nt][u] - base);
+                        f[nt][u] = fm * v_move;
+                        moved |= mn != m[nt][u];
+                        p[u] = ptx::ex2(x[nt][u] - base);
+                        p[2 + u] = ptx::ex2(x[nt][2 + u] - base);
+                        l[nt][u] = l[nt][u] * fm + (p[u] + p[2 + u]);
+                        m[nt][u] = mn;
+                    }
                     if (FP8) {
                         // a masked key's p is 0: its product with a scale that is not finite must be 0 as well
 #pragma unroll
-                        for (int i = 0; i < 4; ++i) p[i] = !whole && p[i] == 0.0f ? 0.0f : p[i] * vs[i >> 1][i & 1];
+                        for (int i = 0; i < 4; ++i) p[i] = !whole && p[i] == 0.0f ? 0.0f : p[i] * (vs[i >> 1] * v_down);
+                        pb[nt][0] = ptx::movmatrix_trans(pack_f16x2(p[0], p[1]));
+                        pb[nt][1] = ptx::movmatrix_trans(pack_f16x2(p[2], p[3]));
+                    } else {
+#pragma unroll
+                        for (int k = 0; k < 2; ++k) {
+                            const uint32_t hi = pack_bf16x2(p[2 * k], p[2 * k + 1]);
+                            pl[nt][k] = ptx::movmatrix_trans(pack_bf16x2(p[2 * k] - __uint_as_float(hi << 16), p[2 * k + 1] - __uint_as_float(hi & 0xFFFF0000u)));
+                            pb[nt][k] = ptx::movmatrix_trans(hi);
+                        }
                     }
-                    pa[u] = pack_bf16x2(p[0], p[1]);
-                    pa[2 + u] = pack_bf16x2(p[2], p[3]);
                 }
                 if (__any_sync(0xffffffffu, moved)) {
 #pragma unroll
-                    for (int i = 0; i < C::kCols; ++i) { o[i][0] *= f[0]; o[i][1] *= f[0]; o[i][2] *= f[1]; o[i][3] *= f[1]; }
+                    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                        for (int i = 0; i < C::kSteps; ++i) { o[nt][i][0] *= f[nt][0]; o[nt][i][1] *= f[nt][1]; o[nt][i][2] *= f[nt][0]; o[nt][i][3] *= f[nt][1]; }
                 }
-                // values: thread (g, cc) takes columns of chunk g in rows 2cc, 2cc+1, 2cc+8, 2cc+9
+                // values: columns of chunk g in rows 2cc, 2cc + 1, 2cc + 8, 2cc + 9; what is not there counts as zero, whatever it is
                 const int vr = warp * 16 + 2 * cc;
-                const uint32_t keep[4] = {(valid >> (2 * cc)) & 1u, (valid >> (2 * cc + 1)) & 1u, (valid >> (2 * cc + 8)) & 1u, (valid >> (2 * cc + 9)) & 1u};
+                bool in[4];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) in[i] = whole || ((valid >> (2 * cc + (i & 1) + 8 * (i >> 1))) & 1u);
                 if constexpr (FP8) {
                     uint32_t w[4][D / 32];
 #pragma unroll
@@ -304,19 +362,21 @@ attn_split_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
                         const int row = vr + (i & 1) + 8 * (i >> 1);
                         if constexpr (D == 128) {
                             const uint4 y = ptx::ld_shared_v4(swizzled<128>(vb, row, g * 16));
-                            w[i][0] = y.x; w[i][1] = y.y; w[i][2] = y.z; w[i][3] = y.w;
+                            w[i][0] = in[i] ? y.x : 0u; w[i][1] = in[i] ? y.y : 0u; w[i][2] = in[i] ? y.z : 0u; w[i][3] = in[i] ? y.w : 0u;
                         } else {
                             const uint2 y = ptx::ld_shared_v2(swizzled<64>(vb, row, g * 8));
-                            w[i][0] = y.x; w[i][1] = y.y;
+                            w[i][0] = in[i] ? y.x : 0u; w[i][1] = in[i] ? y.y : 0u;
                         }
-                    }                                                 // bytes are finite whatever they are: no need to zero them
+                    }
 #pragma unroll
                     for (int j = 0; j < D / 32; ++j)
 #pragma unroll
-                        for (int e = 0; e < 4; ++e) {
-                            const uint32_t sel = (e << 4) | ((4 + e) << 12);
-                            ptx::mma_bf16_16816(o[4 * j + e], pa[0], pa[1], pa[2], pa[3], e4m3x2(__byte_perm(w[0][j], w[1][j], sel)),
-                                                e4m3x2(__byte_perm(w[2][j], w[3][j], sel)));
+                        for (int e = 0; e < 2; ++e) {                // columns 4j + 2e, 4j + 2e + 1 of the chunk
+                            const uint32_t sel = e == 0 ? 0x5140u : 0x7362u;
+                            const uint32_t lo = __byte_perm(w[0][j], w[1][j], sel), hi = __byte_perm(w[2][j], w[3][j], sel);
+                            const uint32_t a0 = ptx::e4m3x2_lo(lo), a1 = ptx::e4m3x2_hi(lo), a2 = ptx::e4m3x2_lo(hi), a3 = ptx::e4m3x2_hi(hi);
+#pragma unroll
+                            for (int nt = 0; nt < NT; ++nt) mma<FP8>(o[nt][2 * j + e], a0, a1, a2, a3, pb[nt][0], pb[nt][1]);
                         }
                 } else {
 #pragma unroll
@@ -325,15 +385,17 @@ attn_split_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
 #pragma unroll
                         for (int i = 0; i < 4; ++i) {
                             const uint4 y = ptx::ld_shared_v4(swizzled<128>(vb + h * C::kHalfBytes, vr + (i & 1) + 8 * (i >> 1), g * 16));
-                            const bool in = whole || keep[i];
-                            w[i][0] = in ? y.x : 0u; w[i][1] = in ? y.y : 0u; w[i][2] = in ? y.z : 0u; w[i][3] = in ? y.w : 0u;
+                            w[i][0] = in[i] ? y.x : 0u; w[i][1] = in[i] ? y.y : 0u; w[i][2] = in[i] ? y.z : 0u; w[i][3] = in[i] ? y.w : 0u;
                         }
 #pragma unroll
                         for (int j = 0; j < 4; ++j) {
-                            ptx::mma_bf16_16816(o[8 * h + 2 * j], pa[0], pa[1], pa[2], pa[3], __byte_perm(w[0][j], w[1][j], 0x5410),
-                                                __byte_perm(w[2][j], w[3][j], 0x5410));
-                            ptx::mma_bf16_16816(o[8 * h + 2 * j + 1], pa[0], pa[1], pa[2], pa[3], __byte_perm(w[0][j], w[1][j], 0x7632),
-                                                __byte_perm(w[2][j], w[3][j], 0x7632));
+                            const uint32_t a0 = __byte_perm(w[0][j], w[1][j], 0x5410), a1 = __byte_perm(w[0][j], w[1][j], 0x7632);
+                            const uint32_t a2 = __byte_perm(w[2][j], w[3][j], 0x5410), a3 = __byte_perm(w[2][j], w[3][j], 0x7632);
+#pragma unroll
+                            for (int nt = 0; nt < NT; ++nt) {
+                                mma<FP8>(o[nt][4 * h + j], a0, a1, a2, a3, pb[nt][0], pb[nt][1]);
+                                mma<FP8>(o[nt][4 * h + j], a0, a1, a2, a3, pl[nt][0], pl[nt][1]);
+                            }
                         }
                     }
                 }
@@ -345,92 +407,92 @@ attn_split_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
 
         // ------------------------------------------------------------------------ the four warps' states become one
 #pragma unroll
-        for (int u = 0; u < 2; ++u) {
-            l[u] += __shfl_xor_sync(0xffffffffu, l[u], 1);
-            l[u] += __shfl_xor_sync(0xffffffffu, l[u], 2);
-            if (cc == 0) state_p[warp * kRows + g + 8 * u] = make_float2(m[u], l[u]);
-        }
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+#pragma unroll
+                for (int w = 4; w <= 16; w <<= 1) l[nt][u] += __shfl_xor_sync(0xffffffffu, l[nt][u], w);
+                if (g == 0) state_p[warp * kRows + 8 * nt + 2 * cc + u] = make_float2(m[nt][u], l[nt][u]);
+            }
         ptx::named_barrier(1, 32 * kConsumers);
-        float mm[2], ll[2];
+        const float v_up = FP8 ? pow2_of_field(v_field) : 1.0f;
 #pragma unroll
-        for (int u = 0; u < 2; ++u) {
-            float2 st[kConsumers];
-            mm[u] = -INFINITY;
+        for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-            for (int w = 0; w < kConsumers; ++w) { st[w] = state_p[w * kRows + g + 8 * u]; mm[u] = ptx::max_nan(mm[u], st[w].x); }
-            const float base = mm[u] == -INFINITY ? 0.0f : mm[u];
-            ll[u] = 0.0f;
+            for (int u = 0; u < 2; ++u) {
+                float2 st[kConsumers];
+                float mm = -INFINITY, ll = 0.0f;
 #pragma unroll
-            for (int w = 0; w < kConsumers; ++w) ll[u] += st[w].y * ptx::ex2(st[w].x - base);
-            const float f = ptx::ex2(m[u] - base);
+                for (int w = 0; w < kConsumers; ++w) { st[w] = state_p[w * kRows + 8 * nt + 2 * cc + u]; mm = ptx::max_nan(mm, st[w].x); }
+                const float base = mm == -INFINITY ? 0.0f : mm;
 #pragma unroll
-            for (int i = 0; i < C::kCols; ++i) { o[i][2 * u] *= f; o[i][2 * u + 1] *= f; }
-        }
+                for (int w = 0; w < kConsumers; ++w) ll += st[w].y * ptx::ex2(st[w].x - base);
+                const float fw = ptx::ex2(m[nt][u] - base) * v_up;
+#pragma unroll
+                for (int i = 0; i < C::kSteps; ++i) { o[nt][i][u] *= fw; o[nt][i][2 + u] *= fw; }
+                m[nt][u] = mm;
+                l[nt][u] = ll;
+            }
 #pragma unroll
         for (int w = kConsumers - 1; w >= 1; --w) {                  // one after the other they hand over to warp 0
             if (warp == w) {
 #pragma unroll
-                for (int i = 0; i < C::kCols; ++i)
-                    *reinterpret_cast<float4*>(join_p + i * 128 + lane * 4) = make_float4(o[i][0], o[i][1], o[i][2], o[i][3]);
+                for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                    for (int i = 0; i < C::kSteps; ++i)
+                        *reinterpret_cast<float4*>(join_p + (nt * C::kSteps + i) * 128 + lane * 4) = make_float4(o[nt][i][0], o[nt][i][1], o[nt][i][2], o[nt][i][3]);
             }
             ptx::named_barrier(1, 32 * kConsumers);
             if (warp == 0) {
 #pragma unroll
-                for (int i = 0; i < C::kCols; ++i) {
-                    const float4 y = *reinterpret_cast<const float4*>(join_p + i * 128 + lane * 4);
-                    o[i][0] += y.x; o[i][1] += y.y; o[i][2] += y.z; o[i][3] += y.w;
-                }
+                for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                    for (int i = 0; i < C::kSteps; ++i) {
+                        const float4 y = *reinterpret_cast<const float4*>(join_p + (nt * C::kSteps + i) * 128 + lane * 4);
+                        o[nt][i][0] += y.x; o[nt][i][1] += y.y; o[nt][i][2] += y.z; o[nt][i][3] += y.w;
+                    }
             }
             if (w > 1) ptx::named_barrier(1, 32 * kConsumers);       // before the buffer is written again
         }
         if (warp == 0) {
             const bool begins = c.tile == 0, ends = c.tile + todo == r.tiles;
-            // column of accumulator i, element e: thread cc holds columns 2cc + e of group i
-            auto column = [&](int i, int e) {
-                if (FP8) return (2 * cc + e) * (D / 8) + i;
-                return (i >> 3) * 64 + (2 * cc + e) * 8 + (i & 7);
-            };
-            if (begins && ends) {
+            // accumulator group i, element 2 * e + u: row 2cc + u, column 2i + e of chunk g (16 columns of an E4M3 row of 128,
+            // else 8; group 4h + j of a bf16 row is columns 2j, 2j + 1 of half h)
+            constexpr int kRun = FP8 && D == 128 ? 16 : 8;
+            const int slot = 2 * blockIdx.x + (begins ? 1 : 0);
+            float* po = a.part + static_cast<size_t>(slot) * kRows * (D + 2);
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
                 for (int u = 0; u < 2; ++u) {
-                    const int row = g + 8 * u;
-                    if (row >= rows) continue;
-                    const int t = (r0 + row) / s.group;
-                    const size_t to = static_cast<size_t>(q.q0 + t) * s.heads + c.h * s.group + (r0 + row) - t * s.group;
-                    const float inv = ll[u] == 0.0f ? 0.0f : __frcp_rn(ll[u]);
-                    // column(i, e) is contiguous in i over runs of 8 (or 16)
+                    const int row = 8 * nt + 2 * cc + u;
+                    if (begins && ends) {
+                        if (row >= rows) continue;
+                        const int t = (r0 + row) / s.group;
+                        const size_t to = static_cast<size_t>(q.q0 + t) * s.heads + c.h * s.group + (r0 + row) - t * s.group;
+                        const float inv = l[nt][u] == 0.0f ? 0.0f : __frcp_rn(l[nt][u]);
 #pragma unroll
-                    for (int e = 0; e < 2; ++e)
+                        for (int i = 0; i < C::kSteps; i += 4) {     // eight columns
+                            uint32_t w[4];
 #pragma unroll
-                        for (int i = 0; i < C::kCols; i += 8) {
-                            uint4 w;
-                            w.x = pack_bf16x2(o[i][2 * u + e] * inv, o[i + 1][2 * u + e] * inv);
-                            w.y = pack_bf16x2(o[i + 2][2 * u + e] * inv, o[i + 3][2 * u + e] * inv);
-                            w.z = pack_bf16x2(o[i + 4][2 * u + e] * inv, o[i + 5][2 * u + e] * inv);
-                            w.w = pack_bf16x2(o[i + 6][2 * u + e] * inv, o[i + 7][2 * u + e] * inv);
-                            *reinterpret_cast<uint4*>(a.out + to * D + column(i, e)) = w;
+                            for (int k = 0; k < 4; ++k) w[k] = pack_bf16x2(o[nt][i + k][u] * inv, o[nt][i + k][2 + u] * inv);
+                            const int col = kRun == 16 ? g * 16 + 2 * i : (i >> 2) * 64 + g * 8;
+                            *reinterpret_cast<uint4*>(a.out + to * D + col) = make_uint4(w[0], w[1], w[2], w[3]);
                         }
-                    if (a.lse != nullptr && cc == 0) a.lse[to] = lse_of(mm[u], ll[u]);
-                }
-            } else {
-                const int slot = 2 * blockIdx.x + (begins ? 1 : 0);
-                float* po = a.part + static_cast<size_t>(slot) * kRows * (D + 2);
+                        if (a.lse != nullptr && g == 0) a.lse[to] = lse_of(m[nt][u], l[nt][u]);
+                    } else {
 #pragma unroll
-                for (int u = 0; u < 2; ++u) {
-                    const int row = g + 8 * u;
-#pragma unroll
-                    for (int e = 0; e < 2; ++e)
-#pragma unroll
-                        for (int i = 0; i < C::kCols; i += 4)
-                            *reinterpret_cast<float4*>(po + row * D + column(i, e)) =
-                                make_float4(o[i][2 * u + e], o[i + 1][2 * u + e], o[i + 2][2 * u + e], o[i + 3][2 * u + e]);
-                    if (cc == 0) *reinterpret_cast<float2*>(po + kRows * D + row * 2) = make_float2(mm[u], ll[u]);
+                        for (int i = 0; i < C::kSteps; i += 2) {
+                            const int col = kRun == 16 ? g * 16 + 2 * i : (i >> 2) * 64 + g * 8 + 2 * (i & 3);
+                            *reinterpret_cast<float4*>(po + row * D + col) = make_float4(o[nt][i][u], o[nt][i][2 + u], o[nt][i + 1][u], o[nt][i + 1][2 + u]);
+                        }
+                        if (g == 0) *reinterpret_cast<float2*>(po + kRows * D + row * 2) = make_float2(m[nt][u], l[nt][u]);
+                    }
                 }
-                if (begins && lane == 0) {
-                    Open* op = a.open + blockIdx.x;
-                    op->token0 = q.q0; op->r0 = r0; op->rows = rows; op->h = c.h;
-                    op->last = owner(c, c.at + r.tiles - 1);
-                }
+            if (begins && !ends && lane == 0) {
+                Open* op = a.open + blockIdx.x;
+                op->token0 = q.q0; op->r0 = r0; op->rows = rows; op->h = c.h;
+                op->last = owner(c, c.at + r.tiles - 1);
             }
         }
         ptx::named_barrier(1, 32 * kConsumers);                       // the state and the join buffer are free again
@@ -439,10 +501,10 @@ attn_split_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
     }
 }
 
-template <int D, bool FP8>
+template <int D, bool FP8, int NT>
 int launch(const Args& args, cudaStream_t stream)
 {
-    using C = Cfg<D, FP8>;
+    using C = Cfg<D, FP8, NT>;
     Args a = args;
     const int box = kTile < (1 << a.s.page_shift) ? kTile : 1 << a.s.page_shift;
     const uint64_t rows = (static_cast<uint64_t>(a.s.num_pages) * a.s.kv_heads) << a.s.page_shift;
@@ -450,7 +512,7 @@ int launch(const Args& args, cudaStream_t stream)
     const CUtensorMapSwizzle sw = C::kBoxBytes == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B;
     if (!make_tmap_2d_u8(&tmK, a.k_cache, rows, C::kRowBytes, C::kRowBytes, box, C::kBoxBytes, sw)) return cudaErrorInvalidValue;
     if (!make_tmap_2d_u8(&tmV, a.v_cache, rows, C::kRowBytes, C::kRowBytes, box, C::kBoxBytes, sw)) return cudaErrorInvalidValue;
-    auto kernel = attn_split_kernel<D, FP8>;
+    auto kernel = attn_split_kernel<D, FP8, NT>;
     static bool configured[64] = {};
     int dev = 0;
     cudaError_t e = cudaGetDevice(&dev);
@@ -461,26 +523,31 @@ int launch(const Args& args, cudaStream_t stream)
         if (dev < 64) configured[dev] = true;
     }
     if (static_cast<long long>(a.s.seqs) * 8 > C::kStages * C::kStageBytes) return cudaErrorInvalidValue;
-    a.block_limit = static_cast<int>((static_cast<long long>(a.max_q) * a.s.group + kRows - 1) / kRows);
-    const int ctas = 2 * num_sms();
+    a.block_limit = static_cast<int>((static_cast<long long>(a.max_q) * a.s.group + C::kRows - 1) / C::kRows);
+    const int ctas = C::kCtasPerSm * num_sms();
     kernel<<<ctas, kThreads, C::kSmemBytes, stream>>>(tmK, tmV, a);
     e = cudaGetLastError();
     if (e != cudaSuccess) return e;
-    return launch_combine<D>(a, ctas, kRows, stream);
+    return launch_combine<D>(a, ctas, C::kRows, stream);
+}
+
+template <int D, bool FP8>
+int launch_rows(const Args& a, cudaStream_t stream)
+{
+    return static_cast<long long>(a.max_q) * a.s.group <= 8 ? launch<D, FP8, 1>(a, stream) : launch<D, FP8, 2>(a, stream);
 }
 
 }  // namespace split
 
 int attn_split(const Args& a, int head_dim, bool fp8, cudaStream_t stream)
 {
-    if (head_dim == 64) return fp8 ? split::launch<64, true>(a, stream) : split::launch<64, false>(a, stream);
-    return fp8 ? split::launch<128, true>(a, stream) : split::launch<128, false>(a, stream);
+    if (head_dim == 64) return fp8 ? split::launch_rows<64, true>(a, stream) : split::launch_rows<64, false>(a, stream);
+    return fp8 ? split::launch_rows<128, true>(a, stream) : split::launch_rows<128, false>(a, stream);
 }
 
-size_t attn_split_workspace(int head_dim)
-{
-    return static_cast<size_t>(2 * num_sms()) * (2 * split::kRows * (head_dim + 2) * sizeof(float) + sizeof(Open)) + 32;
-}
+// the larger of 3 CTAs an SM with 8 rows and 2 with 16
+int attn_split_ctas() { return 3 * num_sms(); }
+size_t attn_split_part_bytes(int head_dim) { return static_cast<size_t>(2 * num_sms()) * 2 * 16 * (head_dim + 2) * sizeof(float); }
 
 }  // namespace paged
 }  // namespace b200q

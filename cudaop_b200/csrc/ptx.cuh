@@ -630,6 +630,38 @@ __device__ __forceinline__ void mma_bf16_16816(float (&d)[4], uint32_t a0, uint3
         : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
+// the same with fp16 operands
+__device__ __forceinline__ void mma_f16_16816(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
+                                              uint32_t b0, uint32_t b1)
+{
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+// movmatrix.m8n8.trans.b16: lane 4g + c holds elements (g, 2c), (g, 2c + 1) of an 8x8 matrix and gets those of its transpose
+__device__ __forceinline__ uint32_t movmatrix_trans(uint32_t x)
+{
+    uint32_t y;
+    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+    return y;
+}
+
+// cvt.rn.f16x2.e4m3x2 of the low / high two bytes of x (exact)
+__device__ __forceinline__ uint32_t e4m3x2_lo(uint32_t x)
+{
+    uint32_t y;
+    asm("{\n\t.reg .b16 l, h;\n\tmov.b32 {l, h}, %1;\n\tcvt.rn.f16x2.e4m3x2 %0, l;\n\t}" : "=r"(y) : "r"(x));
+    return y;
+}
+__device__ __forceinline__ uint32_t e4m3x2_hi(uint32_t x)
+{
+    uint32_t y;
+    asm("{\n\t.reg .b16 l, h;\n\tmov.b32 {l, h}, %1;\n\tcvt.rn.f16x2.e4m3x2 %0, h;\n\t}" : "=r"(y) : "r"(x));
+    return y;
+}
+
 // max that returns NaN when either input is NaN (so a NaN activation reaches the exponent test below)
 __device__ __forceinline__ float max_nan(float a, float b)
 {
