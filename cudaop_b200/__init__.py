@@ -75,6 +75,7 @@ _SIGNATURES = {
     "b200q_paged_cache_write": [_VP] * 7 + [_I] * 3 + [C.c_longlong] * 4 + [_I] * 3 + [_VP],
     "b200q_paged_cache_read": [_VP] * 8 + [_I] * 9 + [_VP],
     "b200q_paged_attention": [_VP] * 10 + [_I] * 5 + [C.c_longlong] * 2 + [_I] * 5 + [_F] + [_I] * 3 + [_VP] * 2,
+    "b200q_paged_set_impl": [_I],
     "b200q_status": [_VP, _I],
     "b200q_set_wait_limit_ms": [_I, _I],
     "b200q_rank_barrier": [_VP, _I, _I, C.c_uint, C.c_uint, _VP],

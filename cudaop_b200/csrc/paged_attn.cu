@@ -5,6 +5,7 @@
 namespace b200q {
 namespace paged {
 int page_shift_of(int page_size);        // paged_cache.cu
+int g_impl = 0;                          // 0 by the number of rows, 1 split-KV kernel, 2 tensor-core kernel
 size_t open_bytes() { return (static_cast<size_t>(attn_split_ctas()) * sizeof(Open) + 15) / 16 * 16; }
 }
 }
@@ -14,7 +15,8 @@ extern "C" {
 size_t b200q_paged_attention_workspace_bytes(int head_dim)
 {
     if (head_dim != 64 && head_dim != 128) return 0;
-    return b200q::paged::open_bytes() + b200q::paged::attn_split_part_bytes(head_dim);
+    const size_t split = b200q::paged::attn_split_part_bytes(head_dim), chunk = b200q::paged::attn_chunk_part_bytes(head_dim);
+    return b200q::paged::open_bytes() + (split > chunk ? split : chunk);
 }
 
 int b200q_paged_attention(const void* q, const void* k_cache, const void* v_cache, const float* k_scale, const float* v_scale,
@@ -55,7 +57,15 @@ int b200q_paged_attention(const void* q, const void* k_cache, const void* v_cach
     if (a.status == nullptr) return cudaErrorInvalidDevice;
     a.open = static_cast<Open*>(workspace);
     a.part = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + open_bytes());
-    return attn_split(a, head_dim, fp8 != 0, static_cast<cudaStream_t>(stream));
+    const bool chunk = g_impl != 0 ? g_impl == 2 : static_cast<long long>(a.max_q) * a.s.group > 64;
+    return chunk ? attn_chunk(a, head_dim, fp8 != 0, static_cast<cudaStream_t>(stream)) : attn_split(a, head_dim, fp8 != 0, static_cast<cudaStream_t>(stream));
+}
+
+int b200q_paged_set_impl(int impl)
+{
+    if (impl < 0 || impl > 2) return cudaErrorInvalidValue;
+    b200q::paged::g_impl = impl;
+    return 0;
 }
 
 }  // extern "C"

@@ -25,6 +25,8 @@ struct Args {
 };
 
 int attn_split(const Args& a, int head_dim, bool fp8, cudaStream_t stream);
+int attn_chunk(const Args& a, int head_dim, bool fp8, cudaStream_t stream);
+size_t attn_chunk_part_bytes(int head_dim);
 int attn_split_ctas();                       // the most CTAs a launch uses
 size_t attn_split_part_bytes(int head_dim);  // the most its parts take
 

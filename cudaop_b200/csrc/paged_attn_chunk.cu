@@ -1,0 +1,557 @@
+// Attention of a chunk of new tokens over a paged cache, for many rows per kv head (prefill in chunks): the tensor-core kernel.
+// The mathematics, the division of the work and the treatment of an E4M3 cache are those of paged_attn_split.cu; what differs is
+// the bound: with 256 rows a key costs 4 * 256 * head_dim operations, so the products run on tcgen05 and the softmax beside them.
+//
+// One CTA per SM takes a block of 256 rows (two halves of 128) through tiles of 128 keys:
+//   warps 0-3, 4-7   softmax of half 0 and 1, a thread per row (= TMEM lane): no shuffles.  They also load the rows of q at the
+//                    start of a block and write the output at its end.
+//   warps 8-11       loaders: keys and values into a ring of [128 keys][D] 16-bit slots, 128-byte swizzle, K(0) V(0) K(1) V(1) ...
+//                    An E4M3 cache is read into registers, converted (exactly, to fp16) and stored; a bf16 cache goes by cp.async.
+//                    Keys that are not there are stored as zeros, so whatever lies in their place reaches no product.
+//   warp 12          issues the products.  S_h = Q_h K^T (both from shared memory) into TMEM; the softmax turns S_h into P_h (fp16 or
+//                    bf16) over the same TMEM columns; O_h += P_h V with P_h as the tensor-memory operand and V as it lies, rows of
+//                    D contiguous elements (MN-major).  The order PV_0(j) S_0(j+1) PV_1(j) S_1(j+1) keeps the tensor cores on one half while
+//                    the other half's softmax runs.
+// TMEM: S_0 S_1 (128 columns each), O_0 O_1 (D columns each).  The running maximum is raised, and O rescaled in TMEM by the row's
+// own thread, only when it grows by more than 2^4 (exact: the sum uses the same base); after the first tiles that is rare.
+#include "paged_common.cuh"
+#include "paged_attn.cuh"
+#include "ptx.cuh"
+
+namespace b200q {
+namespace paged {
+namespace chunk {
+
+constexpr int kRows = 256, kTile = 128, kThreads = 512;
+constexpr int kScaleSlots = 4;
+constexpr int kSoftmaxRegs = 192, kLoaderRegs = 88, kMmaRegs = 40;            // 2 * 192 + 88 + 40 = 4 * 128
+constexpr float kLazy = 4.0f;                  // p is at most 2^4
+// p * scale / (largest scale) is kept times 2^11, so that fp16 holds it from 2^15 down: what falls below its normal range is 2^-29 of the
+// largest value in the cache
+constexpr float kRoom = 2048.0f;
+
+template <int D, bool FP8>
+struct Cfg {
+    static constexpr int kHalves = D / 64;                                    // 128-byte columns of a 16-bit row
+    static constexpr int kHalfBytes = kTile * 128;
+    static constexpr int kSlotBytes = kHalves * kHalfBytes;
+    static constexpr int kSlots = D == 128 ? 4 : 6;
+    static constexpr int kQBytes = 2 * kSlotBytes;
+    // per tile: mask words, largest value scales (4 each), then key scales and value scales
+    static constexpr int kScaleBytes = 32 + (FP8 ? 2 * kTile * 4 : 0);
+    static constexpr int kBars = 2 * kSlots + kScaleSlots + 8;
+    static constexpr int kSmemBytes = 1024 + kQBytes + kSlots * kSlotBytes + kScaleSlots * kScaleBytes + kBars * 8 + 16;
+    static constexpr int kOCol = 256;
+};
+
+__device__ __forceinline__ float pow2_of_field(uint32_t e) { return __uint_as_float(e << 23); }
+__device__ __forceinline__ uint32_t pack_f16x2(float lo, float hi)
+{
+    const __half2 v = __floats2half2_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t*>(&v);
+}
+// 16-byte unit `unit` of row `row` in a [rows][128 bytes] column with the 128-byte swizzle
+__device__ __forceinline__ uint32_t unit_at(uint32_t column, int row, int unit) { return column + row * 128 + ((unit ^ (row & 7)) << 4); }
+
+template <int D, bool FP8>
+__global__ void __launch_bounds__(kThreads, 1)
+attn_chunk_kernel(const Args a)
+{
+    using C = Cfg<D, FP8>;
+    extern __shared__ uint8_t smem_raw[];
+    const uint32_t raw = ptx::smem_u32(smem_raw);
+    const uint32_t q_base = (raw + 1023u) & ~1023u;
+    const uint32_t ring = q_base + C::kQBytes;
+    const uint32_t scales = ring + C::kSlots * C::kSlotBytes;
+    const uint32_t bars = scales + kScaleSlots * C::kScaleBytes;
+    auto full_bar = [&](int s) { return bars + 8u * s; };                     // a slot holds its tile
+    auto empty_bar = [&](int s) { return bars + 8u * (C::kSlots + s); };
+    auto scale_bar = [&](int s) { return bars + 8u * (2 * C::kSlots + s); };  // the softmax is done with a tile's scales
+    const uint32_t more = bars + 8u * (2 * C::kSlots + kScaleSlots);
+    auto q_bar = [&](int h) { return more + 8u * h; };
+    auto s_bar = [&](int h) { return more + 8u * (2 + h); };                  // scores of half h are in TMEM
+    auto p_bar = [&](int h) { return more + 8u * (4 + h); };                  // P of half h is in TMEM
+    auto o_bar = [&](int h) { return more + 8u * (6 + h); };                  // P V of half h is done
+    const uint32_t tmem_slot = bars + C::kBars * 8;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const Shape& s = a.s;
+
+    ptx::pdl_launch_dependents();
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < C::kSlots; ++i) { ptx::mbar_init(full_bar(i), 4); ptx::mbar_init(empty_bar(i), 1); }
+        for (int i = 0; i < kScaleSlots; ++i) ptx::mbar_init(scale_bar(i), 8);
+        for (int h = 0; h < 2; ++h) { ptx::mbar_init(q_bar(h), 4); ptx::mbar_init(s_bar(h), 1); ptx::mbar_init(p_bar(h), 4); ptx::mbar_init(o_bar(h), 1); }
+        ptx::fence_mbar_init();
+        a.open[blockIdx.x].last = -1;
+    }
+    if (warp == 12) { ptx::tmem_alloc(tmem_slot, 512); ptx::tmem_relinquish(); }
+    zero_rest<D>(a);
+    ptx::tcgen05_fence_before_sync();
+    Cursor c = find_work(s, kRows, kTile, reinterpret_cast<long long*>(smem_raw + (q_base - raw)), a.block_limit, blockIdx.x, gridDim.x);
+    ptx::tcgen05_fence_after_sync();
+    const uint32_t tmem = *reinterpret_cast<volatile uint32_t*>(smem_raw + (tmem_slot - raw));
+    Seq q{};
+    if (c.at < c.end) q = load_seq(s, c.b);
+    bool ok = true;
+
+    if (warp < 8) {
+        // ================================================================================================ softmax
+        ptx::regs_inc<kSoftmaxRegs>();
+        const int h = warp >> 2, quad = warp & 3;
+        const int r_in = h * 128 + quad * 32 + lane;                          // row inside the block
+        const uint32_t lanes = static_cast<uint32_t>(quad * 32) << 16;
+        const uint32_t t_s = tmem + lanes + h * 128, t_o = tmem + lanes + C::kOCol + h * D;
+        uint32_t s_phase = 0, o_phase = 0;
+        int slot = 0;                                                         // of the scale ring
+        while (c.at < c.end && ok) {
+            const Range r = block_range(s, q, c.i, kRows, kTile);
+            const int todo = static_cast<int>(min(static_cast<long long>(r.tiles - c.tile), c.end - c.at));
+            const int r0 = c.i * kRows, rows = min(kRows, q.n * s.group - r0);
+            const bool half_on = h * 128 < rows, warp_on = h * 128 + quad * 32 < rows;
+            const int row = min(r_in, rows - 1);                              // rows behind the block repeat its last one
+            const int tok = (r0 + row) / s.group, head = c.h * s.group + (r0 + row) - tok * s.group;
+            const int pos = q.kv - q.n + tok;
+            const size_t out_row = static_cast<size_t>(q.q0 + tok) * s.heads + head;
+            float row_scale = fabsf(a.scale_log2);
+            if (half_on) {
+                // ---- this thread's row of q into shared memory; the sign of the softmax scale goes into it, so that the
+                // factor of the scores is not negative (nor zero)
+                const uint4* qp = reinterpret_cast<const uint4*>(a.q + (q.q0 + tok) * a.q_stride + head * a.q_head);
+                uint4 w[D / 8];
+#pragma unroll
+                for (int i = 0; i < D / 8; ++i) w[i] = __ldg(qp + i);
+                float down = a.scale_log2 > 0.0f ? 1.0f : a.scale_log2 < 0.0f ? -1.0f : 0.0f;
+                if (a.scale_log2 == 0.0f) row_scale = 1.0f;
+                if (FP8) {
+                    uint32_t m2 = 0;
+#pragma unroll
+                    for (int i = 0; i < D / 8; ++i)
+                        m2 = __vmaxu2(__vmaxu2(m2, __vmaxu2(w[i].x & 0x7FFF7FFFu, w[i].y & 0x7FFF7FFFu)), __vmaxu2(w[i].z & 0x7FFF7FFFu, w[i].w & 0x7FFF7FFFu));
+                    const uint32_t e = min(max(max(m2 & 0xFFFFu, m2 >> 16) >> 7, 1u), 253u);
+                    down *= pow2_of_field(254u - e);
+                    row_scale *= pow2_of_field(e);
+                }
+#pragma unroll
+                for (int i = 0; i < D / 8; ++i) {
+                    uint32_t v[4] = {w[i].x, w[i].y, w[i].z, w[i].w};
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) {
+                        const float lo = __uint_as_float(v[k] << 16) * down, hi = __uint_as_float(v[k] & 0xFFFF0000u) * down;
+                        v[k] = FP8 ? pack_f16x2(lo, hi) : pack_bf16x2(lo, hi);
+                    }
+                    ptx::st_shared_v4(unit_at(q_base + h * C::kSlotBytes + (i >> 3) * C::kHalfBytes, quad * 32 + lane, i & 7), v[0], v[1], v[2], v[3]);
+                }
+                ptx::fence_proxy_async_smem();
+                __syncwarp();
+                if (lane == 0) ptx::mbar_arrive(q_bar(h));
+            }
+            const int pos_lo = __shfl_sync(0xffffffffu, pos, 0), pos_hi = __shfl_sync(0xffffffffu, pos, 31);
+            float m = -INFINITY, l = 0.0f;
+            uint32_t v_field = 1;
+            for (int t = 0; t < todo && ok; ++t) {
+                const uint32_t sc = scales + slot * C::kScaleBytes;
+                if (half_on) {
+                    ok = __all_sync(0xffffffffu, ptx::mbar_wait(s_bar(h), s_phase, a.status, 2));
+                    if (!ok) break;
+                    s_phase ^= 1u;
+                    ptx::tcgen05_fence_after_sync();
+                    if (warp_on) {
+                        const int key0 = (r.tile0 + c.tile + t) * kTile;
+                        float x[kTile];
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) ptx::tmem_ld_32x32b_x32(t_s + 32 * i, reinterpret_cast<uint32_t (&)[32]>(x[32 * i]));
+                        const uint4 mask = ptx::ld_shared_v4(sc);
+                        float v_down = 1.0f, v_move = 1.0f;
+                        if (FP8) {
+                            const uint4 top = ptx::ld_shared_v4(sc + 16);
+                            const uint32_t f = max(max(top.x, top.y), max(top.z, top.w));
+                            // two powers of two of room, so that a slightly larger scale does not move the base again
+                            if (f > v_field) {
+                                const uint32_t to = min(f + 2, 253u);
+                                v_move = to - v_field < 127u ? pow2_of_field(127u - (to - v_field)) : 0.0f;
+                                v_field = to;
+                            }
+                            v_down = pow2_of_field(254u - v_field) * kRoom;
+                        }
+                        ptx::tmem_ld_wait();
+                        if (FP8) {
+#pragma unroll
+                            for (int i = 0; i < kTile; i += 4) {
+                                const uint4 k4 = ptx::ld_shared_v4(sc + 32 + 4 * i);
+                                const float2 u = ptx::mul2(make_float2(x[i], x[i + 1]), make_float2(__uint_as_float(k4.x), __uint_as_float(k4.y)));
+                                const float2 v = ptx::mul2(make_float2(x[i + 2], x[i + 3]), make_float2(__uint_as_float(k4.z), __uint_as_float(k4.w)));
+                                x[i] = u.x; x[i + 1] = u.y; x[i + 2] = v.x; x[i + 3] = v.y;
+                            }
+                        }
+                        const bool whole = (mask.x & mask.y & mask.z & mask.w) == 0xFFFFFFFFu && (!s.causal || key0 + kTile - 1 <= pos_lo) &&
+                                           (s.window == 0 || key0 > pos_hi - s.window);
+                        if (!whole) {
+                            const uint32_t mk[4] = {mask.x, mask.y, mask.z, mask.w};
+                            const int last = s.causal ? pos - key0 : kTile, first = s.window > 0 ? pos - s.window + 1 - key0 : 0;
+#pragma unroll
+                            for (int i = 0; i < kTile; ++i)
+                                if (!((mk[i >> 5] >> (i & 31)) & 1u) || i > last || i < first) x[i] = -INFINITY;
+                        }
+                        float mx[4] = {x[0], x[1], x[2], x[3]};
+#pragma unroll
+                        for (int i = 4; i < kTile - 4; i += 8)
+#pragma unroll
+                            for (int k = 0; k < 4; ++k) mx[k] = ptx::max3(mx[k], x[i + k], x[i + 4 + k]);
+#pragma unroll
+                        for (int k = 0; k < 4; ++k) mx[k] = fmaxf(mx[k], x[kTile - 4 + k]);
+                        const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * row_scale;
+                        float f = v_move;
+                        if (top > m + kLazy || m == -INFINITY) {
+                            const float mn = fmaxf(m, top);
+                            const float fm = ptx::ex2(m - (mn == -INFINITY ? 0.0f : mn));
+                            f *= fm;
+                            l *= fm;
+                            m = mn;
+                        }
+                        if (t > 0 && __any_sync(0xffffffffu, f != 1.0f)) {
+                            // O of the tiles so far, on the new base
+                            ok = __all_sync(0xffffffffu, ptx::mbar_wait(o_bar(h), o_phase ^ 1u, a.status, 3));
+                            ptx::tcgen05_fence_after_sync();
+#pragma unroll 1
+                            for (int i = 0; i < D; i += 16) {
+                                uint32_t o[16];
+                                ptx::tmem_ld_32x32b_x16(t_o + i, o);
+                                ptx::tmem_ld_wait();
+#pragma unroll
+                                for (int k = 0; k < 16; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * f);
+                                ptx::tmem_st_32x32b_x16(t_o + i, o);
+                            }
+                        }
+                        const float base = m == -INFINITY ? 0.0f : -m;
+                        const float2 rs2 = make_float2(row_scale, row_scale), b2 = make_float2(base, base), d2 = make_float2(v_down, v_down);
+                        float2 sum[2] = {make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f)};
+#pragma unroll
+                        for (int g = 0; g < kTile; g += 64) {
+                            uint32_t p[32];
+#pragma unroll
+                            for (int i = 0; i < 64; i += 4) {
+                                float2 u = ptx::fma2(make_float2(x[g + i], x[g + i + 1]), rs2, b2);
+                                float2 v = ptx::fma2(make_float2(x[g + i + 2], x[g + i + 3]), rs2, b2);
+                                u = make_float2(ptx::ex2(u.x), ptx::ex2(u.y));
+                                v = make_float2(ptx::ex2(v.x), ptx::ex2(v.y));
+                                sum[0] = ptx::add2(sum[0], u);
+                                sum[1] = ptx::add2(sum[1], v);
+                                if (FP8) {
+                                    const uint4 y = ptx::ld_shared_v4(sc + 32 + 4 * kTile + 4 * (g + i));
+                                    float2 vu = ptx::mul2(make_float2(__uint_as_float(y.x), __uint_as_float(y.y)), d2);
+                                    float2 vv = ptx::mul2(make_float2(__uint_as_float(y.z), __uint_as_float(y.w)), d2);
+                                    vu = ptx::mul2(u, vu);
+                                    vv = ptx::mul2(v, vv);
+                                    if (!whole) {                             // a masked key's p is 0, whatever its scale
+                                        vu.x = u.x == 0.0f ? 0.0f : vu.x; vu.y = u.y == 0.0f ? 0.0f : vu.y;
+                                        vv.x = v.x == 0.0f ? 0.0f : vv.x; vv.y = v.y == 0.0f ? 0.0f : vv.y;
+                                    }
+                                    p[i / 2] = pack_f16x2(vu.x, vu.y);
+                                    p[i / 2 + 1] = pack_f16x2(vv.x, vv.y);
+                                } else {
+                                    p[i / 2] = pack_bf16x2(u.x, u.y);
+                                    p[i / 2 + 1] = pack_bf16x2(v.x, v.y);
+                                }
+                            }
+                            ptx::tmem_st_32x32b_x32(t_s + g / 2, p);
+                        }
+                        sum[0] = ptx::add2(sum[0], sum[1]);
+                        l += sum[0].x + sum[0].y;
+                        ptx::tmem_st_wait();
+                    }
+                    ptx::tcgen05_fence_before_sync();
+                    __syncwarp();
+                    if (lane == 0) ptx::mbar_arrive(p_bar(h));
+                    o_phase ^= 1u;                                            // the tile's P V completes one more phase
+                }
+                // eight arrivals a tile; in a block of one half its warps arrive for the others too (which nothing would pace)
+                __syncwarp();
+                if (lane == 0 && half_on) {
+                    ptx::mbar_arrive(scale_bar(slot));
+                    if (rows <= 128) ptx::mbar_arrive(scale_bar(slot));
+                }
+                if (++slot == kScaleSlots) slot = 0;
+            }
+            if (half_on && ok) {
+                ok = __all_sync(0xffffffffu, ptx::mbar_wait(o_bar(h), o_phase ^ 1u, a.status, 3));
+                ptx::tcgen05_fence_after_sync();
+                const bool begins = c.tile == 0, ends = c.tile + todo == r.tiles;
+                const float v_up = FP8 ? pow2_of_field(v_field) * (1.0f / kRoom) : 1.0f;
+                const int part = 2 * blockIdx.x + (begins ? 1 : 0);
+                float* po = a.part + static_cast<size_t>(part) * kRows * (D + 2);
+                const bool whole_block = begins && ends;
+                const float f = !whole_block ? v_up : l == 0.0f ? 0.0f : __frcp_rn(l) * v_up;
+                if (warp_on) {
+#pragma unroll 1
+                    for (int i = 0; i < D; i += 32) {
+                        uint32_t o[32];
+                        ptx::tmem_ld_32x32b_x32(t_o + i, o);
+                        ptx::tmem_ld_wait();
+                        if (r_in < rows) {
+                            if (whole_block) {
+#pragma unroll
+                                for (int k = 0; k < 32; k += 8) {
+                                    uint32_t w[4];
+#pragma unroll
+                                    for (int e = 0; e < 4; ++e) w[e] = pack_bf16x2(__uint_as_float(o[k + 2 * e]) * f, __uint_as_float(o[k + 2 * e + 1]) * f);
+                                    *reinterpret_cast<uint4*>(a.out + out_row * D + i + k) = make_uint4(w[0], w[1], w[2], w[3]);
+                                }
+                            } else {
+#pragma unroll
+                                for (int k = 0; k < 32; k += 4)
+                                    *reinterpret_cast<float4*>(po + r_in * D + i + k) = make_float4(__uint_as_float(o[k]) * f, __uint_as_float(o[k + 1]) * f,
+                                                                                                    __uint_as_float(o[k + 2]) * f, __uint_as_float(o[k + 3]) * f);
+                            }
+                        }
+                    }
+                    if (r_in < rows) {
+                        if (!whole_block) *reinterpret_cast<float2*>(po + kRows * D + r_in * 2) = make_float2(m, l);
+                        else if (a.lse != nullptr) a.lse[out_row] = lse_of(m, l);
+                    }
+                }
+                ptx::tcgen05_fence_before_sync();
+                if (threadIdx.x == 0 && begins && !ends) {
+                    Open* op = a.open + blockIdx.x;
+                    op->token0 = q.q0; op->r0 = r0; op->rows = rows; op->h = c.h;
+                    op->last = owner(c, c.at + r.tiles - 1);
+                }
+            }
+            c.at += todo;
+            if (c.at < c.end) next_block(s, c, q, kRows);
+        }
+    } else if (warp < 12) {
+        // ================================================================================================ loaders
+        ptx::regs_dec<kLoaderRegs>();
+        const int lw = warp - 8;                                              // keys 32 * lw .. + 31 of a tile
+        int slot = 0, sslot = 0;
+        uint32_t phase = 0, sphase = 0;
+        int pending = -1;                                                     // bf16: the slot whose copies are in flight
+        while (c.at < c.end && ok) {
+            const Range r = block_range(s, q, c.i, kRows, kTile);
+            const int todo = static_cast<int>(min(static_cast<long long>(r.tiles - c.tile), c.end - c.at));
+            const int* table = s.table + static_cast<size_t>(c.b) * s.max_pages;
+            // the cache row of this lane's key of a tile, -1 for none
+            auto row_of = [&](int tile) {
+                const int key = tile * kTile + lw * 32 + lane;
+                if (key < r.lo || key >= r.hi) return -1;
+                const int page = __ldg(table + (key >> s.page_shift));
+                if (page < 0 || page >= s.num_pages) return -1;
+                return ((page * s.kv_heads + c.h) << s.page_shift) + (key & ((1 << s.page_shift) - 1));
+            };
+            int row = row_of(r.tile0 + c.tile);
+            constexpr int kPerRow = (FP8 ? D : 2 * D) / 16;                   // 16-byte pieces of a row
+            constexpr int kRowsAt = 32 / kPerRow;                             // rows a warp instruction covers
+            const int piece = lane % kPerRow, sub = lane / kPerRow;
+            constexpr int kGroup = FP8 ? (D == 128 ? 4 : 2) : 1;              // instructions of half an item
+            uint4 buf[2][kGroup];
+            auto fetch = [&](uint4 (&to)[kGroup], const void* cache, int rows_of_lane, int half) {
+#pragma unroll
+                for (int i = 0; i < kGroup; ++i) {
+                    const int from = __shfl_sync(0xffffffffu, rows_of_lane, (half * kGroup + i) * kRowsAt + sub);
+                    to[i] = from >= 0 ? __ldg(reinterpret_cast<const uint4*>(static_cast<const uint8_t*>(cache) + static_cast<size_t>(from) * D) + piece)
+                                      : make_uint4(0, 0, 0, 0);
+                }
+            };
+            auto store = [&](const uint4 (&from)[kGroup], uint32_t to, int half) {
+#pragma unroll
+                for (int i = 0; i < kGroup; ++i) {
+                    const int rr = lw * 32 + (half * kGroup + i) * kRowsAt + sub;
+                    const uint32_t w[4] = {from[i].x, from[i].y, from[i].z, from[i].w};
+                    uint32_t v[8];
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) { v[2 * k] = ptx::e4m3x2_lo(w[k]); v[2 * k + 1] = ptx::e4m3x2_hi(w[k]); }
+                    // 16 elements = units 2p and 2p + 1 of the row; a row of 128's upper half stores them in the other order, so that
+                    // its eight lanes hit eight different units
+                    const uint32_t column = to + (piece >> 2) * C::kHalfBytes;
+                    const int unit = (piece & 3) * 2;
+                    const bool swap = D == 128 && piece >= 4;
+                    const uint32_t at0 = unit_at(column, rr, unit + (swap ? 1 : 0)), at1 = unit_at(column, rr, unit + (swap ? 0 : 1));
+                    ptx::st_shared_v4(at0, swap ? v[4] : v[0], swap ? v[5] : v[1], swap ? v[6] : v[2], swap ? v[7] : v[3]);
+                    ptx::st_shared_v4(at1, swap ? v[0] : v[4], swap ? v[1] : v[5], swap ? v[2] : v[6], swap ? v[3] : v[7]);
+                }
+            };
+            if (FP8) { fetch(buf[0], a.k_cache, row, 0); fetch(buf[1], a.k_cache, row, 1); }
+            for (int t = 0; t < todo && ok; ++t) {
+                const int next = t + 1 < todo ? row_of(r.tile0 + c.tile + t + 1) : -1;
+                float ks = 0.0f, vs = 0.0f;
+                if (FP8 && row >= 0) { ks = __ldg(a.k_scale + row); vs = __ldg(a.v_scale + row); }
+                // ---- the tile's mask and scales
+                ok = __all_sync(0xffffffffu, ptx::mbar_wait(scale_bar(sslot), sphase ^ 1u, a.status, 4));
+                if (!ok) break;
+                {
+                    const uint32_t sc = scales + sslot * C::kScaleBytes;
+                    uint8_t* scp = smem_raw + (sc - raw);
+                    const uint32_t there = __ballot_sync(0xffffffffu, row >= 0);
+                    uint32_t top = __float_as_uint(vs) & 0x7FFFFFFFu;
+                    top = __reduce_max_sync(0xffffffffu, top < 0x7F800000u ? top : 0u);
+                    if (lane == 0) {
+                        reinterpret_cast<uint32_t*>(scp)[lw] = there;
+                        reinterpret_cast<uint32_t*>(scp)[4 + lw] = (top >> 23) + 1;
+                    }
+                    if (FP8) {
+                        reinterpret_cast<float*>(scp + 32)[lw * 32 + lane] = ks;
+                        reinterpret_cast<float*>(scp + 32)[kTile + lw * 32 + lane] = vs;
+                    }
+                    if (++sslot == kScaleSlots) { sslot = 0; sphase ^= 1u; }
+                }
+                // ---- keys, then values
+#pragma unroll
+                for (int kv = 0; kv < 2; ++kv) {
+                    ok = __all_sync(0xffffffffu, ptx::mbar_wait(empty_bar(slot), phase ^ 1u, a.status, 1));
+                    if (!ok) break;
+                    const uint32_t to = ring + slot * C::kSlotBytes;
+                    if constexpr (FP8) {
+                        store(buf[0], to, 0);
+                        if (kv == 0) fetch(buf[0], a.v_cache, row, 0);
+                        else fetch(buf[0], a.k_cache, next, 0);
+                        store(buf[1], to, 1);
+                        if (kv == 0) fetch(buf[1], a.v_cache, row, 1);
+                        else fetch(buf[1], a.k_cache, next, 1);
+                        ptx::fence_proxy_async_smem();
+                        __syncwarp();
+                        if (lane == 0) ptx::mbar_arrive(full_bar(slot));
+                    } else {
+                        const uint8_t* cache = static_cast<const uint8_t*>(kv == 0 ? a.k_cache : a.v_cache);
+#pragma unroll
+                        for (int i = 0; i < 32 / kRowsAt; ++i) {
+                            const int from = __shfl_sync(0xffffffffu, row, i * kRowsAt + sub);
+                            ptx::cp_async_16(unit_at(to + (piece >> 3) * C::kHalfBytes, lw * 32 + i * kRowsAt + sub, piece & 7),
+                                             cache + static_cast<size_t>(max(from, 0)) * (2 * D) + piece * 16, from >= 0 ? 16u : 0u);
+                        }
+                        ptx::cp_async_commit();
+                        if (pending >= 0) {                                   // publish the one before while this one is in flight
+                            ptx::cp_async_wait<1>();
+                            ptx::fence_proxy_async_smem();
+                            __syncwarp();
+                            if (lane == 0) ptx::mbar_arrive(full_bar(pending));
+                        }
+                        pending = slot;
+                    }
+                    if (++slot == C::kSlots) { slot = 0; phase ^= 1u; }
+                }
+                row = next;
+            }
+            c.at += todo;
+            if (c.at < c.end) next_block(s, c, q, kRows);
+        }
+        if (!FP8) {
+            ptx::cp_async_wait<0>();
+            if (pending >= 0 && ok) {
+                ptx::fence_proxy_async_smem();
+                __syncwarp();
+                if (lane == 0) ptx::mbar_arrive(full_bar(pending));
+            }
+        }
+    } else {
+        // ================================================================================================ products
+        ptx::regs_dec<kMmaRegs>();
+        if (warp == 12 && ptx::elect_one()) {
+            constexpr uint32_t fmt = FP8 ? 0u : 1u;                           // fp16 / bf16
+            constexpr uint32_t id_s = ptx::umma_idesc(fmt, fmt, 128, kTile);
+            constexpr uint32_t id_o = ptx::umma_idesc(fmt, fmt, 128, D) | ptx::kIdescBMnMajor;
+            int slot = 0;
+            uint32_t phase = 0, q_phase[2] = {0, 0}, p_phase[2] = {0, 0};
+            auto scores = [&](int h, uint32_t k_at) {
+                const uint64_t dq = ptx::smem_desc_sw128_kmajor(q_base + h * C::kSlotBytes), dk = ptx::smem_desc_sw128_kmajor(k_at);
+#pragma unroll
+                for (int i = 0; i < D / 16; ++i) {
+                    const uint64_t step = (i >> 2) * (C::kHalfBytes >> 4) + 2 * (i & 3);
+                    ptx::umma_f16(tmem + h * 128, dq + step, dk + step, id_s, i > 0);
+                }
+                ptx::umma_commit(s_bar(h));
+            };
+            while (c.at < c.end && ok) {
+                const Range r = block_range(s, q, c.i, kRows, kTile);
+                const int todo = static_cast<int>(min(static_cast<long long>(r.tiles - c.tile), c.end - c.at));
+                const int halves = min(kRows, q.n * s.group - c.i * kRows) > 128 ? 2 : 1;
+                // scores of the first tile
+                ok = ptx::mbar_wait(full_bar(slot), phase, a.status, 5);
+                for (int h = 0; h < halves && ok; ++h) {
+                    ok = ptx::mbar_wait(q_bar(h), q_phase[h], a.status, 6);
+                    q_phase[h] ^= 1u;
+                    ptx::tcgen05_fence_after_sync();
+                    if (ok) scores(h, ring + slot * C::kSlotBytes);
+                }
+                ptx::umma_commit(empty_bar(slot));
+                if (++slot == C::kSlots) { slot = 0; phase ^= 1u; }
+                for (int t = 0; t < todo && ok; ++t) {
+                    const int v_slot = slot;
+                    const uint32_t v_phase = phase;
+                    if (++slot == C::kSlots) { slot = 0; phase ^= 1u; }
+                    const bool on = t + 1 < todo;
+                    const int k_slot = slot;
+                    const uint32_t k_phase = phase;
+                    if (on && ++slot == C::kSlots) { slot = 0; phase ^= 1u; }
+                    for (int h = 0; h < halves && ok; ++h) {
+                        if (h == 0) ok = ptx::mbar_wait(full_bar(v_slot), v_phase, a.status, 5);
+                        ok = ok && ptx::mbar_wait(p_bar(h), p_phase[h], a.status, 7);
+                        if (!ok) break;
+                        p_phase[h] ^= 1u;
+                        ptx::tcgen05_fence_after_sync();
+                        const uint64_t dv = ptx::smem_desc_sw128_mnmajor(ring + v_slot * C::kSlotBytes, C::kHalfBytes);
+#pragma unroll
+                        for (int i = 0; i < kTile / 16; ++i)                  // 16 keys: 8 columns of P, 2 KB of each column of V
+                            ptx::umma_f16_ts(tmem + C::kOCol + h * D, tmem + h * 128 + 8 * i, dv + (2048 >> 4) * i, id_o, t > 0 || i > 0);
+                        ptx::umma_commit(o_bar(h));
+                        if (h == halves - 1) ptx::umma_commit(empty_bar(v_slot));
+                        if (on) {
+                            if (h == 0) {
+                                ok = ptx::mbar_wait(full_bar(k_slot), k_phase, a.status, 5);
+                                if (!ok) break;
+                                ptx::tcgen05_fence_after_sync();
+                            }
+                            scores(h, ring + k_slot * C::kSlotBytes);
+                            if (h == halves - 1) ptx::umma_commit(empty_bar(k_slot));
+                        }
+                    }
+                }
+                c.at += todo;
+                if (c.at < c.end) next_block(s, c, q, kRows);
+            }
+        }
+        __syncwarp();
+    }
+    ptx::tcgen05_fence_before_sync();
+    __syncthreads();
+    if (warp == 12) {
+        ptx::tcgen05_fence_after_sync();
+        ptx::tmem_dealloc(tmem, 512);
+    }
+}
+
+template <int D, bool FP8>
+int launch(const Args& args, cudaStream_t stream)
+{
+    using C = Cfg<D, FP8>;
+    Args a = args;
+    auto kernel = attn_chunk_kernel<D, FP8>;
+    static bool configured[64] = {};
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e != cudaSuccess) return e;
+    if (dev >= 64 || !configured[dev]) {
+        e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmemBytes);
+        if (e != cudaSuccess) return e;
+        if (dev < 64) configured[dev] = true;
+    }
+    if (static_cast<long long>(a.s.seqs) * 8 > C::kQBytes + C::kSlots * C::kSlotBytes) return cudaErrorInvalidValue;
+    a.block_limit = static_cast<int>((static_cast<long long>(a.max_q) * a.s.group + kRows - 1) / kRows);
+    const int ctas = num_sms();
+    kernel<<<ctas, kThreads, C::kSmemBytes, stream>>>(a);
+    e = cudaGetLastError();
+    if (e != cudaSuccess) return e;
+    return launch_combine<D>(a, ctas, kRows, stream);
+}
+
+}  // namespace chunk
+
+int attn_chunk(const Args& a, int head_dim, bool fp8, cudaStream_t stream)
+{
+    if (head_dim == 64) return fp8 ? chunk::launch<64, true>(a, stream) : chunk::launch<64, false>(a, stream);
+    return fp8 ? chunk::launch<128, true>(a, stream) : chunk::launch<128, false>(a, stream);
+}
+
+size_t attn_chunk_part_bytes(int head_dim) { return static_cast<size_t>(num_sms()) * 2 * chunk::kRows * (head_dim + 2) * sizeof(float); }
+
+}  // namespace paged
+}  // namespace b200q

@@ -80,6 +80,9 @@ __device__ __forceinline__ uint32_t pack_f16x2(float lo, float hi)
     const __half2 v = __floats2half2_rn(lo, hi);
     return *reinterpret_cast<const uint32_t*>(&v);
 }
+// p * scale / (power of two above the largest scale) is kept times 2^15, so that fp16 holds it from 2^15 down: what falls below
+// its normal range is 2^-29 of the largest value in the cache
+constexpr float kRoom = 32768.0f;
 __device__ __forceinline__ float pow2_of_field(uint32_t e) { return __uint_as_float(e << 23); }      // 2^(e - 127), 1 <= e <= 254
 
 template <int D, bool FP8, int NT>
@@ -294,7 +297,7 @@ attn_split_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
                     }
                     f = min((__reduce_max_sync(0xffffffffu, f) >> 23) + 1, 253u);
                     if (f > v_field) { v_move = f - v_field < 127u ? pow2_of_field(127u - (f - v_field)) : 0.0f; v_field = f; }
-                    v_down = pow2_of_field(254u - v_field);
+                    v_down = pow2_of_field(254u - v_field) * kRoom;
                 }
                 // keys that are not there for the whole block, that come after a row, or that have left its window
                 const bool whole = valid == 0xFFFFu && (!s.causal || key0 + 15 <= pos_lo) && (s.window == 0 || key0 > pos_hi - s.window);
@@ -415,7 +418,7 @@ attn_split_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
                 if (g == 0) state_p[warp * kRows + 8 * nt + 2 * cc + u] = make_float2(m[nt][u], l[nt][u]);
             }
         ptx::named_barrier(1, 32 * kConsumers);
-        const float v_up = FP8 ? pow2_of_field(v_field) : 1.0f;
+        const float v_up = FP8 ? pow2_of_field(v_field) * (1.0f / kRoom) : 1.0f;
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll

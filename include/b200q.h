@@ -178,6 +178,7 @@ int b200q_paged_attention(const void* q, const void* k_cache, const void* v_cach
                           int num_pages, int page_size, int fp8, float softmax_scale, int causal, int window, int zero_rest,
                           void* workspace, void* stream);
 size_t b200q_paged_attention_workspace_bytes(int head_dim);
+int b200q_paged_set_impl(int impl);   /* attention kernel: 0 = by the rows per kv head (default), 1 = split-KV, 2 = tensor-core */
 
 /* Tuning knobs.  Every b200q_*_set_* function changes a PROCESS-WIDE setting read by later calls on any
  * device; they are not synchronised with calls in flight on other host threads — set them once at

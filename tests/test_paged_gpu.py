@@ -10,6 +10,15 @@ pytestmark = pytest.mark.gpu
 NAN = float("nan")
 
 
+@pytest.fixture(params=["by size", "split", "chunk"])
+def kernel(request):
+    """The attention test that asks for it runs with the kernel the sizes choose and with each of the two."""
+    import cudaop_b200 as ops
+    assert ops.lib().b200q_paged_set_impl(["by size", "split", "chunk"].index(request.param)) == 0
+    yield request.param
+    ops.lib().b200q_paged_set_impl(0)
+
+
 # ------------------------------------------------------------------------------------------------------ plain forms
 def quantise_rows(x):
     """Per-row E4M3 by the library's rule, in the same 32-bit steps: (bytes, scales)."""
@@ -229,7 +238,7 @@ def test_read_back(dim, page, kv_heads, fp8):
 @pytest.mark.parametrize("fp8", [True, False])
 @pytest.mark.parametrize("dim", [64, 128])
 @pytest.mark.parametrize("heads,kv_heads", [(1, 1), (8, 8), (8, 1), (12, 2), (32, 4), (40, 2)])
-def test_one_token(heads, kv_heads, dim, fp8):
+def test_one_token(kernel, heads, kv_heads, dim, fp8):
     """Decode: lengths from one token to many tiles, at and around the borders of pages and tiles."""
     kv = [1, 2, 15, 16, 17, 63, 64, 65, 127, 128, 129, 500, 1000, 3]
     b = Batch([1] * len(kv), kv, heads, kv_heads, dim, page=16, fp8=fp8)
@@ -238,7 +247,7 @@ def test_one_token(heads, kv_heads, dim, fp8):
 
 @pytest.mark.parametrize("page", [16, 32, 64, 128])
 @pytest.mark.parametrize("dim,fp8", [(128, True), (64, True), (128, False), (64, False)])
-def test_page_sizes_and_mixed_chunks(dim, fp8, page):
+def test_page_sizes_and_mixed_chunks(kernel, dim, fp8, page):
     n = [1, 5, 0, 33, 2, 130, 64]
     kv = [300, 5, 40, 200, 1000, 131, 64]
     b = Batch(n, kv, 8, 2, dim, page, fp8)
@@ -247,20 +256,20 @@ def test_page_sizes_and_mixed_chunks(dim, fp8, page):
 
 @pytest.mark.parametrize("dim,fp8", [(128, True), (64, False)])
 @pytest.mark.parametrize("window", [1, 2, 16, 100, 5000])
-def test_windows(window, dim, fp8):
+def test_windows(kernel, window, dim, fp8):
     b = Batch([1, 7, 100, 20, 300], [900, 7, 400, 21, 700], 8, 2, dim, 16, fp8)
     b.check(b.call(window=window), window=window)
 
 
 @pytest.mark.parametrize("dim,fp8", [(64, True), (128, False), (128, True)])
-def test_every_key_is_seen_without_causal(dim, fp8):
+def test_every_key_is_seen_without_causal(kernel, dim, fp8):
     b = Batch([1, 7, 100, 300], [900, 7, 400, 700], 8, 4, dim, 32, fp8)
     b.check(b.call(causal=False), causal=False)
 
 
 @pytest.mark.parametrize("dim,fp8", [(128, True), (128, False), (64, True)])
 @pytest.mark.parametrize("causal", [True, False])
-def test_rows_that_see_nothing(causal, dim, fp8):
+def test_rows_that_see_nothing(kernel, causal, dim, fp8):
     """Fewer cached tokens than new ones, none at all, a negative length: zero rows and lse -inf."""
     b = Batch([4, 3, 1, 40, 2, 300], [2, 0, 0, 7, -3, 290], 8, 2, dim, 16, fp8)
     b.check(b.call(causal=causal), causal=causal)
@@ -268,7 +277,7 @@ def test_rows_that_see_nothing(causal, dim, fp8):
 
 @pytest.mark.parametrize("dim,fp8", [(128, True), (64, False)])
 @pytest.mark.parametrize("n", [1, 140])
-def test_pages_that_are_not_in_the_cache_are_left_out(n, dim, fp8):
+def test_pages_that_are_not_in_the_cache_are_left_out(kernel, n, dim, fp8):
     b = Batch([n, n], [400, 150], 8, 2, dim, 16, fp8)
     absent = [(0, 0), (0, 7), (0, 24), (1, 3)]
     for i, (s, col) in enumerate(absent):
@@ -279,7 +288,7 @@ def test_pages_that_are_not_in_the_cache_are_left_out(n, dim, fp8):
     b.check(b.call(), absent=absent[:3] + [(1, col) for col in range(10)])
 
 
-def test_length_longer_than_the_table():
+def test_length_longer_than_the_table(kernel):
     """Keys behind the table's last page are not there; positions still count from kv_lens."""
     b = Batch([3], [100], 4, 2, 128, 16, True, wide=0)
     b.kv = [130]                                                     # 7 pages hold 112 slots; 100 are written, the rest is NaN
@@ -288,7 +297,7 @@ def test_length_longer_than_the_table():
 
 
 @pytest.mark.parametrize("n", [1, 9, 200])
-def test_strided_queries_scale_and_given_output(n):
+def test_strided_queries_scale_and_given_output(kernel, n):
     """Queries inside a fused projection's output; rows of no sequence stay as they are in a given output, else are zero."""
     b = Batch([n, 2 * n], [300, 450], 8, 2, 128, 64, True)
     T = 3 * n
@@ -307,7 +316,7 @@ def test_strided_queries_scale_and_given_output(n):
 
 
 @pytest.mark.parametrize("n,fp8", [(1, True), (1, False), (40, True), (200, False)])
-def test_large_scores_and_equal_runs(n, fp8):
+def test_large_scores_and_equal_runs(kernel, n, fp8):
     """Scores of hundreds: the running maximum moves at every tile; and two runs give the same bits."""
     b = Batch([n, n], [1000, 777], 16, 2, 128, 32, fp8, seed=5)
     b.q = (b.q.float() * 20).bfloat16()
@@ -317,7 +326,7 @@ def test_large_scores_and_equal_runs(n, fp8):
     assert torch.equal(got[0], again[0]) and torch.equal(got[1], again[1])
 
 
-def test_a_nan_key_reaches_the_rows_that_see_it():
+def test_a_nan_key_reaches_the_rows_that_see_it(kernel):
     """E4M3 rows with NaN: rows that see the token are NaN, rows in front of it are as if it were not there."""
     import cudaop_b200 as ops
     b = Batch([8], [64], 2, 1, 128, 16, True)
@@ -331,7 +340,7 @@ def test_a_nan_key_reaches_the_rows_that_see_it():
     assert ((out[:4].double().cpu() - want[:4]).abs() <= tol[:4]).all()
 
 
-def test_many_sequences_and_a_chunk_bound_that_is_too_small():
+def test_many_sequences_and_a_chunk_bound_that_is_too_small(kernel):
     g = np.random.default_rng(3)
     kv = [int(x) for x in g.integers(1, 90, 700)]
     b = Batch([1] * 700, kv, 4, 2, 64, 16, True)
@@ -341,7 +350,7 @@ def test_many_sequences_and_a_chunk_bound_that_is_too_small():
     b.check(b.call(max_q=10 ** 6))
 
 
-def test_offsets_that_pass_32_bits():
+def test_offsets_that_pass_32_bits(kernel):
     """A cache of more than 2^32 elements, its tokens at both ends."""
     import cudaop_b200 as ops
     pages, heads, page, dim = 280000, 8, 16, 128
