@@ -6,7 +6,8 @@
 //   warps 0-3, 4-7   softmax of half 0 and 1, a thread per row (= TMEM lane): no shuffles.  They also load the rows of q at the
 //                    start of a block and write the output at its end.
 //   warps 8-11       loaders: keys and values into a ring of [128 keys][D] 16-bit slots, 128-byte swizzle, K(0) V(0) K(1) V(1) ...
-//                    An E4M3 cache is read into registers, converted (exactly, to fp16) and stored; a bf16 cache goes by cp.async.
+//                    Both caches go by cp.async, a bf16 one into the slot, an E4M3 one into a staging area from which the thread that
+//                    asked for the bytes converts them (exactly, to fp16).
 //                    Keys that are not there are stored as zeros, so whatever lies in their place reaches no product.
 //   warp 12          issues the products.  S_h = Q_h K^T (both from shared memory) into TMEM; the softmax turns S_h into P_h (fp16 or
 //                    bf16) over the same TMEM columns; O_h += P_h V with P_h as the tensor-memory operand and V as it lies, rows of
@@ -24,26 +25,30 @@ namespace chunk {
 
 constexpr int kRows = 256, kTile = 128, kThreads = 512;
 constexpr int kScaleSlots = 4;
-constexpr int kSoftmaxRegs = 192, kLoaderRegs = 88, kMmaRegs = 40;            // 2 * 192 + 88 + 40 = 4 * 128
+constexpr int kSoftmaxRegs = 200, kLoaderRegs = 72, kMmaRegs = 40;            // 2 * 200 + 72 + 40 = 4 * 128
 constexpr float kLazy = 4.0f;                  // p is at most 2^4
-// p * scale / (largest scale) is kept times 2^11, so that fp16 holds it from 2^15 down: what falls below its normal range is 2^-29 of the
-// largest value in the cache
-constexpr float kRoom = 2048.0f;
 
 template <int D, bool FP8>
 struct Cfg {
     static constexpr int kHalves = D / 64;                                    // 128-byte columns of a 16-bit row
     static constexpr int kHalfBytes = kTile * 128;
     static constexpr int kSlotBytes = kHalves * kHalfBytes;
-    static constexpr int kSlots = D == 128 ? 4 : 6;
+    static constexpr int kSlots = D == 64 ? 6 : FP8 ? 3 : 4;
+    static constexpr int kStagedBytes = FP8 ? kTile * D : 0;                  // E4M3 bytes of a tile of keys or values, on their way
     static constexpr int kQBytes = 2 * kSlotBytes;
-    // per tile: mask words, largest value scales (4 each), then key scales and value scales
-    static constexpr int kScaleBytes = 32 + (FP8 ? 2 * kTile * 4 : 0);
-    static constexpr int kBars = 2 * kSlots + kScaleSlots + 8;
-    static constexpr int kSmemBytes = 1024 + kQBytes + kSlots * kSlotBytes + kScaleSlots * kScaleBytes + kBars * 8 + 16;
+    // per tile: mask words, largest value scales, words of the keys whose value scale is not finite (4 each), key scales, value scales
+    static constexpr int kScaleAt = 48;
+    static constexpr int kScaleBytes = kScaleAt + (FP8 ? 2 * kTile * 4 : 0);
+    static constexpr int kBars = 2 * kSlots + kScaleSlots + 10;
+    static constexpr int kSmemBytes = 1024 + kQBytes + kSlots * kSlotBytes + 3 * kStagedBytes + kScaleSlots * kScaleBytes + kBars * 8 + 32;
     static constexpr int kOCol = 256;
 };
 
+// p * scale / (power of two above the largest scale) is kept times kRoom = 2^11: at most 2^15, and fp16 starts to lose bits only where
+// it is below 2^-25 of the largest
+constexpr int kRoomLog2 = 11;
+// log2 of kRoom / 2^(v_field - 127)
+__device__ __forceinline__ float log2_factor(uint32_t v_field) { return static_cast<float>(kRoomLog2 + 127 - static_cast<int>(v_field)); }
 __device__ __forceinline__ float pow2_of_field(uint32_t e) { return __uint_as_float(e << 23); }
 __device__ __forceinline__ uint32_t pack_f16x2(float lo, float hi)
 {
@@ -62,7 +67,8 @@ attn_chunk_kernel(const Args a)
     const uint32_t raw = ptx::smem_u32(smem_raw);
     const uint32_t q_base = (raw + 1023u) & ~1023u;
     const uint32_t ring = q_base + C::kQBytes;
-    const uint32_t scales = ring + C::kSlots * C::kSlotBytes;
+    const uint32_t staging = ring + C::kSlots * C::kSlotBytes;
+    const uint32_t scales = staging + 3 * C::kStagedBytes;
     const uint32_t bars = scales + kScaleSlots * C::kScaleBytes;
     auto full_bar = [&](int s) { return bars + 8u * s; };                     // a slot holds its tile
     auto empty_bar = [&](int s) { return bars + 8u * (C::kSlots + s); };
@@ -70,9 +76,10 @@ attn_chunk_kernel(const Args a)
     const uint32_t more = bars + 8u * (2 * C::kSlots + kScaleSlots);
     auto q_bar = [&](int h) { return more + 8u * h; };
     auto s_bar = [&](int h) { return more + 8u * (2 + h); };                  // scores of half h are in TMEM
-    auto p_bar = [&](int h) { return more + 8u * (4 + h); };                  // P of half h is in TMEM
-    auto o_bar = [&](int h) { return more + 8u * (6 + h); };                  // P V of half h is done
+    auto p_bar = [&](int h, int k) { return more + 8u * (4 + 2 * h + k); };   // P of half h, keys 64 * k .., is in TMEM
+    auto o_bar = [&](int h) { return more + 8u * (8 + h); };                  // P V of half h is done
     const uint32_t tmem_slot = bars + C::kBars * 8;
+    int* block_info = reinterpret_cast<int*>(smem_raw + (tmem_slot + 4 - raw));        // for the products: tiles (0: no more blocks), halves
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const Shape& s = a.s;
 
@@ -80,7 +87,7 @@ attn_chunk_kernel(const Args a)
     if (threadIdx.x == 0) {
         for (int i = 0; i < C::kSlots; ++i) { ptx::mbar_init(full_bar(i), 4); ptx::mbar_init(empty_bar(i), 1); }
         for (int i = 0; i < kScaleSlots; ++i) ptx::mbar_init(scale_bar(i), 8);
-        for (int h = 0; h < 2; ++h) { ptx::mbar_init(q_bar(h), 4); ptx::mbar_init(s_bar(h), 1); ptx::mbar_init(p_bar(h), 4); ptx::mbar_init(o_bar(h), 1); }
+        for (int h = 0; h < 2; ++h) { ptx::mbar_init(q_bar(h), 4); ptx::mbar_init(s_bar(h), 1); ptx::mbar_init(p_bar(h, 0), 4); ptx::mbar_init(p_bar(h, 1), 4); ptx::mbar_init(o_bar(h), 1); }
         ptx::fence_mbar_init();
         a.open[blockIdx.x].last = -1;
     }
@@ -142,11 +149,14 @@ attn_chunk_kernel(const Args a)
                     ptx::st_shared_v4(unit_at(q_base + h * C::kSlotBytes + (i >> 3) * C::kHalfBytes, quad * 32 + lane, i & 7), v[0], v[1], v[2], v[3]);
                 }
                 ptx::fence_proxy_async_smem();
+                if (threadIdx.x == 0) { block_info[0] = todo; block_info[1] = rows > 128 ? 2 : 1; }
                 __syncwarp();
                 if (lane == 0) ptx::mbar_arrive(q_bar(h));
             }
             const int pos_lo = __shfl_sync(0xffffffffu, pos, 0), pos_hi = __shfl_sync(0xffffffffu, pos, 31);
-            float m = -INFINITY, l = 0.0f;
+            // m: the base of the row's exponents.  For an E4M3 cache p is kept times kRoom / 2^v_exp, 2^v_exp a power of two above the
+            // largest value scale so far: sum and output alike, so it cancels, and m - log2 of it is the base that the parts carry.
+            float m = -INFINITY, l = 0.0f, poison = 0.0f;
             uint32_t v_field = 1;
             for (int t = 0; t < todo && ok; ++t) {
                 const uint32_t sc = scales + slot * C::kScaleBytes;
@@ -161,8 +171,10 @@ attn_chunk_kernel(const Args a)
 #pragma unroll
                         for (int i = 0; i < 4; ++i) ptx::tmem_ld_32x32b_x32(t_s + 32 * i, reinterpret_cast<uint32_t (&)[32]>(x[32 * i]));
                         const uint4 mask = ptx::ld_shared_v4(sc);
-                        float v_down = 1.0f, v_move = 1.0f;
+                        float v_move = 1.0f;
+                        uint4 odd = make_uint4(0, 0, 0, 0);
                         if (FP8) {
+                            odd = ptx::ld_shared_v4(sc + 32);
                             const uint4 top = ptx::ld_shared_v4(sc + 16);
                             const uint32_t f = max(max(top.x, top.y), max(top.z, top.w));
                             // two powers of two of room, so that a slightly larger scale does not move the base again
@@ -171,27 +183,38 @@ attn_chunk_kernel(const Args a)
                                 v_move = to - v_field < 127u ? pow2_of_field(127u - (to - v_field)) : 0.0f;
                                 v_field = to;
                             }
-                            v_down = pow2_of_field(254u - v_field) * kRoom;
                         }
                         ptx::tmem_ld_wait();
                         if (FP8) {
 #pragma unroll
                             for (int i = 0; i < kTile; i += 4) {
-                                const uint4 k4 = ptx::ld_shared_v4(sc + 32 + 4 * i);
+                                const uint4 k4 = ptx::ld_shared_v4(sc + C::kScaleAt + 4 * i);
                                 const float2 u = ptx::mul2(make_float2(x[i], x[i + 1]), make_float2(__uint_as_float(k4.x), __uint_as_float(k4.y)));
                                 const float2 v = ptx::mul2(make_float2(x[i + 2], x[i + 3]), make_float2(__uint_as_float(k4.z), __uint_as_float(k4.w)));
                                 x[i] = u.x; x[i + 1] = u.y; x[i + 2] = v.x; x[i + 3] = v.y;
                             }
                         }
+                        // keys 32 * w .. + 31 of the tile that this row's position lets it see, as bits
+                        auto visible = [&](int w) {
+                            const int last = s.causal ? pos - key0 - 32 * w : 31, first = s.window > 0 ? pos - s.window + 1 - key0 - 32 * w : 0;
+                            const uint32_t upto = last < 0 ? 0u : last >= 31 ? 0xFFFFFFFFu : (2u << last) - 1u;
+                            return first <= 0 ? upto : first > 31 ? 0u : upto & ~((1u << first) - 1u);
+                        };
                         const bool whole = (mask.x & mask.y & mask.z & mask.w) == 0xFFFFFFFFu && (!s.causal || key0 + kTile - 1 <= pos_lo) &&
                                            (s.window == 0 || key0 > pos_hi - s.window);
                         if (!whole) {
                             const uint32_t mk[4] = {mask.x, mask.y, mask.z, mask.w};
-                            const int last = s.causal ? pos - key0 : kTile, first = s.window > 0 ? pos - s.window + 1 - key0 : 0;
 #pragma unroll
-                            for (int i = 0; i < kTile; ++i)
-                                if (!((mk[i >> 5] >> (i & 31)) & 1u) || i > last || i < first) x[i] = -INFINITY;
+                            for (int w = 0; w < 4; ++w) {
+                                const uint32_t seen = mk[w] & visible(w);
+#pragma unroll
+                                for (int i = 0; i < 32; ++i)
+                                    if (!((seen >> i) & 1u)) x[32 * w + i] = -INFINITY;
+                            }
                         }
+                        if (FP8 && (odd.x | odd.y | odd.z | odd.w) != 0u &&
+                            ((odd.x & visible(0)) | (odd.y & visible(1)) | (odd.z & visible(2)) | (odd.w & visible(3))) != 0u)
+                            poison = __uint_as_float(0x7FC00000u);
                         float mx[4] = {x[0], x[1], x[2], x[3]};
 #pragma unroll
                         for (int i = 4; i < kTile - 4; i += 8)
@@ -205,9 +228,9 @@ attn_chunk_kernel(const Args a)
                             const float mn = fmaxf(m, top);
                             const float fm = ptx::ex2(m - (mn == -INFINITY ? 0.0f : mn));
                             f *= fm;
-                            l *= fm;
                             m = mn;
                         }
+                        l *= f;
                         if (t > 0 && __any_sync(0xffffffffu, f != 1.0f)) {
                             // O of the tiles so far, on the new base
                             ok = __all_sync(0xffffffffu, ptx::mbar_wait(o_bar(h), o_phase ^ 1u, a.status, 3));
@@ -222,8 +245,8 @@ attn_chunk_kernel(const Args a)
                                 ptx::tmem_st_32x32b_x16(t_o + i, o);
                             }
                         }
-                        const float base = m == -INFINITY ? 0.0f : -m;
-                        const float2 rs2 = make_float2(row_scale, row_scale), b2 = make_float2(base, base), d2 = make_float2(v_down, v_down);
+                        const float base = (m == -INFINITY ? 0.0f : -m) + (FP8 ? log2_factor(v_field) : 0.0f);
+                        const float2 rs2 = make_float2(row_scale, row_scale), b2 = make_float2(base, base);
                         float2 sum[2] = {make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f)};
 #pragma unroll
                         for (int g = 0; g < kTile; g += 64) {
@@ -237,31 +260,28 @@ attn_chunk_kernel(const Args a)
                                 sum[0] = ptx::add2(sum[0], u);
                                 sum[1] = ptx::add2(sum[1], v);
                                 if (FP8) {
-                                    const uint4 y = ptx::ld_shared_v4(sc + 32 + 4 * kTile + 4 * (g + i));
-                                    float2 vu = ptx::mul2(make_float2(__uint_as_float(y.x), __uint_as_float(y.y)), d2);
-                                    float2 vv = ptx::mul2(make_float2(__uint_as_float(y.z), __uint_as_float(y.w)), d2);
-                                    vu = ptx::mul2(u, vu);
-                                    vv = ptx::mul2(v, vv);
-                                    if (!whole) {                             // a masked key's p is 0, whatever its scale
-                                        vu.x = u.x == 0.0f ? 0.0f : vu.x; vu.y = u.y == 0.0f ? 0.0f : vu.y;
-                                        vv.x = v.x == 0.0f ? 0.0f : vv.x; vv.y = v.y == 0.0f ? 0.0f : vv.y;
-                                    }
-                                    p[i / 2] = pack_f16x2(vu.x, vu.y);
-                                    p[i / 2 + 1] = pack_f16x2(vv.x, vv.y);
+                                    const uint4 y = ptx::ld_shared_v4(sc + C::kScaleAt + 4 * kTile + 4 * (g + i));
+                                    u = ptx::mul2(u, make_float2(__uint_as_float(y.x), __uint_as_float(y.y)));
+                                    v = ptx::mul2(v, make_float2(__uint_as_float(y.z), __uint_as_float(y.w)));
+                                    p[i / 2] = pack_f16x2(u.x, u.y);
+                                    p[i / 2 + 1] = pack_f16x2(v.x, v.y);
                                 } else {
                                     p[i / 2] = pack_bf16x2(u.x, u.y);
                                     p[i / 2 + 1] = pack_bf16x2(v.x, v.y);
                                 }
                             }
                             ptx::tmem_st_32x32b_x32(t_s + g / 2, p);
+                            ptx::tmem_st_wait();
+                            ptx::tcgen05_fence_before_sync();
+                            __syncwarp();
+                            if (lane == 0) ptx::mbar_arrive(p_bar(h, g / 64));      // the products over these keys can start
                         }
                         sum[0] = ptx::add2(sum[0], sum[1]);
                         l += sum[0].x + sum[0].y;
-                        ptx::tmem_st_wait();
+                    } else if (lane == 0) {
+                        ptx::mbar_arrive(p_bar(h, 0));
+                        ptx::mbar_arrive(p_bar(h, 1));
                     }
-                    ptx::tcgen05_fence_before_sync();
-                    __syncwarp();
-                    if (lane == 0) ptx::mbar_arrive(p_bar(h));
                     o_phase ^= 1u;                                            // the tile's P V completes one more phase
                 }
                 // eight arrivals a tile; in a block of one half its warps arrive for the others too (which nothing would pace)
@@ -276,11 +296,11 @@ attn_chunk_kernel(const Args a)
                 ok = __all_sync(0xffffffffu, ptx::mbar_wait(o_bar(h), o_phase ^ 1u, a.status, 3));
                 ptx::tcgen05_fence_after_sync();
                 const bool begins = c.tile == 0, ends = c.tile + todo == r.tiles;
-                const float v_up = FP8 ? pow2_of_field(v_field) * (1.0f / kRoom) : 1.0f;
+                if (FP8) m -= log2_factor(v_field);
                 const int part = 2 * blockIdx.x + (begins ? 1 : 0);
                 float* po = a.part + static_cast<size_t>(part) * kRows * (D + 2);
                 const bool whole_block = begins && ends;
-                const float f = !whole_block ? v_up : l == 0.0f ? 0.0f : __frcp_rn(l) * v_up;
+                const float f = !whole_block ? 1.0f : l == 0.0f ? 0.0f : __frcp_rn(l);
                 if (warp_on) {
 #pragma unroll 1
                     for (int i = 0; i < D; i += 32) {
@@ -293,14 +313,14 @@ attn_chunk_kernel(const Args a)
                                 for (int k = 0; k < 32; k += 8) {
                                     uint32_t w[4];
 #pragma unroll
-                                    for (int e = 0; e < 4; ++e) w[e] = pack_bf16x2(__uint_as_float(o[k + 2 * e]) * f, __uint_as_float(o[k + 2 * e + 1]) * f);
+                                    for (int e = 0; e < 4; ++e) w[e] = pack_bf16x2(__uint_as_float(o[k + 2 * e]) * f + poison, __uint_as_float(o[k + 2 * e + 1]) * f + poison);
                                     *reinterpret_cast<uint4*>(a.out + out_row * D + i + k) = make_uint4(w[0], w[1], w[2], w[3]);
                                 }
                             } else {
 #pragma unroll
                                 for (int k = 0; k < 32; k += 4)
-                                    *reinterpret_cast<float4*>(po + r_in * D + i + k) = make_float4(__uint_as_float(o[k]) * f, __uint_as_float(o[k + 1]) * f,
-                                                                                                    __uint_as_float(o[k + 2]) * f, __uint_as_float(o[k + 3]) * f);
+                                    *reinterpret_cast<float4*>(po + r_in * D + i + k) = make_float4(__uint_as_float(o[k]) + poison, __uint_as_float(o[k + 1]) + poison,
+                                                                                                    __uint_as_float(o[k + 2]) + poison, __uint_as_float(o[k + 3]) + poison);
                             }
                         }
                     }
@@ -319,6 +339,11 @@ attn_chunk_kernel(const Args a)
             c.at += todo;
             if (c.at < c.end) next_block(s, c, q, kRows);
         }
+        if (h == 0 && ok) {
+            if (threadIdx.x == 0) block_info[0] = 0;
+            __syncwarp();
+            if (lane == 0) ptx::mbar_arrive(q_bar(0));
+        }
     } else if (warp < 12) {
         // ================================================================================================ loaders
         ptx::regs_dec<kLoaderRegs>();
@@ -326,6 +351,7 @@ attn_chunk_kernel(const Args a)
         int slot = 0, sslot = 0;
         uint32_t phase = 0, sphase = 0;
         int pending = -1;                                                     // bf16: the slot whose copies are in flight
+        int stage_in = 0, stage_out = 0;                                      // E4M3: of the staging area's three items
         while (c.at < c.end && ok) {
             const Range r = block_range(s, q, c.i, kRows, kTile);
             const int todo = static_cast<int>(min(static_cast<long long>(r.tiles - c.tile), c.end - c.at));
@@ -338,43 +364,44 @@ attn_chunk_kernel(const Args a)
                 if (page < 0 || page >= s.num_pages) return -1;
                 return ((page * s.kv_heads + c.h) << s.page_shift) + (key & ((1 << s.page_shift) - 1));
             };
-            int row = row_of(r.tile0 + c.tile);
             constexpr int kPerRow = (FP8 ? D : 2 * D) / 16;                   // 16-byte pieces of a row
             constexpr int kRowsAt = 32 / kPerRow;                             // rows a warp instruction covers
-            const int piece = lane % kPerRow, sub = lane / kPerRow;
-            constexpr int kGroup = FP8 ? (D == 128 ? 4 : 2) : 1;              // instructions of half an item
-            uint4 buf[2][kGroup];
-            auto fetch = [&](uint4 (&to)[kGroup], const void* cache, int rows_of_lane, int half) {
+            constexpr int kInstr = 32 / kRowsAt;                              // instructions of a warp's 32 rows
+            // E4M3 rows of 128: eight neighbouring lanes take four pieces of two rows, so that their stores of 32 bytes hit eight
+            // different 16-byte units
+            const int piece = FP8 && D == 128 ? (lane & 3) + ((lane >> 1) & 4) : lane % kPerRow;
+            const int sub = FP8 && D == 128 ? ((lane >> 2) & 1) + ((lane >> 3) & 2) : lane / kPerRow;
+            // E4M3: a thread's pieces wait in its own places of the staging area (three items) until it converts them
+            const uint32_t staged = staging + (lw * 32 + lane) * 16;
+            uint32_t at[8 / kRowsAt > 0 ? 8 / kRowsAt : 1][2];                // where a piece's 16 elements (two units) go; the swizzle repeats after 8 rows
+            if constexpr (FP8) {
 #pragma unroll
-                for (int i = 0; i < kGroup; ++i) {
-                    const int from = __shfl_sync(0xffffffffu, rows_of_lane, (half * kGroup + i) * kRowsAt + sub);
-                    to[i] = from >= 0 ? __ldg(reinterpret_cast<const uint4*>(static_cast<const uint8_t*>(cache) + static_cast<size_t>(from) * D) + piece)
-                                      : make_uint4(0, 0, 0, 0);
+                for (int o = 0; o < 8 / kRowsAt; ++o)
+#pragma unroll
+                    for (int u = 0; u < 2; ++u) at[o][u] = unit_at((piece >> 2) * C::kHalfBytes, lw * 32 + o * kRowsAt + sub, (piece & 3) * 2 + u);
+            }
+            auto stage_item = [&](const void* cache, int rows_of_lane) {
+                const uint32_t to = staged + stage_in * C::kStagedBytes;
+#pragma unroll
+                for (int i = 0; i < kInstr; ++i) {
+                    const int from = __shfl_sync(0xffffffffu, rows_of_lane, i * kRowsAt + sub);
+                    ptx::cp_async_16(to + i * 2048, static_cast<const uint8_t*>(cache) + static_cast<size_t>(max(from, 0)) * D + piece * 16, from >= 0 ? 16u : 0u);
                 }
+                ptx::cp_async_commit();
+                if (++stage_in == 3) stage_in = 0;
             };
-            auto store = [&](const uint4 (&from)[kGroup], uint32_t to, int half) {
-#pragma unroll
-                for (int i = 0; i < kGroup; ++i) {
-                    const int rr = lw * 32 + (half * kGroup + i) * kRowsAt + sub;
-                    const uint32_t w[4] = {from[i].x, from[i].y, from[i].z, from[i].w};
-                    uint32_t v[8];
-#pragma unroll
-                    for (int k = 0; k < 4; ++k) { v[2 * k] = ptx::e4m3x2_lo(w[k]); v[2 * k + 1] = ptx::e4m3x2_hi(w[k]); }
-                    // 16 elements = units 2p and 2p + 1 of the row; a row of 128's upper half stores them in the other order, so that
-                    // its eight lanes hit eight different units
-                    const uint32_t column = to + (piece >> 2) * C::kHalfBytes;
-                    const int unit = (piece & 3) * 2;
-                    const bool swap = D == 128 && piece >= 4;
-                    const uint32_t at0 = unit_at(column, rr, unit + (swap ? 1 : 0)), at1 = unit_at(column, rr, unit + (swap ? 0 : 1));
-                    ptx::st_shared_v4(at0, swap ? v[4] : v[0], swap ? v[5] : v[1], swap ? v[6] : v[2], swap ? v[7] : v[3]);
-                    ptx::st_shared_v4(at1, swap ? v[0] : v[4], swap ? v[1] : v[5], swap ? v[2] : v[6], swap ? v[3] : v[7]);
-                }
-            };
-            if (FP8) { fetch(buf[0], a.k_cache, row, 0); fetch(buf[1], a.k_cache, row, 1); }
+            // one tile ahead: the scales; two ahead: the rows
+            int row = row_of(r.tile0 + c.tile), next = todo > 1 ? row_of(r.tile0 + c.tile + 1) : -1;
+            float ks = 0.0f, vs = 0.0f;
+            if (FP8) {
+                if (row >= 0) { ks = __ldg(a.k_scale + row); vs = __ldg(a.v_scale + row); }
+                stage_item(a.k_cache, row);
+                stage_item(a.v_cache, row);
+            }
             for (int t = 0; t < todo && ok; ++t) {
-                const int next = t + 1 < todo ? row_of(r.tile0 + c.tile + t + 1) : -1;
-                float ks = 0.0f, vs = 0.0f;
-                if (FP8 && row >= 0) { ks = __ldg(a.k_scale + row); vs = __ldg(a.v_scale + row); }
+                const int after = t + 2 < todo ? row_of(r.tile0 + c.tile + t + 2) : -1;
+                float ks_next = 0.0f, vs_next = 0.0f;
+                if (FP8 && next >= 0) { ks_next = __ldg(a.k_scale + next); vs_next = __ldg(a.v_scale + next); }
                 // ---- the tile's mask and scales
                 ok = __all_sync(0xffffffffu, ptx::mbar_wait(scale_bar(sslot), sphase ^ 1u, a.status, 4));
                 if (!ok) break;
@@ -382,38 +409,49 @@ attn_chunk_kernel(const Args a)
                     const uint32_t sc = scales + sslot * C::kScaleBytes;
                     uint8_t* scp = smem_raw + (sc - raw);
                     const uint32_t there = __ballot_sync(0xffffffffu, row >= 0);
-                    uint32_t top = __float_as_uint(vs) & 0x7FFFFFFFu;
-                    top = __reduce_max_sync(0xffffffffu, top < 0x7F800000u ? top : 0u);
+                    const uint32_t bits = __float_as_uint(vs) & 0x7FFFFFFFu;
+                    const uint32_t odd = __ballot_sync(0xffffffffu, bits >= 0x7F800000u);
+                    if (bits >= 0x7F800000u) vs = 0.0f;
+                    const uint32_t top = __reduce_max_sync(0xffffffffu, bits < 0x7F800000u ? bits : 0u);
                     if (lane == 0) {
                         reinterpret_cast<uint32_t*>(scp)[lw] = there;
                         reinterpret_cast<uint32_t*>(scp)[4 + lw] = (top >> 23) + 1;
+                        reinterpret_cast<uint32_t*>(scp)[8 + lw] = odd;
                     }
                     if (FP8) {
-                        reinterpret_cast<float*>(scp + 32)[lw * 32 + lane] = ks;
-                        reinterpret_cast<float*>(scp + 32)[kTile + lw * 32 + lane] = vs;
+                        reinterpret_cast<float*>(scp + C::kScaleAt)[lw * 32 + lane] = ks;
+                        reinterpret_cast<float*>(scp + C::kScaleAt)[kTile + lw * 32 + lane] = vs;
                     }
                     if (++sslot == kScaleSlots) { sslot = 0; sphase ^= 1u; }
                 }
                 // ---- keys, then values
 #pragma unroll
                 for (int kv = 0; kv < 2; ++kv) {
+                    const uint8_t* cache = static_cast<const uint8_t*>(kv == 0 ? a.k_cache : a.v_cache);
+                    if (FP8) {
+                        stage_item(cache, next);                              // (an empty item behind the last tile)
+                        ptx::cp_async_wait<2>();
+                    }
                     ok = __all_sync(0xffffffffu, ptx::mbar_wait(empty_bar(slot), phase ^ 1u, a.status, 1));
                     if (!ok) break;
                     const uint32_t to = ring + slot * C::kSlotBytes;
                     if constexpr (FP8) {
-                        store(buf[0], to, 0);
-                        if (kv == 0) fetch(buf[0], a.v_cache, row, 0);
-                        else fetch(buf[0], a.k_cache, next, 0);
-                        store(buf[1], to, 1);
-                        if (kv == 0) fetch(buf[1], a.v_cache, row, 1);
-                        else fetch(buf[1], a.k_cache, next, 1);
+                        const uint32_t from = staged + stage_out * C::kStagedBytes;
+#pragma unroll
+                        for (int i = 0; i < kInstr; ++i) {
+                            const uint4 w = ptx::ld_shared_v4(from + i * 2048);
+                            constexpr int kPeriod = 8 / kRowsAt;
+                            const uint32_t go = to + (i / kPeriod) * 1024;
+                            ptx::st_shared_v4(go + at[i % kPeriod][0], ptx::e4m3x2_lo(w.x), ptx::e4m3x2_hi(w.x), ptx::e4m3x2_lo(w.y), ptx::e4m3x2_hi(w.y));
+                            ptx::st_shared_v4(go + at[i % kPeriod][1], ptx::e4m3x2_lo(w.z), ptx::e4m3x2_hi(w.z), ptx::e4m3x2_lo(w.w), ptx::e4m3x2_hi(w.w));
+                        }
+                        if (++stage_out == 3) stage_out = 0;
                         ptx::fence_proxy_async_smem();
                         __syncwarp();
                         if (lane == 0) ptx::mbar_arrive(full_bar(slot));
                     } else {
-                        const uint8_t* cache = static_cast<const uint8_t*>(kv == 0 ? a.k_cache : a.v_cache);
 #pragma unroll
-                        for (int i = 0; i < 32 / kRowsAt; ++i) {
+                        for (int i = 0; i < kInstr; ++i) {
                             const int from = __shfl_sync(0xffffffffu, row, i * kRowsAt + sub);
                             ptx::cp_async_16(unit_at(to + (piece >> 3) * C::kHalfBytes, lw * 32 + i * kRowsAt + sub, piece & 7),
                                              cache + static_cast<size_t>(max(from, 0)) * (2 * D) + piece * 16, from >= 0 ? 16u : 0u);
@@ -429,7 +467,12 @@ attn_chunk_kernel(const Args a)
                     }
                     if (++slot == C::kSlots) { slot = 0; phase ^= 1u; }
                 }
-                row = next;
+                row = next; next = after;
+                ks = ks_next; vs = vs_next;
+            }
+            if (FP8) {
+                ptx::cp_async_wait<0>();                                      // the two empty items
+                stage_in = stage_out;
             }
             c.at += todo;
             if (c.at < c.end) next_block(s, c, q, kRows);
@@ -460,15 +503,19 @@ attn_chunk_kernel(const Args a)
                 }
                 ptx::umma_commit(s_bar(h));
             };
-            while (c.at < c.end && ok) {
-                const Range r = block_range(s, q, c.i, kRows, kTile);
-                const int todo = static_cast<int>(min(static_cast<long long>(r.tiles - c.tile), c.end - c.at));
-                const int halves = min(kRows, q.n * s.group - c.i * kRows) > 128 ? 2 : 1;
+            while (ok) {
                 // scores of the first tile
+                ok = ptx::mbar_wait(q_bar(0), q_phase[0], a.status, 6);
+                if (!ok) break;
+                q_phase[0] ^= 1u;
+                const int todo = *static_cast<volatile int*>(block_info), halves = *static_cast<volatile int*>(block_info + 1);
+                if (todo == 0) break;
                 ok = ptx::mbar_wait(full_bar(slot), phase, a.status, 5);
                 for (int h = 0; h < halves && ok; ++h) {
-                    ok = ptx::mbar_wait(q_bar(h), q_phase[h], a.status, 6);
-                    q_phase[h] ^= 1u;
+                    if (h == 1) {
+                        ok = ptx::mbar_wait(q_bar(1), q_phase[1], a.status, 6);
+                        q_phase[1] ^= 1u;
+                    }
                     ptx::tcgen05_fence_after_sync();
                     if (ok) scores(h, ring + slot * C::kSlotBytes);
                 }
@@ -484,14 +531,18 @@ attn_chunk_kernel(const Args a)
                     if (on && ++slot == C::kSlots) { slot = 0; phase ^= 1u; }
                     for (int h = 0; h < halves && ok; ++h) {
                         if (h == 0) ok = ptx::mbar_wait(full_bar(v_slot), v_phase, a.status, 5);
-                        ok = ok && ptx::mbar_wait(p_bar(h), p_phase[h], a.status, 7);
-                        if (!ok) break;
-                        p_phase[h] ^= 1u;
-                        ptx::tcgen05_fence_after_sync();
                         const uint64_t dv = ptx::smem_desc_sw128_mnmajor(ring + v_slot * C::kSlotBytes, C::kHalfBytes);
 #pragma unroll
-                        for (int i = 0; i < kTile / 16; ++i)                  // 16 keys: 8 columns of P, 2 KB of each column of V
+                        for (int i = 0; i < kTile / 16; ++i) {                // 16 keys: 8 columns of P, 2 KB of each column of V
+                            if (i % 4 == 0) {
+                                ok = ok && ptx::mbar_wait(p_bar(h, i / 4), p_phase[h], a.status, 7);
+                                if (!ok) break;
+                                ptx::tcgen05_fence_after_sync();
+                            }
                             ptx::umma_f16_ts(tmem + C::kOCol + h * D, tmem + h * 128 + 8 * i, dv + (2048 >> 4) * i, id_o, t > 0 || i > 0);
+                        }
+                        if (!ok) break;
+                        p_phase[h] ^= 1u;
                         ptx::umma_commit(o_bar(h));
                         if (h == halves - 1) ptx::umma_commit(empty_bar(v_slot));
                         if (on) {
@@ -505,8 +556,6 @@ attn_chunk_kernel(const Args a)
                         }
                     }
                 }
-                c.at += todo;
-                if (c.at < c.end) next_block(s, c, q, kRows);
             }
         }
         __syncwarp();

@@ -80,8 +80,7 @@ __device__ __forceinline__ uint32_t pack_f16x2(float lo, float hi)
     const __half2 v = __floats2half2_rn(lo, hi);
     return *reinterpret_cast<const uint32_t*>(&v);
 }
-// p * scale / (power of two above the largest scale) is kept times 2^15, so that fp16 holds it from 2^15 down: what falls below
-// its normal range is 2^-29 of the largest value in the cache
+// p * scale / (power of two above the largest scale) is kept times 2^15: fp16 starts to lose bits only where it is below 2^-29
 constexpr float kRoom = 32768.0f;
 __device__ __forceinline__ float pow2_of_field(uint32_t e) { return __uint_as_float(e << 23); }      // 2^(e - 127), 1 <= e <= 254
 
