@@ -45,8 +45,8 @@ __device__ __forceinline__ void zero_rest(const Args& a)
     if (lo == 0 && hi == a.s.tokens) return;
     const long long vecs = static_cast<long long>(a.s.heads) * (D / 8);
     const int rest = lo + a.s.tokens - hi;
-    for (long long i = static_cast<long long>(blockIdx.x) * blockDim.x + threadIdx.x; i < rest * vecs;
-         i += static_cast<long long>(gridDim.x) * blockDim.x) {
+    const long long block = static_cast<long long>(blockIdx.y) * gridDim.x + blockIdx.x, blocks = static_cast<long long>(gridDim.x) * gridDim.y;
+    for (long long i = block * blockDim.x + threadIdx.x; i < rest * vecs; i += blocks * blockDim.x) {
         int t = static_cast<int>(i / vecs);
         const long long e = i - t * vecs;
         if (t >= lo) t += hi - lo;
@@ -62,6 +62,7 @@ __global__ void __launch_bounds__(256)
 combine_kernel(const Args a, int rows_per_block)
 {
     constexpr int kPer = D / 32;
+    zero_rest<D>(a);                           // (nothing else writes these rows)
     ptx::pdl_wait();
     const Open op = a.open[blockIdx.x];
     const int row = blockIdx.y * 8 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
@@ -69,26 +70,36 @@ combine_kernel(const Args a, int rows_per_block)
     const size_t slot_floats = static_cast<size_t>(rows_per_block) * (D + 2);
     const int c0 = blockIdx.x, parts = op.last - c0 + 1;
     auto part = [&](int i) { return a.part + static_cast<size_t>(i == 0 ? 2 * c0 + 1 : 2 * (c0 + i)) * slot_floats; };
+    // a lane has the state of every 32nd part; 32 parts at a time, their outputs' loads are independent of one another
     float m = -INFINITY;
     for (int i = lane; i < parts; i += 32) m = ptx::max_nan(m, part(i)[rows_per_block * D + row * 2]);
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) m = ptx::max_nan(m, __shfl_xor_sync(0xffffffffu, m, o));
     const float base = m == -INFINITY ? 0.0f : m;
     float l = 0.0f, acc[kPer] = {};
-#pragma unroll 4
-    for (int i = 0; i < parts; ++i) {
-        const float* p = part(i);
-        const float2 st = *reinterpret_cast<const float2*>(p + rows_per_block * D + row * 2);
-        const float f = ptx::ex2(st.x - base);
-        l += st.y * f;
-        if constexpr (kPer == 4) {
-            const float4 v = *reinterpret_cast<const float4*>(p + row * D + lane * 4);
-            acc[0] += v.x * f; acc[1] += v.y * f; acc[2] += v.z * f; acc[3] += v.w * f;
-        } else {
-            const float2 v = *reinterpret_cast<const float2*>(p + row * D + lane * 2);
-            acc[0] += v.x * f; acc[1] += v.y * f;
+    for (int i0 = 0; i0 < parts; i0 += 32) {
+        float f = 0.0f;
+        if (i0 + lane < parts) {
+            const float2 st = *reinterpret_cast<const float2*>(part(i0 + lane) + rows_per_block * D + row * 2);
+            f = ptx::ex2(st.x - base);
+            l += st.y * f;
+        }
+        const int n = min(32, parts - i0);
+#pragma unroll 8
+        for (int i = 0; i < n; ++i) {
+            const float* p = part(i0 + i) + row * D;
+            const float fi = __shfl_sync(0xffffffffu, f, i);
+            if constexpr (kPer == 4) {
+                const float4 v = *reinterpret_cast<const float4*>(p + lane * 4);
+                acc[0] += v.x * fi; acc[1] += v.y * fi; acc[2] += v.z * fi; acc[3] += v.w * fi;
+            } else {
+                const float2 v = *reinterpret_cast<const float2*>(p + lane * 2);
+                acc[0] += v.x * fi; acc[1] += v.y * fi;
+            }
         }
     }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
     const int r = op.r0 + row, t = r / a.s.group;
     const size_t to = static_cast<size_t>(op.token0 + t) * a.s.heads + op.h * a.s.group + r - t * a.s.group;
     const float inv = l == 0.0f ? 0.0f : __frcp_rn(l);

@@ -92,7 +92,6 @@ attn_chunk_kernel(const Args a)
         a.open[blockIdx.x].last = -1;
     }
     if (warp == 12) { ptx::tmem_alloc(tmem_slot, 512); ptx::tmem_relinquish(); }
-    zero_rest<D>(a);
     ptx::tcgen05_fence_before_sync();
     Cursor c = find_work(s, kRows, kTile, reinterpret_cast<long long*>(smem_raw + (q_base - raw)), a.block_limit, blockIdx.x, gridDim.x);
     ptx::tcgen05_fence_after_sync();

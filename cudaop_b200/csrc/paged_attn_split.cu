@@ -108,7 +108,6 @@ attn_split_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
         for (int i = 0; i < C::kStages; ++i) { ptx::mbar_init(full_bar(i), 1); ptx::mbar_init(empty_bar(i), kConsumers); }
         ptx::fence_mbar_init();
     }
-    zero_rest<D>(a);
     Cursor c = find_work(s, kRows, kTile, reinterpret_cast<long long*>(smem_raw + (ring - raw)), a.block_limit, blockIdx.x, gridDim.x);
     if (threadIdx.x == 0) a.open[blockIdx.x].last = -1;
     if (c.at == c.end) return;

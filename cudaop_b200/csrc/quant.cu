@@ -298,8 +298,8 @@ extern "C" int b200q_quant_rows_mxfp4(const void* X, void* Q, void* SF_blocked, 
     uint8_t* sf = static_cast<uint8_t*>(SF_blocked);
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     const long long vecs = static_cast<long long>(rows) * cols / 8;
-    // few vectors: one per thread, so that a decode batch is one pass of the machine; many: eight loads in flight a thread
-    if (vecs <= 256LL * sms) {
+    // up to what the machine holds at once: one vector a thread; more: eight loads in flight a thread
+    if (vecs <= 2048LL * sms) {
         quant::quant_rows_mxfp4_kernel<1><<<static_cast<int>((vecs + 255) / 256), 256, 0, st>>>(x, q, sf, rows, cols / 32);
     } else {
         long long blocks = (vecs + 2047) / 2048;
