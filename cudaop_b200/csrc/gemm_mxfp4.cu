@@ -29,12 +29,15 @@ constexpr int kSlabElems = 256;
 constexpr int kSfBytes = 1024;                 // two 512-byte scale blocks (128 rows x 128 K each) per operand and stage
 constexpr int kThreads = 192;                  // warp 0 TMA, warp 1 MMA, warps 2-5 epilogue (one per TMEM lane quadrant)
 constexpr int kMaxStages = 8;
+constexpr int kAhead = 8;                      // slabs of B brought into L2 while the kernel before this one runs
 constexpr uint32_t kTmemCols = 256;            // accumulator (up to 128) + scales (8 + 8); two CTAs fit an SM
 
 struct Params {
     int M, N, slabs, ksteps;                   // K slabs of 256 and MMAs of 64 along K
     int mt, stages, stage_bytes;               // rows of A per tile, depth of the load ring
     __nv_bfloat16* C;
+    const uint8_t* sfw;                        // blocked scales of B
+    long long sfw_row;                         // bytes of one 128-row block of them
     uint32_t* status;
 };
 
@@ -75,6 +78,13 @@ gemm_mxfp4_few_rows_kernel(const __grid_constant__ CUtensorMap tmW, const __grid
         if (ptx::elect_one()) {
             ptx::tma_prefetch_desc(&tmW); ptx::tma_prefetch_desc(&tmX);
             ptx::tma_prefetch_desc(&tmSFW); ptx::tma_prefetch_desc(&tmSFX);
+            // The launch does not wait for the kernel before this one (normally the quantiser of A).  Until its results are there
+            // B is brought into L2: a hint, so it does not matter if that kernel writes B.
+            const int ahead = min(slab1 - slab0, kAhead);
+            for (int sl = slab0; sl < slab0 + ahead; ++sl) ptx::tma_prefetch_2d(&tmW, sl * kSlabBytes, n0);
+            ptx::bulk_prefetch(p.sfw + (n0 / 128) * p.sfw_row + slab0 * kSfBytes,
+                               static_cast<uint32_t>(min(static_cast<long long>(ahead) * kSfBytes, p.sfw_row - slab0 * kSfBytes)));
+            ptx::pdl_wait();
             int stage = 0; uint32_t phase = 0; bool ok = true;
             for (int sl = slab0; sl < slab1 && ok; ++sl) {
                 if (!ptx::mbar_wait(empty_bar(stage), phase ^ 1u, p.status, 1)) { ok = false; break; }
@@ -148,14 +158,24 @@ gemm_mxfp4_few_rows_kernel(const __grid_constant__ CUtensorMap tmW, const __grid
         ptx::cluster_arrive();
         ptx::cluster_wait();
         // this CTA's share of the tile's rows, summed over the cluster in rank order
-        const int rows = min(p.mt, p.M - m0);
-        const int total = rows * kBN;
-        for (int e = split * kThreads + threadIdx.x; e < total; e += splits * kThreads) {
-            const uint32_t at = smem_base + 4u * e;
-            float v = 0.0f;
-            for (int s = 0; s < splits; ++s) v += ptx::ld_dsmem_f32(ptx::mapa(at, s));
-            const int m = m0 + e / kBN, n = n0 + e % kBN;
-            if (n < p.N) p.C[static_cast<size_t>(m) * p.N + n] = __float2bfloat16_rn(v);
+        const int quads = min(p.mt, p.M - m0) * (kBN / 4);
+        for (int e = split * kThreads + threadIdx.x; e < quads; e += splits * kThreads) {
+            const uint32_t at = smem_base + 16u * e;
+            float4 v[8];
+#pragma unroll
+            for (int s = 0; s < 8; ++s) v[s] = s < splits ? ptx::ld_dsmem_f32x4(ptx::mapa(at, s)) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+            float4 t = v[0];
+#pragma unroll
+            for (int s = 1; s < 8; ++s) { t.x += v[s].x; t.y += v[s].y; t.z += v[s].z; t.w += v[s].w; }
+            const int m = m0 + e / (kBN / 4), n = n0 + e % (kBN / 4) * 4;
+            __nv_bfloat16* to = p.C + static_cast<size_t>(m) * p.N + n;
+            if (n + 4 <= p.N && (reinterpret_cast<uintptr_t>(to) & 7u) == 0) {
+                *reinterpret_cast<uint2*>(to) = make_uint2(pack_bf16x2(t.x, t.y), pack_bf16x2(t.z, t.w));
+            } else {
+                const float w[4] = {t.x, t.y, t.z, t.w};
+                for (int i = 0; i < 4; ++i)
+                    if (n + i < p.N) to[i] = __float2bfloat16_rn(w[i]);
+            }
         }
         ptx::cluster_arrive();                 // a CTA's shared memory must outlive its peers' reads
         ptx::cluster_wait();
@@ -174,6 +194,7 @@ int few_rows(const void* X, const void* SFX, const void* W, const void* SFW, voi
     if (sms <= 0) return cudaErrorInvalidDevice;
     Params p{};
     p.M = M; p.N = N; p.C = static_cast<__nv_bfloat16*>(C);
+    p.sfw = static_cast<const uint8_t*>(SFW); p.sfw_row = static_cast<long long>((K + 127) / 128) * 512;
     p.slabs = (K + kSlabElems - 1) / kSlabElems; p.ksteps = (K + 63) / 64;
     p.mt = M >= 128 ? 128 : (M + 15) / 16 * 16;
     p.status = status_ptr();
@@ -222,10 +243,12 @@ int few_rows(const void* X, const void* SFX, const void* W, const void* SFW, voi
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = dim3(splits, tiles_n, tiles_m); cfg.blockDim = dim3(kThreads);
     cfg.dynamicSmemBytes = smem; cfg.stream = static_cast<cudaStream_t>(stream);
-    cudaLaunchAttribute attr[1];
+    cudaLaunchAttribute attr[2];
     attr[0].id = cudaLaunchAttributeClusterDimension;
     attr[0].val.clusterDim.x = splits; attr[0].val.clusterDim.y = 1; attr[0].val.clusterDim.z = 1;
-    cfg.attrs = attr; cfg.numAttrs = 1;
+    attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[1].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr; cfg.numAttrs = 2;
     return cudaLaunchKernelEx(&cfg, gemm_mxfp4_few_rows_kernel, tmW, tmX, tmSFW, tmSFX, p);
 }
 
@@ -242,7 +265,12 @@ int b200q_gemm_mxfp4_blocked(const void* A, const void* SFA_blocked, const void*
     if (M <= 0 || N <= 0 || K <= 0 || K % 32 != 0) return cudaErrorInvalidValue;
     if (!aligned16(A) || !aligned16(B) || !aligned16(SFA_blocked) || !aligned16(SFB_blocked)) return cudaErrorInvalidValue;
     if (M <= 128) return mxfp4::few_rows(A, SFA_blocked, B, SFB_blocked, C, M, N, K, stream);
-    return gemm_block_scaled_pair(2, A, SFA_blocked, B, SFB_blocked, C, M, N, K, 1.0f, 256, stream);
+    // the width whose last wave of CTA pairs wastes less: tiles of 192 where they fit the same number of waves
+    // (256 x 8192 x 8192: 14.4 us with 192 columns, 16.7 with 256; 512 x 8192 x 8192: 22.0 and 17.0)
+    const long long tiles_m = (M + 255) / 256, pairs = num_sms() / 2;
+    if (pairs <= 0) return cudaErrorInvalidDevice;
+    auto cost = [&](int bn) { return (tiles_m * ((N + bn - 1) / bn) + pairs - 1) / pairs * bn; };
+    return gemm_block_scaled_pair(2, A, SFA_blocked, B, SFB_blocked, C, M, N, K, 1.0f, cost(192) < cost(256) ? 192 : 256, stream);
 }
 
 // Both MX formats share the scale layout: one UE8M0 byte per 32 K, 512-byte blocks of 128 rows x 128 K.

@@ -128,6 +128,7 @@ gemm_nvfp4_2cta_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_con
     ptx::cluster_wait();
     ptx::tcgen05_fence_after_sync();
     const uint32_t tmem_base = *tmem_slot_ptr;
+    if constexpr (FMT == kFmtMxfp4) ptx::pdl_wait();         // launched without waiting for the kernel before it (the quantiser of A)
 
     if (warp == 0) {
         // ------------------------------------------------------------ producer (both CTAs)
@@ -355,10 +356,12 @@ cudaError_t launch(const CUtensorMap& tmA, const CUtensorMap& tmB, const CUtenso
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = dim3(2 * pairs); cfg.blockDim = dim3(kThreads);
     cfg.dynamicSmemBytes = Cfg<BN, FMT>::kSmemBytes; cfg.stream = stream;
-    cudaLaunchAttribute attr[1];
+    cudaLaunchAttribute attr[2];
     attr[0].id = cudaLaunchAttributeClusterDimension;
     attr[0].val.clusterDim.x = 2; attr[0].val.clusterDim.y = 1; attr[0].val.clusterDim.z = 1;
-    cfg.attrs = attr; cfg.numAttrs = 1;
+    attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[1].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr; cfg.numAttrs = FMT == kFmtMxfp4 ? 2 : 1;
     return cudaLaunchKernelEx(&cfg, kernel, tmA, tmB, tmSFA, tmSFB, tmC, p);
 }
 

@@ -600,6 +600,11 @@ __device__ __forceinline__ void tma_load_3d(uint32_t smem_dst, const CUtensorMap
         ::"r"(smem_dst), "l"(reinterpret_cast<uint64_t>(tm)), "r"(bar), "r"(x), "r"(y), "r"(z)
         : "memory");
 }
+// cp.async.bulk.prefetch.L2: brings a contiguous range (16-byte aligned, a multiple of 16 bytes) into L2 only
+__device__ __forceinline__ void bulk_prefetch(const void* gsrc, uint32_t bytes)
+{
+    asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(gsrc), "r"(bytes) : "memory");
+}
 // cp.async.bulk.prefetch.tensor.2d.L2: brings a box into L2 only
 __device__ __forceinline__ void tma_prefetch_2d(const CUtensorMap* tm, int x, int y)
 {
@@ -836,6 +841,13 @@ __device__ __forceinline__ float max3(float a, float b, float c)
 __device__ __forceinline__ void named_barrier(int id, int threads)
 {
     asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(threads) : "memory");
+}
+
+__device__ __forceinline__ float4 ld_dsmem_f32x4(uint32_t cluster_addr)
+{
+    float4 v;
+    asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(cluster_addr));
+    return v;
 }
 
 __device__ __forceinline__ void st_release_sys(uint32_t* p, uint32_t v)

@@ -8,12 +8,15 @@
 // phases (load, reduce, convert + store) and only the first keeps memory busy, so short rows get small
 // CTAs, many of which are resident per SM in different phases.
 #include "common.cuh"
+#include "ptx.cuh"
 #include <cuda_fp4.h>
 #include <cuda_fp8.h>
 #include "../../include/b200q.h"
 
 namespace b200q {
 namespace quant {
+
+using ptx::pdl_launch_dependents;
 
 __device__ __forceinline__ float bf16_lo(uint32_t w) { return __uint_as_float(w << 16); }
 __device__ __forceinline__ float bf16_hi(uint32_t w) { return __uint_as_float(w & 0xFFFF0000u); }
@@ -184,6 +187,7 @@ template <int kVecs>
 __global__ void __launch_bounds__(256)
 quant_rows_mxfp4_kernel(const __nv_bfloat16* __restrict__ X, uint32_t* __restrict__ Q, uint8_t* __restrict__ SF, int rows, int k32)
 {
+    pdl_launch_dependents();                                          // the product may set up and bring its weights nearer meanwhile
     const int lane = threadIdx.x & 31;
     const int k128 = (k32 + 3) / 4;
     const bool words = (k32 & 3) == 0;                                // four scales of a 128-K slab lie in sixteen neighbouring lanes
@@ -300,7 +304,10 @@ extern "C" int b200q_quant_rows_mxfp4(const void* X, void* Q, void* SF_blocked, 
     const long long vecs = static_cast<long long>(rows) * cols / 8;
     // up to what the machine holds at once: one vector a thread; more: eight loads in flight a thread
     if (vecs <= 2048LL * sms) {
-        quant::quant_rows_mxfp4_kernel<1><<<static_cast<int>((vecs + 255) / 256), 256, 0, st>>>(x, q, sf, rows, cols / 32);
+        // (a small batch has more scale words to zero, the rows up to the next 128, than vectors)
+        const long long pads = static_cast<long long>((rows + 127) / 128 * 128 - rows) * ((cols + 127) / 128);
+        const long long work = vecs > pads ? vecs : pads;
+        quant::quant_rows_mxfp4_kernel<1><<<static_cast<int>((work + 255) / 256), 256, 0, st>>>(x, q, sf, rows, cols / 32);
     } else {
         long long blocks = (vecs + 2047) / 2048;
         if (blocks > sms * 8LL) blocks = sms * 8LL;
