@@ -29,15 +29,12 @@ constexpr int kSlabElems = 256;
 constexpr int kSfBytes = 1024;                 // two 512-byte scale blocks (128 rows x 128 K each) per operand and stage
 constexpr int kThreads = 192;                  // warp 0 TMA, warp 1 MMA, warps 2-5 epilogue (one per TMEM lane quadrant)
 constexpr int kMaxStages = 8;
-constexpr int kAhead = 8;                      // slabs of B brought into L2 while the kernel before this one runs
 constexpr uint32_t kTmemCols = 256;            // accumulator (up to 128) + scales (8 + 8); two CTAs fit an SM
 
 struct Params {
     int M, N, slabs, ksteps;                   // K slabs of 256 and MMAs of 64 along K
     int mt, stages, stage_bytes;               // rows of A per tile, depth of the load ring
     __nv_bfloat16* C;
-    const uint8_t* sfw;                        // blocked scales of B
-    long long sfw_row;                         // bytes of one 128-row block of them
     uint32_t* status;
 };
 
@@ -78,12 +75,9 @@ gemm_mxfp4_few_rows_kernel(const __grid_constant__ CUtensorMap tmW, const __grid
         if (ptx::elect_one()) {
             ptx::tma_prefetch_desc(&tmW); ptx::tma_prefetch_desc(&tmX);
             ptx::tma_prefetch_desc(&tmSFW); ptx::tma_prefetch_desc(&tmSFX);
-            // The launch does not wait for the kernel before this one (normally the quantiser of A).  Until its results are there
-            // B is brought into L2: a hint, so it does not matter if that kernel writes B.
-            const int ahead = min(slab1 - slab0, kAhead);
-            for (int sl = slab0; sl < slab0 + ahead; ++sl) ptx::tma_prefetch_2d(&tmW, sl * kSlabBytes, n0);
-            ptx::bulk_prefetch(p.sfw + (n0 / 128) * p.sfw_row + slab0 * kSfBytes,
-                               static_cast<uint32_t>(min(static_cast<long long>(ahead) * kSfBytes, p.sfw_row - slab0 * kSfBytes)));
+            // The launch does not wait for the kernel before this one (normally the quantiser of A): what comes before this line runs
+            // beside it.  B waits too, since that kernel may have written it; bringing B into L2 meanwhile (prefetches are hints) did
+            // not pay: 11.7 us for quantiser and product of 1 x 8192 x 8192 with it, 10.5 us without.
             ptx::pdl_wait();
             int stage = 0; uint32_t phase = 0; bool ok = true;
             for (int sl = slab0; sl < slab1 && ok; ++sl) {
@@ -194,7 +188,6 @@ int few_rows(const void* X, const void* SFX, const void* W, const void* SFW, voi
     if (sms <= 0) return cudaErrorInvalidDevice;
     Params p{};
     p.M = M; p.N = N; p.C = static_cast<__nv_bfloat16*>(C);
-    p.sfw = static_cast<const uint8_t*>(SFW); p.sfw_row = static_cast<long long>((K + 127) / 128) * 512;
     p.slabs = (K + kSlabElems - 1) / kSlabElems; p.ksteps = (K + 63) / 64;
     p.mt = M >= 128 ? 128 : (M + 15) / 16 * 16;
     p.status = status_ptr();

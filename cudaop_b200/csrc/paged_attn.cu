@@ -5,6 +5,10 @@
 namespace b200q {
 namespace paged {
 int page_shift_of(int page_size);        // paged_cache.cu
+// Rows per kv head up to which the split-KV kernel is taken.  It reads the keys once per 16 rows, mostly from L2; the tensor-core kernel
+// once, but takes longer to start.  24 sequences of up to 8192 tokens, 8 rows a token, E4M3, heads of 128: 52 / 66 / 111 us with 16 / 32 /
+// 64 rows against 98 us.
+constexpr int kSplitRows = 48;
 int g_impl = 0;                          // 0 by the number of rows, 1 split-KV kernel, 2 tensor-core kernel
 size_t open_bytes() { return (static_cast<size_t>(attn_split_ctas()) * sizeof(Open) + 15) / 16 * 16; }
 }
@@ -57,7 +61,7 @@ int b200q_paged_attention(const void* q, const void* k_cache, const void* v_cach
     if (a.status == nullptr) return cudaErrorInvalidDevice;
     a.open = static_cast<Open*>(workspace);
     a.part = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + open_bytes());
-    const bool chunk = g_impl != 0 ? g_impl == 2 : static_cast<long long>(a.max_q) * a.s.group > 64;
+    const bool chunk = g_impl != 0 ? g_impl == 2 : static_cast<long long>(a.max_q) * a.s.group > kSplitRows;
     return chunk ? attn_chunk(a, head_dim, fp8 != 0, static_cast<cudaStream_t>(stream)) : attn_split(a, head_dim, fp8 != 0, static_cast<cudaStream_t>(stream));
 }
 

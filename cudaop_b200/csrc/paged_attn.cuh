@@ -30,6 +30,14 @@ size_t attn_chunk_part_bytes(int head_dim);
 int attn_split_ctas();                       // the most CTAs a launch uses
 size_t attn_split_part_bytes(int head_dim);  // the most its parts take
 
+// Whether the tiles of a call, however its arrays divide the rows and keys, can be counted in 32 bits.
+inline bool tiles_fit(const Args& a, int rm, int kt)
+{
+    const double blocks = static_cast<double>(a.s.tokens) * a.s.group / rm + a.s.seqs;
+    const double keys = static_cast<double>(a.s.max_pages) * (1 << a.s.page_shift);
+    return blocks * a.s.kv_heads * (keys / kt + 2) < 2.0e9;
+}
+
 // natural log of sum_j e^(scale * q.k_j), from the maximum in units of log2 and the sum of 2^(x - max); -inf for no keys
 __device__ __forceinline__ float lse_of(float m, float l)
 {
@@ -65,49 +73,51 @@ combine_kernel(const Args a, int rows_per_block)
     zero_rest<D>(a);                           // (nothing else writes these rows)
     ptx::pdl_wait();
     const Open op = a.open[blockIdx.x];
-    const int row = blockIdx.y * 8 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
-    if (op.last < 0 || row >= op.rows) return;
-    const size_t slot_floats = static_cast<size_t>(rows_per_block) * (D + 2);
-    const int c0 = blockIdx.x, parts = op.last - c0 + 1;
-    auto part = [&](int i) { return a.part + static_cast<size_t>(i == 0 ? 2 * c0 + 1 : 2 * (c0 + i)) * slot_floats; };
-    // a lane has the state of every 32nd part; 32 parts at a time, their outputs' loads are independent of one another
-    float m = -INFINITY;
-    for (int i = lane; i < parts; i += 32) m = ptx::max_nan(m, part(i)[rows_per_block * D + row * 2]);
+    const int lane = threadIdx.x & 31;
+    if (op.last < 0) return;
+    for (int row = blockIdx.y * 8 + (threadIdx.x >> 5); row < op.rows; row += gridDim.y * 8) {
+        const size_t slot_floats = static_cast<size_t>(rows_per_block) * (D + 2);
+        const int c0 = blockIdx.x, parts = op.last - c0 + 1;
+        auto part = [&](int i) { return a.part + static_cast<size_t>(i == 0 ? 2 * c0 + 1 : 2 * (c0 + i)) * slot_floats; };
+        // a lane has the state of every 32nd part; 32 parts at a time, their outputs' loads are independent of one another
+        float m = -INFINITY;
+        for (int i = lane; i < parts; i += 32) m = ptx::max_nan(m, part(i)[rows_per_block * D + row * 2]);
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) m = ptx::max_nan(m, __shfl_xor_sync(0xffffffffu, m, o));
-    const float base = m == -INFINITY ? 0.0f : m;
-    float l = 0.0f, acc[kPer] = {};
-    for (int i0 = 0; i0 < parts; i0 += 32) {
-        float f = 0.0f;
-        if (i0 + lane < parts) {
-            const float2 st = *reinterpret_cast<const float2*>(part(i0 + lane) + rows_per_block * D + row * 2);
-            f = ptx::ex2(st.x - base);
-            l += st.y * f;
-        }
-        const int n = min(32, parts - i0);
+        for (int o = 16; o > 0; o >>= 1) m = ptx::max_nan(m, __shfl_xor_sync(0xffffffffu, m, o));
+        const float base = m == -INFINITY ? 0.0f : m;
+        float l = 0.0f, acc[kPer] = {};
+        for (int i0 = 0; i0 < parts; i0 += 32) {
+            float f = 0.0f;
+            if (i0 + lane < parts) {
+                const float2 st = *reinterpret_cast<const float2*>(part(i0 + lane) + rows_per_block * D + row * 2);
+                f = ptx::ex2(st.x - base);
+                l += st.y * f;
+            }
+            const int n = min(32, parts - i0);
 #pragma unroll 8
-        for (int i = 0; i < n; ++i) {
-            const float* p = part(i0 + i) + row * D;
-            const float fi = __shfl_sync(0xffffffffu, f, i);
-            if constexpr (kPer == 4) {
-                const float4 v = *reinterpret_cast<const float4*>(p + lane * 4);
-                acc[0] += v.x * fi; acc[1] += v.y * fi; acc[2] += v.z * fi; acc[3] += v.w * fi;
-            } else {
-                const float2 v = *reinterpret_cast<const float2*>(p + lane * 2);
-                acc[0] += v.x * fi; acc[1] += v.y * fi;
+            for (int i = 0; i < n; ++i) {
+                const float* p = part(i0 + i) + row * D;
+                const float fi = __shfl_sync(0xffffffffu, f, i);
+                if constexpr (kPer == 4) {
+                    const float4 v = *reinterpret_cast<const float4*>(p + lane * 4);
+                    acc[0] += v.x * fi; acc[1] += v.y * fi; acc[2] += v.z * fi; acc[3] += v.w * fi;
+                } else {
+                    const float2 v = *reinterpret_cast<const float2*>(p + lane * 2);
+                    acc[0] += v.x * fi; acc[1] += v.y * fi;
+                }
             }
         }
-    }
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
-    const int r = op.r0 + row, t = r / a.s.group;
-    const size_t to = static_cast<size_t>(op.token0 + t) * a.s.heads + op.h * a.s.group + r - t * a.s.group;
-    const float inv = l == 0.0f ? 0.0f : __frcp_rn(l);
-    if constexpr (kPer == 4)
-        *reinterpret_cast<uint2*>(a.out + to * D + lane * 4) = make_uint2(pack_bf16x2(acc[0] * inv, acc[1] * inv), pack_bf16x2(acc[2] * inv, acc[3] * inv));
-    else
-        *reinterpret_cast<uint32_t*>(a.out + to * D + lane * 2) = pack_bf16x2(acc[0] * inv, acc[1] * inv);
-    if (a.lse != nullptr && lane == 0) a.lse[to] = lse_of(m, l);
+        for (int o = 16; o > 0; o >>= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
+        const int r = op.r0 + row, t = r / a.s.group;
+        const size_t to = static_cast<size_t>(op.token0 + t) * a.s.heads + op.h * a.s.group + r - t * a.s.group;
+        const float inv = l == 0.0f ? 0.0f : __frcp_rn(l);
+        if constexpr (kPer == 4)
+            *reinterpret_cast<uint2*>(a.out + to * D + lane * 4) = make_uint2(pack_bf16x2(acc[0] * inv, acc[1] * inv), pack_bf16x2(acc[2] * inv, acc[3] * inv));
+        else
+            *reinterpret_cast<uint32_t*>(a.out + to * D + lane * 2) = pack_bf16x2(acc[0] * inv, acc[1] * inv);
+        if (a.lse != nullptr && lane == 0) a.lse[to] = lse_of(m, l);
+    }
 }
 
 // The kernel may start while its predecessor runs (it waits for its results before it reads anything).
@@ -115,7 +125,20 @@ template <int D>
 int launch_combine(const Args& a, int ctas, int rows_per_block, cudaStream_t stream)
 {
     cudaLaunchConfig_t cfg{};
-    cfg.gridDim = dim3(ctas, (rows_per_block + 7) / 8); cfg.blockDim = dim3(256); cfg.stream = stream;
+    // eight rows a CTA, as many as a block has or the caller's bound of the chunk lengths allows
+    const long long rows = static_cast<long long>(a.max_q) * a.s.group;
+    const int most = rows < rows_per_block ? static_cast<int>(rows) : rows_per_block;
+    cfg.gridDim = dim3(ctas, (most + 7) / 8); cfg.blockDim = dim3(256); cfg.stream = stream;
+    // the split of shared memory and L1 that the kernel before it has: another one would have to wait for an idle SM
+    static bool configured[64] = {};
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e != cudaSuccess) return e;
+    if (dev >= 64 || !configured[dev]) {
+        e = cudaFuncSetAttribute(combine_kernel<D>, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared);
+        if (e != cudaSuccess) return e;
+        if (dev < 64) configured[dev] = true;
+    }
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[0].val.programmaticStreamSerializationAllowed = 1;

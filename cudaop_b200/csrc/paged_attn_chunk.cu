@@ -13,6 +13,10 @@
 //                    bf16) over the same TMEM columns; O_h += P_h V with P_h as the tensor-memory operand and V as it lies, rows of
 //                    D contiguous elements (MN-major).  The order PV_0(j) S_0(j+1) PV_1(j) S_1(j+1) keeps the tensor cores on one half while
 //                    the other half's softmax runs.
+// A block of no more than 128 rows has no second half: its even tiles go through S_0, O_0 and warps 0-3, its odd tiles through S_1, O_1
+// and warps 4-7, with a running maximum and sum of their own, and warps 0-3 join the two at the end (the same TMEM lanes hold the
+// same rows).  With one half alone the block was one chain of product, softmax, product (24 sequences of up to 16 new on up to 8192 tokens, 32/4
+// heads of 64: 49 us, 32 us so).
 // TMEM: S_0 S_1 (128 columns each), O_0 O_1 (D columns each).  The running maximum is raised, and O rescaled in TMEM by the row's
 // own thread, only when it grows by more than 2^4 (exact: the sum uses the same base); after the first tiles that is rare.
 #include "paged_common.cuh"
@@ -35,12 +39,13 @@ struct Cfg {
     static constexpr int kSlotBytes = kHalves * kHalfBytes;
     static constexpr int kSlots = D == 64 ? 6 : FP8 ? 3 : 4;
     static constexpr int kStagedBytes = FP8 ? kTile * D : 0;                  // E4M3 bytes of a tile of keys or values, on their way
+    static constexpr int kStaged = D == 64 ? 6 : 3;
     static constexpr int kQBytes = 2 * kSlotBytes;
     // per tile: mask words, largest value scales, words of the keys whose value scale is not finite (4 each), key scales, value scales
     static constexpr int kScaleAt = 48;
     static constexpr int kScaleBytes = kScaleAt + (FP8 ? 2 * kTile * 4 : 0);
-    static constexpr int kBars = 2 * kSlots + kScaleSlots + 10;
-    static constexpr int kSmemBytes = 1024 + kQBytes + kSlots * kSlotBytes + 3 * kStagedBytes + kScaleSlots * kScaleBytes + kBars * 8 + 32;
+    static constexpr int kBars = 2 * kSlots + kScaleSlots + 12;
+    static constexpr int kSmemBytes = 1024 + kQBytes + kSlots * kSlotBytes + kStaged * kStagedBytes + kScaleSlots * kScaleBytes + kBars * 8 + 32 + 128 * 16;
     static constexpr int kOCol = 256;
 };
 
@@ -68,7 +73,7 @@ attn_chunk_kernel(const Args a)
     const uint32_t q_base = (raw + 1023u) & ~1023u;
     const uint32_t ring = q_base + C::kQBytes;
     const uint32_t staging = ring + C::kSlots * C::kSlotBytes;
-    const uint32_t scales = staging + 3 * C::kStagedBytes;
+    const uint32_t scales = staging + C::kStaged * C::kStagedBytes;
     const uint32_t bars = scales + kScaleSlots * C::kScaleBytes;
     auto full_bar = [&](int s) { return bars + 8u * s; };                     // a slot holds its tile
     auto empty_bar = [&](int s) { return bars + 8u * (C::kSlots + s); };
@@ -78,22 +83,25 @@ attn_chunk_kernel(const Args a)
     auto s_bar = [&](int h) { return more + 8u * (2 + h); };                  // scores of half h are in TMEM
     auto p_bar = [&](int h, int k) { return more + 8u * (4 + 2 * h + k); };   // P of half h, keys 64 * k .., is in TMEM
     auto o_bar = [&](int h) { return more + 8u * (8 + h); };                  // P V of half h is done
+    const uint32_t joined_bar = more + 8u * 10, read_bar = more + 8u * 11;    // odd tiles' states are there / have been read
     const uint32_t tmem_slot = bars + C::kBars * 8;
     int* block_info = reinterpret_cast<int*>(smem_raw + (tmem_slot + 4 - raw));        // for the products: tiles (0: no more blocks), halves
+    float4* odd_state = reinterpret_cast<float4*>(smem_raw + ((bars + C::kBars * 8 + 32 + 15) / 16 * 16 - raw));       // [128] maximum, sum, poison
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const Shape& s = a.s;
 
     ptx::pdl_launch_dependents();
     if (threadIdx.x == 0) {
-        for (int i = 0; i < C::kSlots; ++i) { ptx::mbar_init(full_bar(i), 4); ptx::mbar_init(empty_bar(i), 1); }
+        for (int i = 0; i < C::kSlots; ++i) { ptx::mbar_init(full_bar(i), FP8 ? 4 : 128); ptx::mbar_init(empty_bar(i), 1); }
         for (int i = 0; i < kScaleSlots; ++i) ptx::mbar_init(scale_bar(i), 8);
         for (int h = 0; h < 2; ++h) { ptx::mbar_init(q_bar(h), 4); ptx::mbar_init(s_bar(h), 1); ptx::mbar_init(p_bar(h, 0), 4); ptx::mbar_init(p_bar(h, 1), 4); ptx::mbar_init(o_bar(h), 1); }
+        ptx::mbar_init(joined_bar, 4); ptx::mbar_init(read_bar, 4);
         ptx::fence_mbar_init();
         a.open[blockIdx.x].last = -1;
     }
     if (warp == 12) { ptx::tmem_alloc(tmem_slot, 512); ptx::tmem_relinquish(); }
     ptx::tcgen05_fence_before_sync();
-    Cursor c = find_work(s, kRows, kTile, reinterpret_cast<long long*>(smem_raw + (q_base - raw)), a.block_limit, blockIdx.x, gridDim.x);
+    Cursor c = find_work(s, kRows, kTile, reinterpret_cast<int*>(smem_raw + (q_base - raw)), a.block_limit, blockIdx.x, gridDim.x);
     ptx::tcgen05_fence_after_sync();
     const uint32_t tmem = *reinterpret_cast<volatile uint32_t*>(smem_raw + (tmem_slot - raw));
     Seq q{};
@@ -104,16 +112,17 @@ attn_chunk_kernel(const Args a)
         // ================================================================================================ softmax
         ptx::regs_inc<kSoftmaxRegs>();
         const int h = warp >> 2, quad = warp & 3;
-        const int r_in = h * 128 + quad * 32 + lane;                          // row inside the block
         const uint32_t lanes = static_cast<uint32_t>(quad * 32) << 16;
         const uint32_t t_s = tmem + lanes + h * 128, t_o = tmem + lanes + C::kOCol + h * D;
-        uint32_t s_phase = 0, o_phase = 0;
+        uint32_t s_phase = 0, o_phase = 0, join_phase = 0;
         int slot = 0;                                                         // of the scale ring
         while (c.at < c.end && ok) {
             const Range r = block_range(s, q, c.i, kRows, kTile);
-            const int todo = static_cast<int>(min(static_cast<long long>(r.tiles - c.tile), c.end - c.at));
+            const int todo = min(r.tiles - c.tile, c.end - c.at);
             const int r0 = c.i * kRows, rows = min(kRows, q.n * s.group - r0);
-            const bool half_on = h * 128 < rows, warp_on = h * 128 + quad * 32 < rows;
+            const bool two = rows > 128;                                      // two halves of rows; else odd tiles go to h = 1
+            const int r_in = (two ? h * 128 : 0) + quad * 32 + lane;          // row inside the block
+            const bool half_on = two || todo > h, warp_on = (two ? h * 128 : 0) + quad * 32 < rows;
             const int row = min(r_in, rows - 1);                              // rows behind the block repeat its last one
             const int tok = (r0 + row) / s.group, head = c.h * s.group + (r0 + row) - tok * s.group;
             const int pos = q.kv - q.n + tok;
@@ -145,21 +154,23 @@ attn_chunk_kernel(const Args a)
                         const float lo = __uint_as_float(v[k] << 16) * down, hi = __uint_as_float(v[k] & 0xFFFF0000u) * down;
                         v[k] = FP8 ? pack_f16x2(lo, hi) : pack_bf16x2(lo, hi);
                     }
-                    ptx::st_shared_v4(unit_at(q_base + h * C::kSlotBytes + (i >> 3) * C::kHalfBytes, quad * 32 + lane, i & 7), v[0], v[1], v[2], v[3]);
+                    if (two || h == 0) ptx::st_shared_v4(unit_at(q_base + h * C::kSlotBytes + (i >> 3) * C::kHalfBytes, quad * 32 + lane, i & 7), v[0], v[1], v[2], v[3]);
                 }
                 ptx::fence_proxy_async_smem();
-                if (threadIdx.x == 0) { block_info[0] = todo; block_info[1] = rows > 128 ? 2 : 1; }
+                if (threadIdx.x == 0) { block_info[0] = todo; block_info[1] = two ? 2 : 1; }
                 __syncwarp();
-                if (lane == 0) ptx::mbar_arrive(q_bar(h));
+                if (lane == 0 && (two || h == 0)) ptx::mbar_arrive(q_bar(h));
             }
             const int pos_lo = __shfl_sync(0xffffffffu, pos, 0), pos_hi = __shfl_sync(0xffffffffu, pos, 31);
             // m: the base of the row's exponents.  For an E4M3 cache p is kept times kRoom / 2^v_exp, 2^v_exp a power of two above the
             // largest value scale so far: sum and output alike, so it cancels, and m - log2 of it is the base that the parts carry.
             float m = -INFINITY, l = 0.0f, poison = 0.0f;
             uint32_t v_field = 1;
+            bool fresh = true;                                                // O holds nothing of this block yet
             for (int t = 0; t < todo && ok; ++t) {
                 const uint32_t sc = scales + slot * C::kScaleBytes;
-                if (half_on) {
+                const bool mine = two || (t & 1) == h;
+                if (mine) {
                     ok = __all_sync(0xffffffffu, ptx::mbar_wait(s_bar(h), s_phase, a.status, 2));
                     if (!ok) break;
                     s_phase ^= 1u;
@@ -230,7 +241,7 @@ attn_chunk_kernel(const Args a)
                             m = mn;
                         }
                         l *= f;
-                        if (t > 0 && __any_sync(0xffffffffu, f != 1.0f)) {
+                        if (!fresh && __any_sync(0xffffffffu, f != 1.0f)) {
                             // O of the tiles so far, on the new base
                             ok = __all_sync(0xffffffffu, ptx::mbar_wait(o_bar(h), o_phase ^ 1u, a.status, 3));
                             ptx::tcgen05_fence_after_sync();
@@ -282,12 +293,13 @@ attn_chunk_kernel(const Args a)
                         ptx::mbar_arrive(p_bar(h, 1));
                     }
                     o_phase ^= 1u;                                            // the tile's P V completes one more phase
+                    fresh = false;
                 }
-                // eight arrivals a tile; in a block of one half its warps arrive for the others too (which nothing would pace)
+                // eight arrivals a tile: one of each warp, or two of each that has the tile to itself
                 __syncwarp();
-                if (lane == 0 && half_on) {
+                if (lane == 0 && mine) {
                     ptx::mbar_arrive(scale_bar(slot));
-                    if (rows <= 128) ptx::mbar_arrive(scale_bar(slot));
+                    if (!two) ptx::mbar_arrive(scale_bar(slot));
                 }
                 if (++slot == kScaleSlots) slot = 0;
             }
@@ -298,37 +310,93 @@ attn_chunk_kernel(const Args a)
                 if (FP8) m -= log2_factor(v_field);
                 const int part = 2 * blockIdx.x + (begins ? 1 : 0);
                 float* po = a.part + static_cast<size_t>(part) * kRows * (D + 2);
-                const bool whole_block = begins && ends;
-                const float f = !whole_block ? 1.0f : l == 0.0f ? 0.0f : __frcp_rn(l);
-                if (warp_on) {
+                const bool whole_block = begins && ends, joins = !two && todo > 1;
+                float f0 = 1.0f, f1 = 0.0f;
+                if (joins && h == 1) {
+                    odd_state[quad * 32 + lane] = make_float4(m, l, poison, 0.0f);
+                    ptx::tcgen05_fence_before_sync();
+                    __syncwarp();
+                    if (lane == 0) ptx::mbar_arrive(joined_bar);
+                    ok = ok && __all_sync(0xffffffffu, ptx::mbar_wait(read_bar, join_phase, a.status, 8));
+                } else if (joins) {
+                    ok = ok && __all_sync(0xffffffffu, ptx::mbar_wait(joined_bar, join_phase, a.status, 8));
+                    ptx::tcgen05_fence_after_sync();
+                    const float4 st = odd_state[quad * 32 + lane];
+                    const float mn = fmaxf(m, st.x), base = mn == -INFINITY ? 0.0f : mn;
+                    f0 = ptx::ex2(m - base);
+                    f1 = ptx::ex2(st.x - base);
+                    l = l * f0 + st.y * f1;
+                    m = mn;
+                    poison += st.z;
+                }
+                if (joins) join_phase ^= 1u;
+                const float inv = !whole_block ? 1.0f : l == 0.0f ? 0.0f : __frcp_rn(l);
+                f0 *= inv;
+                f1 *= inv;
+                if (warp_on && (two || h == 0)) {
+                    // A thread has a row: written from here, every 16 bytes would be a line of their own.  The rows of q (whose products
+                    // are done) lend the warp their place in shared memory, 256 (D = 64: 128) bytes a row, and it writes whole rows.
+                    const uint32_t place = q_base + h * C::kSlotBytes;
+                    const int my = quad * 32 + lane, in_warp = min(32, rows - (r_in - lane));
+                    constexpr int kPieces = D / 8;                            // 16-byte pieces of a row's place
+                    auto flush = [&](int col, bool f32) {
+                        __syncwarp();
+#pragma unroll
+                        for (int i = 0; i < kPieces; ++i) {                   // 32 * kPieces pieces, 32 at a time
+                            const int rr = i * (32 / kPieces) + lane / kPieces, piece = lane % kPieces;
+                            const uint4 w = ptx::ld_shared_v4(unit_at(place + (piece >> 3) * C::kHalfBytes, quad * 32 + rr, piece & 7));
+                            const size_t to = __shfl_sync(0xffffffffu, out_row, rr);
+                            if (rr < in_warp) {
+                                if (f32) *reinterpret_cast<uint4*>(po + (r_in - lane + rr) * D + col + piece * 4) = w;
+                                else *reinterpret_cast<uint4*>(a.out + to * D + piece * 8) = w;
+                            }
+                        }
+                        __syncwarp();
+                    };
 #pragma unroll 1
                     for (int i = 0; i < D; i += 32) {
                         uint32_t o[32];
                         ptx::tmem_ld_32x32b_x32(t_o + i, o);
                         ptx::tmem_ld_wait();
-                        if (r_in < rows) {
-                            if (whole_block) {
 #pragma unroll
-                                for (int k = 0; k < 32; k += 8) {
-                                    uint32_t w[4];
+                        for (int k = 0; k < 32; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * f0 + poison);
+                        if (joins) {
+                            uint32_t y[32];
+                            ptx::tmem_ld_32x32b_x32(t_o + D + i, y);
+                            ptx::tmem_ld_wait();
 #pragma unroll
-                                    for (int e = 0; e < 4; ++e) w[e] = pack_bf16x2(__uint_as_float(o[k + 2 * e]) * f + poison, __uint_as_float(o[k + 2 * e + 1]) * f + poison);
-                                    *reinterpret_cast<uint4*>(a.out + out_row * D + i + k) = make_uint4(w[0], w[1], w[2], w[3]);
-                                }
-                            } else {
+                            for (int k = 0; k < 32; ++k) o[k] = __float_as_uint(__uint_as_float(y[k]) * f1 + __uint_as_float(o[k]));
+                        }
+                        if (whole_block) {
 #pragma unroll
-                                for (int k = 0; k < 32; k += 4)
-                                    *reinterpret_cast<float4*>(po + r_in * D + i + k) = make_float4(__uint_as_float(o[k]) + poison, __uint_as_float(o[k + 1]) + poison,
-                                                                                                    __uint_as_float(o[k + 2]) + poison, __uint_as_float(o[k + 3]) + poison);
+                            for (int k = 0; k < 32; k += 8) {
+                                uint32_t w[4];
+#pragma unroll
+                                for (int e = 0; e < 4; ++e) w[e] = pack_bf16x2(__uint_as_float(o[k + 2 * e]), __uint_as_float(o[k + 2 * e + 1]));
+                                const int unit = (i + k) / 8;
+                                ptx::st_shared_v4(unit_at(place + (unit >> 3) * C::kHalfBytes, my, unit & 7), w[0], w[1], w[2], w[3]);
                             }
+                        } else {
+                            // 32 columns are half (D = 64: all) of the place
+#pragma unroll
+                            for (int k = 0; k < 32; k += 4) {
+                                const int unit = (i % (D / 2) + k) / 4;
+                                ptx::st_shared_v4(unit_at(place + (unit >> 3) * C::kHalfBytes, my, unit & 7), o[k], o[k + 1], o[k + 2], o[k + 3]);
+                            }
+                            if ((i + 32) % (D / 2) == 0) flush(i + 32 - D / 2, true);
                         }
                     }
+                    if (whole_block) flush(0, false);
                     if (r_in < rows) {
                         if (!whole_block) *reinterpret_cast<float2*>(po + kRows * D + r_in * 2) = make_float2(m, l);
                         else if (a.lse != nullptr) a.lse[out_row] = lse_of(m, l);
                     }
                 }
                 ptx::tcgen05_fence_before_sync();
+                if (joins && h == 0) {
+                    __syncwarp();
+                    if (lane == 0) ptx::mbar_arrive(read_bar);
+                }
                 if (threadIdx.x == 0 && begins && !ends) {
                     Open* op = a.open + blockIdx.x;
                     op->token0 = q.q0; op->r0 = r0; op->rows = rows; op->h = c.h;
@@ -349,11 +417,10 @@ attn_chunk_kernel(const Args a)
         const int lw = warp - 8;                                              // keys 32 * lw .. + 31 of a tile
         int slot = 0, sslot = 0;
         uint32_t phase = 0, sphase = 0;
-        int pending = -1;                                                     // bf16: the slot whose copies are in flight
-        int stage_in = 0, stage_out = 0;                                      // E4M3: of the staging area's three items
+        int stage_in = 0, stage_out = 0;                                      // E4M3: of the staging area's items
         while (c.at < c.end && ok) {
             const Range r = block_range(s, q, c.i, kRows, kTile);
-            const int todo = static_cast<int>(min(static_cast<long long>(r.tiles - c.tile), c.end - c.at));
+            const int todo = min(r.tiles - c.tile, c.end - c.at);
             const int* table = s.table + static_cast<size_t>(c.b) * s.max_pages;
             // the cache row of this lane's key of a tile, -1 for none
             auto row_of = [&](int tile) {
@@ -370,7 +437,7 @@ attn_chunk_kernel(const Args a)
             // different 16-byte units
             const int piece = FP8 && D == 128 ? (lane & 3) + ((lane >> 1) & 4) : lane % kPerRow;
             const int sub = FP8 && D == 128 ? ((lane >> 2) & 1) + ((lane >> 3) & 2) : lane / kPerRow;
-            // E4M3: a thread's pieces wait in its own places of the staging area (three items) until it converts them
+            // E4M3: a thread's pieces wait in its own places of the staging area until it converts them
             const uint32_t staged = staging + (lw * 32 + lane) * 16;
             uint32_t at[8 / kRowsAt > 0 ? 8 / kRowsAt : 1][2];                // where a piece's 16 elements (two units) go; the swizzle repeats after 8 rows
             if constexpr (FP8) {
@@ -387,20 +454,24 @@ attn_chunk_kernel(const Args a)
                     ptx::cp_async_16(to + i * 2048, static_cast<const uint8_t*>(cache) + static_cast<size_t>(max(from, 0)) * D + piece * 16, from >= 0 ? 16u : 0u);
                 }
                 ptx::cp_async_commit();
-                if (++stage_in == 3) stage_in = 0;
+                if (++stage_in == C::kStaged) stage_in = 0;
             };
-            // one tile ahead: the scales; two ahead: the rows
-            int row = row_of(r.tile0 + c.tile), next = todo > 1 ? row_of(r.tile0 + c.tile + 1) : -1;
+            // items are staged kStaged - 1 ahead (one tile, or two and a half); scales one tile ahead; rows as far as the items need them
+            constexpr int kFar = C::kStaged / 2;                              // tiles between an item and the one staged with it
+            int rows_ahead[kFar + 1];
+#pragma unroll
+            for (int i = 0; i <= kFar; ++i) rows_ahead[i] = i < todo ? row_of(r.tile0 + c.tile + i) : -1;
             float ks = 0.0f, vs = 0.0f;
             if (FP8) {
-                if (row >= 0) { ks = __ldg(a.k_scale + row); vs = __ldg(a.v_scale + row); }
-                stage_item(a.k_cache, row);
-                stage_item(a.v_cache, row);
+                if (rows_ahead[0] >= 0) { ks = __ldg(a.k_scale + rows_ahead[0]); vs = __ldg(a.v_scale + rows_ahead[0]); }
+#pragma unroll
+                for (int i = 0; i < C::kStaged - 1; ++i) stage_item(i % 2 == 0 ? a.k_cache : a.v_cache, rows_ahead[i / 2]);
             }
             for (int t = 0; t < todo && ok; ++t) {
-                const int after = t + 2 < todo ? row_of(r.tile0 + c.tile + t + 2) : -1;
+                const int row = rows_ahead[0];
+                const int after = t + kFar + 1 < todo ? row_of(r.tile0 + c.tile + t + kFar + 1) : -1;
                 float ks_next = 0.0f, vs_next = 0.0f;
-                if (FP8 && next >= 0) { ks_next = __ldg(a.k_scale + next); vs_next = __ldg(a.v_scale + next); }
+                if (FP8 && rows_ahead[1] >= 0) { ks_next = __ldg(a.k_scale + rows_ahead[1]); vs_next = __ldg(a.v_scale + rows_ahead[1]); }
                 // ---- the tile's mask and scales
                 ok = __all_sync(0xffffffffu, ptx::mbar_wait(scale_bar(sslot), sphase ^ 1u, a.status, 4));
                 if (!ok) break;
@@ -428,8 +499,11 @@ attn_chunk_kernel(const Args a)
                 for (int kv = 0; kv < 2; ++kv) {
                     const uint8_t* cache = static_cast<const uint8_t*>(kv == 0 ? a.k_cache : a.v_cache);
                     if (FP8) {
-                        stage_item(cache, next);                              // (an empty item behind the last tile)
-                        ptx::cp_async_wait<2>();
+                        // the item kStaged - 1 further on: with an odd distance of the other kind
+                        constexpr bool kOther = (C::kStaged - 1) % 2 != 0;
+                        const int far = kOther && kv == 1 ? rows_ahead[kFar] : rows_ahead[(C::kStaged - 1) / 2];
+                        stage_item(kOther == (kv == 0) ? a.v_cache : a.k_cache, far);   // (empty items behind the last tile)
+                        ptx::cp_async_wait<C::kStaged - 1>();
                     }
                     ok = __all_sync(0xffffffffu, ptx::mbar_wait(empty_bar(slot), phase ^ 1u, a.status, 1));
                     if (!ok) break;
@@ -444,7 +518,7 @@ attn_chunk_kernel(const Args a)
                             ptx::st_shared_v4(go + at[i % kPeriod][0], ptx::e4m3x2_lo(w.x), ptx::e4m3x2_hi(w.x), ptx::e4m3x2_lo(w.y), ptx::e4m3x2_hi(w.y));
                             ptx::st_shared_v4(go + at[i % kPeriod][1], ptx::e4m3x2_lo(w.z), ptx::e4m3x2_hi(w.z), ptx::e4m3x2_lo(w.w), ptx::e4m3x2_hi(w.w));
                         }
-                        if (++stage_out == 3) stage_out = 0;
+                        if (++stage_out == C::kStaged) stage_out = 0;
                         ptx::fence_proxy_async_smem();
                         __syncwarp();
                         if (lane == 0) ptx::mbar_arrive(full_bar(slot));
@@ -455,34 +529,25 @@ attn_chunk_kernel(const Args a)
                             ptx::cp_async_16(unit_at(to + (piece >> 3) * C::kHalfBytes, lw * 32 + i * kRowsAt + sub, piece & 7),
                                              cache + static_cast<size_t>(max(from, 0)) * (2 * D) + piece * 16, from >= 0 ? 16u : 0u);
                         }
-                        ptx::cp_async_commit();
-                        if (pending >= 0) {                                   // publish the one before while this one is in flight
-                            ptx::cp_async_wait<1>();
-                            ptx::fence_proxy_async_smem();
-                            __syncwarp();
-                            if (lane == 0) ptx::mbar_arrive(full_bar(pending));
-                        }
-                        pending = slot;
+                        ptx::cp_async_arrive(full_bar(slot));                 // as many items in flight as there are slots
                     }
                     if (++slot == C::kSlots) { slot = 0; phase ^= 1u; }
                 }
-                row = next; next = after;
+#pragma unroll
+                for (int i = 0; i < kFar; ++i) rows_ahead[i] = rows_ahead[i + 1];
+                rows_ahead[kFar] = after;
                 ks = ks_next; vs = vs_next;
             }
             if (FP8) {
-                ptx::cp_async_wait<0>();                                      // the two empty items
+                ptx::cp_async_wait<0>();                                      // the empty items
                 stage_in = stage_out;
             }
             c.at += todo;
             if (c.at < c.end) next_block(s, c, q, kRows);
         }
         if (!FP8) {
+            ptx::cp_async_commit();
             ptx::cp_async_wait<0>();
-            if (pending >= 0 && ok) {
-                ptx::fence_proxy_async_smem();
-                __syncwarp();
-                if (lane == 0) ptx::mbar_arrive(full_bar(pending));
-            }
         }
     } else {
         // ================================================================================================ products
@@ -493,8 +558,11 @@ attn_chunk_kernel(const Args a)
             constexpr uint32_t id_o = ptx::umma_idesc(fmt, fmt, 128, D) | ptx::kIdescBMnMajor;
             int slot = 0;
             uint32_t phase = 0, q_phase[2] = {0, 0}, p_phase[2] = {0, 0};
-            auto scores = [&](int h, uint32_t k_at) {
-                const uint64_t dq = ptx::smem_desc_sw128_kmajor(q_base + h * C::kSlotBytes), dk = ptx::smem_desc_sw128_kmajor(k_at);
+            // copied (not converted) tiles reach the barrier by the copies themselves: their writers pass no proxy fence
+            auto landed = [&]() { if (!FP8) ptx::fence_proxy_async_smem(); };
+            auto advance = [&]() { if (++slot == C::kSlots) { slot = 0; phase ^= 1u; } };
+            auto scores = [&](int h, int q_half, uint32_t k_at) {
+                const uint64_t dq = ptx::smem_desc_sw128_kmajor(q_base + q_half * C::kSlotBytes), dk = ptx::smem_desc_sw128_kmajor(k_at);
 #pragma unroll
                 for (int i = 0; i < D / 16; ++i) {
                     const uint64_t step = (i >> 2) * (C::kHalfBytes >> 4) + 2 * (i & 3);
@@ -516,20 +584,31 @@ attn_chunk_kernel(const Args a)
                         q_phase[1] ^= 1u;
                     }
                     ptx::tcgen05_fence_after_sync();
-                    if (ok) scores(h, ring + slot * C::kSlotBytes);
+                    landed();
+                    if (ok) scores(h, h, ring + slot * C::kSlotBytes);
                 }
                 ptx::umma_commit(empty_bar(slot));
-                if (++slot == C::kSlots) { slot = 0; phase ^= 1u; }
+                advance();
                 for (int t = 0; t < todo && ok; ++t) {
                     const int v_slot = slot;
                     const uint32_t v_phase = phase;
-                    if (++slot == C::kSlots) { slot = 0; phase ^= 1u; }
+                    advance();
                     const bool on = t + 1 < todo;
                     const int k_slot = slot;
                     const uint32_t k_phase = phase;
-                    if (on && ++slot == C::kSlots) { slot = 0; phase ^= 1u; }
-                    for (int h = 0; h < halves && ok; ++h) {
-                        if (h == 0) ok = ptx::mbar_wait(full_bar(v_slot), v_phase, a.status, 5);
+                    if (on) advance();
+                    if (halves == 1 && on) {                                  // the next tile's scores go to the other S first
+                        ok = ptx::mbar_wait(full_bar(k_slot), k_phase, a.status, 5);
+                        if (!ok) break;
+                        ptx::tcgen05_fence_after_sync();
+                        landed();
+                        scores((t + 1) & 1, 0, ring + k_slot * C::kSlotBytes);
+                        ptx::umma_commit(empty_bar(k_slot));
+                    }
+                    for (int n = 0; n < halves && ok; ++n) {
+                        const int h = halves == 2 ? n : t & 1;
+                        const bool sum = halves == 2 ? t > 0 : t > 1;         // O_h holds earlier tiles
+                        if (n == 0) { ok = ptx::mbar_wait(full_bar(v_slot), v_phase, a.status, 5); landed(); }
                         const uint64_t dv = ptx::smem_desc_sw128_mnmajor(ring + v_slot * C::kSlotBytes, C::kHalfBytes);
 #pragma unroll
                         for (int i = 0; i < kTile / 16; ++i) {                // 16 keys: 8 columns of P, 2 KB of each column of V
@@ -538,20 +617,21 @@ attn_chunk_kernel(const Args a)
                                 if (!ok) break;
                                 ptx::tcgen05_fence_after_sync();
                             }
-                            ptx::umma_f16_ts(tmem + C::kOCol + h * D, tmem + h * 128 + 8 * i, dv + (2048 >> 4) * i, id_o, t > 0 || i > 0);
+                            ptx::umma_f16_ts(tmem + C::kOCol + h * D, tmem + h * 128 + 8 * i, dv + (2048 >> 4) * i, id_o, sum || i > 0);
                         }
                         if (!ok) break;
                         p_phase[h] ^= 1u;
                         ptx::umma_commit(o_bar(h));
-                        if (h == halves - 1) ptx::umma_commit(empty_bar(v_slot));
-                        if (on) {
-                            if (h == 0) {
+                        if (n == halves - 1) ptx::umma_commit(empty_bar(v_slot));
+                        if (halves == 2 && on) {
+                            if (n == 0) {
                                 ok = ptx::mbar_wait(full_bar(k_slot), k_phase, a.status, 5);
                                 if (!ok) break;
                                 ptx::tcgen05_fence_after_sync();
+                                landed();
                             }
-                            scores(h, ring + k_slot * C::kSlotBytes);
-                            if (h == halves - 1) ptx::umma_commit(empty_bar(k_slot));
+                            scores(h, h, ring + k_slot * C::kSlotBytes);
+                            if (n == 1) ptx::umma_commit(empty_bar(k_slot));
                         }
                     }
                 }
@@ -582,7 +662,8 @@ int launch(const Args& args, cudaStream_t stream)
         if (e != cudaSuccess) return e;
         if (dev < 64) configured[dev] = true;
     }
-    if (static_cast<long long>(a.s.seqs) * 8 > C::kQBytes + C::kSlots * C::kSlotBytes) return cudaErrorInvalidValue;
+    if (static_cast<long long>(a.s.seqs) * 4 > C::kQBytes + C::kSlots * C::kSlotBytes) return cudaErrorInvalidValue;
+    if (!tiles_fit(a, kRows, kTile)) return cudaErrorInvalidValue;
     a.block_limit = static_cast<int>((static_cast<long long>(a.max_q) * a.s.group + kRows - 1) / kRows);
     const int ctas = num_sms();
     kernel<<<ctas, kThreads, C::kSmemBytes, stream>>>(a);

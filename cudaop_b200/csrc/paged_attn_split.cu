@@ -43,7 +43,7 @@ struct Cfg {
     static constexpr int kScaleBytes = FP8 ? kTile * 4 : 0;
     static constexpr int kStageBytes = (2 * kTensorBytes + 2 * kScaleBytes + 1023) / 1024 * 1024;
     static constexpr int kJoinBytes = kRows * D * 4;                          // one warp's accumulators
-    static constexpr int kBudget = 227 * 1024 / kCtasPerSm - 1024 - 3 * 1024 - kJoinBytes;
+    static constexpr int kBudget = 227 * 1024 / kCtasPerSm - 1024 - 1024 - 768 - kJoinBytes;     // (1 KB the system keeps, 1 KB to align, states)
     static constexpr int kStages = kBudget / kStageBytes < 8 ? kBudget / kStageBytes : 8;
     static_assert(kStages >= 2, "ring");
     static constexpr int kStateBytes = kConsumers * kRows * 8;                // running maximum and sum per warp and row
@@ -108,7 +108,7 @@ attn_split_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
         for (int i = 0; i < C::kStages; ++i) { ptx::mbar_init(full_bar(i), 1); ptx::mbar_init(empty_bar(i), kConsumers); }
         ptx::fence_mbar_init();
     }
-    Cursor c = find_work(s, kRows, kTile, reinterpret_cast<long long*>(smem_raw + (ring - raw)), a.block_limit, blockIdx.x, gridDim.x);
+    Cursor c = find_work(s, kRows, kTile, reinterpret_cast<int*>(smem_raw + (ring - raw)), a.block_limit, blockIdx.x, gridDim.x);
     if (threadIdx.x == 0) a.open[blockIdx.x].last = -1;
     if (c.at == c.end) return;
     ptx::fence_proxy_async_smem();             // the ring held the prefix sums; the loads that follow are the async proxy's
@@ -124,7 +124,7 @@ attn_split_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
         bool ok = true;
         while (c.at < c.end && ok) {
             const Range r = block_range(s, q, c.i, kRows, kTile);
-            const int todo = static_cast<int>(min(static_cast<long long>(r.tiles - c.tile), c.end - c.at));
+            const int todo = min(r.tiles - c.tile, c.end - c.at);
             const int* table = s.table + static_cast<size_t>(c.b) * s.max_pages;
             auto page_of = [&](int tile) {                          // lane < boxes: the page of its box of the tile, -1 for none
                 const int key = tile * kTile + lane * box;
@@ -187,7 +187,7 @@ attn_split_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
     bool ok = true;
     while (c.at < c.end) {
         const Range r = block_range(s, q, c.i, kRows, kTile);
-        const int todo = static_cast<int>(min(static_cast<long long>(r.tiles - c.tile), c.end - c.at));
+        const int todo = min(r.tiles - c.tile, c.end - c.at);
         const int r0 = c.i * kRows, rows = min(kRows, q.n * s.group - r0);
         // q: this thread holds row 8 * nt + g; what belongs to rows 2cc + {0, 1} comes from the lanes that hold them
         uint32_t qb[NT][C::kSteps][2];
@@ -523,7 +523,8 @@ int launch(const Args& args, cudaStream_t stream)
         if (e != cudaSuccess) return e;
         if (dev < 64) configured[dev] = true;
     }
-    if (static_cast<long long>(a.s.seqs) * 8 > C::kStages * C::kStageBytes) return cudaErrorInvalidValue;
+    if (static_cast<long long>(a.s.seqs) * 4 > C::kStages * C::kStageBytes) return cudaErrorInvalidValue;
+    if (!tiles_fit(a, C::kRows, kTile)) return cudaErrorInvalidValue;
     a.block_limit = static_cast<int>((static_cast<long long>(a.max_q) * a.s.group + C::kRows - 1) / C::kRows);
     const int ctas = C::kCtasPerSm * num_sms();
     kernel<<<ctas, kThreads, C::kSmemBytes, stream>>>(tmK, tmV, a);

@@ -54,30 +54,29 @@ __device__ __forceinline__ Range block_range(const Shape& s, const Seq& q, int i
 }
 
 // The work of a call is the list of all tiles: sequence by sequence, kv head by kv head, row block by row block, tile by
-// tile.  CTA c of g (g at most W / kMinTiles) takes the tiles [c * W / g, (c + 1) * W / g), whatever the lengths are: every CTA gets the same number, and a
-// long sequence is split over as many CTAs as it takes.  A block whose tiles lie in several CTAs leaves partial results
-// (running maximum, sum, unnormalised output), joined by the combine kernel in CTA order.
+// tile.  The CTAs take equal shares of it (of kMinTiles at least), whatever the lengths are; a long sequence is split over as
+// many CTAs as it takes.  A block whose tiles lie in several CTAs leaves partial results (running maximum, sum,
+// unnormalised output), joined by the combine kernel in CTA order.  Tile counts are 32-bit numbers (the host checks the bound).
 // Tiles a CTA has at least: a part costs a write, a read and a turn of the combine kernel (one sequence of 1500 tokens, 8 kv heads: 13.9 us with
 // 1, 11.5 with 2, 11.3 with 3, 11.7 with 4).
 constexpr int kMinTiles = 3;
 struct Cursor {
     int b, h, i;              // sequence, kv head, row block
     int tile;                 // first tile (counted from the block's tile0) this CTA takes of the block
-    long long at, end;        // this CTA's tiles, as indices of the list; at == end: nothing left
-    long long total;          // length of the list
-    int ctas;                 // CTAs that have work
+    int at, end;              // this CTA's tiles, as indices of the list; at == end: nothing left
+    int share, extra;         // tiles of a CTA; the first `extra` CTAs have one more
 };
 
-// Whole CTA; `prefix` holds seqs 64-bit words in shared memory (free again after the call, which ends in a barrier).
+// Whole CTA; `prefix` holds seqs words in shared memory (free again after the call, which ends in a barrier).
 // `block_limit`: an upper bound of the row blocks of one sequence.
-__device__ __forceinline__ Cursor find_work(const Shape& s, int rm, int kt, long long* prefix, int block_limit, int cta, int ctas)
+__device__ __forceinline__ Cursor find_work(const Shape& s, int rm, int kt, int* prefix, int block_limit, int cta, int ctas)
 {
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
     if (block_limit <= 8) {                        // a thread per sequence
         for (int b = threadIdx.x; b < s.seqs; b += blockDim.x) {
             const Seq q = load_seq(s, b);
             const int blocks = (q.n * s.group + rm - 1) / rm;
-            long long w = 0;
+            int w = 0;
             for (int i = 0; i < blocks; ++i) w += block_range(s, q, i, rm, kt).tiles;
             prefix[b] = w * s.kv_heads;
         }
@@ -85,21 +84,20 @@ __device__ __forceinline__ Cursor find_work(const Shape& s, int rm, int kt, long
         for (int b = warp; b < s.seqs; b += warps) {
             const Seq q = load_seq(s, b);
             const int blocks = (q.n * s.group + rm - 1) / rm;
-            long long w = 0;
+            int w = 0;
             for (int i = lane; i < blocks; i += 32) w += block_range(s, q, i, rm, kt).tiles;
-#pragma unroll
-            for (int o = 16; o > 0; o >>= 1) w += __shfl_xor_sync(0xffffffffu, w, o);
+            w = __reduce_add_sync(0xffffffffu, w);
             if (lane == 0) prefix[b] = w * s.kv_heads;
         }
     }
     __syncthreads();
     if (warp == 0) {                               // inclusive prefix sums
-        long long run = 0;
+        int run = 0;
         for (int b0 = 0; b0 < s.seqs; b0 += 32) {
-            long long v = b0 + lane < s.seqs ? prefix[b0 + lane] : 0;
+            int v = b0 + lane < s.seqs ? prefix[b0 + lane] : 0;
 #pragma unroll
             for (int o = 1; o < 32; o <<= 1) {
-                const long long u = __shfl_up_sync(0xffffffffu, v, o);
+                const int u = __shfl_up_sync(0xffffffffu, v, o);
                 if (lane >= o) v += u;
             }
             v += run;
@@ -108,24 +106,24 @@ __device__ __forceinline__ Cursor find_work(const Shape& s, int rm, int kt, long
         }
     }
     __syncthreads();
-    const long long total = s.seqs > 0 ? prefix[s.seqs - 1] : 0;
+    const int total = s.seqs > 0 ? prefix[s.seqs - 1] : 0;
+    const int used = min(ctas, (total + kMinTiles - 1) / kMinTiles);
     Cursor c{};
-    c.total = total;
-    c.ctas = static_cast<int>(min(static_cast<long long>(ctas), (total + kMinTiles - 1) / kMinTiles));
-    if (cta < c.ctas) {
-        const long long first = total * cta / c.ctas;
-        c.at = first;
-        c.end = total * (cta + 1) / c.ctas;
-        int lo = 0, hi = s.seqs - 1;               // first sequence whose inclusive prefix exceeds `first`
+    if (cta < used) {
+        c.share = total / used;
+        c.extra = total - c.share * used;
+        c.at = cta * c.share + min(cta, c.extra);
+        c.end = c.at + c.share + (cta < c.extra ? 1 : 0);
+        int lo = 0, hi = s.seqs - 1;               // first sequence whose inclusive prefix exceeds c.at
         while (lo < hi) {
             const int mid = (lo + hi) / 2;
-            if (prefix[mid] > first) hi = mid; else lo = mid + 1;
+            if (prefix[mid] > c.at) hi = mid; else lo = mid + 1;
         }
         c.b = lo;
-        const long long before = lo > 0 ? prefix[lo - 1] : 0;
-        const long long per_head = (prefix[lo] - before) / s.kv_heads;
-        long long rem = first - before;
-        c.h = static_cast<int>(rem / per_head);
+        const int before = lo > 0 ? prefix[lo - 1] : 0;
+        const int per_head = (prefix[lo] - before) / s.kv_heads;
+        int rem = c.at - before;
+        c.h = rem / per_head;
         rem -= c.h * per_head;
         const Seq q = load_seq(s, lo);
         for (c.i = 0;; ++c.i) {
@@ -133,10 +131,17 @@ __device__ __forceinline__ Cursor find_work(const Shape& s, int rm, int kt, long
             if (rem < t) break;
             rem -= t;
         }
-        c.tile = static_cast<int>(rem);
+        c.tile = rem;
     }
     __syncthreads();
     return c;
+}
+
+// The CTA that does tile t of the list.
+__device__ __forceinline__ int owner(const Cursor& c, int t)
+{
+    const int head = c.extra * (c.share + 1);      // tiles of the CTAs that have one more
+    return t < head ? t / (c.share + 1) : c.extra + (t - head) / c.share;
 }
 
 // The next block after (b, h, i), called while tiles are left; sequences without rows are passed over.
@@ -149,9 +154,6 @@ __device__ __forceinline__ void next_block(const Shape& s, Cursor& c, Seq& q, in
     c.h = 0;
     do { q = load_seq(s, ++c.b); } while (q.n == 0);
 }
-
-// The CTA that does tile t of the list.
-__device__ __forceinline__ int owner(const Cursor& c, long long t) { return static_cast<int>(((t + 1) * c.ctas - 1) / c.total); }
 
 // What a CTA leaves for the combine kernel: the block whose first tiles it did and whose last it did not.
 struct Open {

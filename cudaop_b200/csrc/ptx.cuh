@@ -600,19 +600,6 @@ __device__ __forceinline__ void tma_load_3d(uint32_t smem_dst, const CUtensorMap
         ::"r"(smem_dst), "l"(reinterpret_cast<uint64_t>(tm)), "r"(bar), "r"(x), "r"(y), "r"(z)
         : "memory");
 }
-// cp.async.bulk.prefetch.L2: brings a contiguous range (16-byte aligned, a multiple of 16 bytes) into L2 only
-__device__ __forceinline__ void bulk_prefetch(const void* gsrc, uint32_t bytes)
-{
-    asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(gsrc), "r"(bytes) : "memory");
-}
-// cp.async.bulk.prefetch.tensor.2d.L2: brings a box into L2 only
-__device__ __forceinline__ void tma_prefetch_2d(const CUtensorMap* tm, int x, int y)
-{
-    asm volatile("cp.async.bulk.prefetch.tensor.2d.L2.global.tile [%0, {%1, %2}];"
-                 ::"l"(reinterpret_cast<uint64_t>(tm)), "r"(x), "r"(y)
-                 : "memory");
-}
-
 // tcgen05.cp.cta_group::2.128x128b: both CTAs copy 128 rows x 16 bytes from their own shared memory into four
 // columns of their own tensor memory
 __device__ __forceinline__ void tmem_cp_128x128b_pair(uint32_t taddr, uint64_t smem_desc)
@@ -793,6 +780,11 @@ __device__ __forceinline__ float ld_shared_f32(uint32_t smem_addr)
 __device__ __forceinline__ void cp_async_16(uint32_t smem_dst, const void* src, uint32_t bytes)
 {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_dst), "l"(src), "r"(bytes) : "memory");
+}
+// cp.async.mbarrier.arrive.noinc: one of the barrier's expected arrivals, once this thread's copies so far have landed
+__device__ __forceinline__ void cp_async_arrive(uint32_t bar)
+{
+    asm volatile("cp.async.mbarrier.arrive.noinc.shared.b64 [%0];" ::"r"(bar) : "memory");
 }
 __device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N>

@@ -187,7 +187,7 @@ template <int kVecs>
 __global__ void __launch_bounds__(256)
 quant_rows_mxfp4_kernel(const __nv_bfloat16* __restrict__ X, uint32_t* __restrict__ Q, uint8_t* __restrict__ SF, int rows, int k32)
 {
-    pdl_launch_dependents();                                          // the product may set up and bring its weights nearer meanwhile
+    pdl_launch_dependents();                                          // the product that reads this may set up meanwhile
     const int lane = threadIdx.x & 31;
     const int k128 = (k32 + 3) / 4;
     const bool words = (k32 & 3) == 0;                                // four scales of a 128-K slab lie in sixteen neighbouring lanes
@@ -196,42 +196,47 @@ quant_rows_mxfp4_kernel(const __nv_bfloat16* __restrict__ X, uint32_t* __restric
     const long long spans = (vecs + 32 * kVecs - 1) / (32 * kVecs);
     const uint4* x = reinterpret_cast<const uint4*>(X);
     for (long long sp = (static_cast<long long>(blockIdx.x) * blockDim.x + threadIdx.x) >> 5; sp < spans; sp += warps) {
+        const long long v0 = sp * (32 * kVecs) + lane;
+        const int left = static_cast<int>(min(vecs - v0, static_cast<long long>(32 * kVecs)));       // this lane's vectors: i * 32 < left
+        const uint4* xp = x + v0;
         uint4 v[kVecs];
 #pragma unroll
-        for (int i = 0; i < kVecs; ++i) {
-            const long long vi = (sp * kVecs + i) * 32 + lane;
-            v[i] = vi < vecs ? __ldg(x + vi) : make_uint4(0, 0, 0, 0);
-        }
+        for (int i = 0; i < kVecs; ++i) v[i] = i * 32 < left ? __ldg(xp + i * 32) : make_uint4(0, 0, 0, 0);
+        // row and block of the first vector; the next one of a lane is eight blocks further on  (2^32 blocks would be more than
+        // the memory holds; a 64-bit division here per vector was a quarter of the kernel's instructions)
+        const uint32_t blk = static_cast<uint32_t>(v0 >> 2);
+        uint32_t r = blk / static_cast<uint32_t>(k32), j = blk - r * k32;
+        auto row_at = [&]() { return SF + static_cast<size_t>(r >> 7) * k128 * 512 + (r & 31) * 16 + ((r >> 5) & 3) * 4; };
+        uint8_t* sf_row = row_at();
 #pragma unroll
         for (int i = 0; i < kVecs; ++i) {
-            const long long vi = (sp * kVecs + i) * 32 + lane;
             const uint32_t w[4] = {v[i].x, v[i].y, v[i].z, v[i].w};
-            uint32_t m2 = 0;
-#pragma unroll
-            for (int k = 0; k < 4; ++k) m2 = __vmaxu2(m2, w[k] & 0x7FFF7FFFu);
+            const uint32_t m2 = __vmaxu2(__vmaxu2(w[0] & 0x7FFF7FFFu, w[1] & 0x7FFF7FFFu), __vmaxu2(w[2] & 0x7FFF7FFFu, w[3] & 0x7FFF7FFFu));
             uint32_t mx = max(m2 & 0xFFFFu, m2 >> 16);
             mx = max(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
             mx = max(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
             const uint32_t ex = mx >> 7;                              // biased exponent of the maximum
             const bool finite = ex < 255u;
-            const uint32_t s8 = !finite ? 255u : ex > 2u ? ex - 2u : 0u;
+            const uint32_t s8 = !finite ? 255u : max(ex, 2u) - 2u;
             const float inv = __uint_as_float((254u - s8) << 23);     // 2^(127 - s8); unused when not finite
             float y[8];
 #pragma unroll
             for (int k = 0; k < 4; ++k) { y[2 * k] = bf16_lo(w[k]) * inv; y[2 * k + 1] = bf16_hi(w[k]) * inv; }
-            if (vi < vecs) Q[vi] = finite ? cvt8_e2m1(y) : 0u;
-            uint32_t word = s8;
+            const uint32_t q = finite ? cvt8_e2m1(y) : 0u;
+            if (i * 32 < left) Q[v0 + i * 32] = q;
             if (words) {
-                word |= __shfl_down_sync(0xffffffffu, s8, 4) << 8;
-                word |= __shfl_down_sync(0xffffffffu, s8, 8) << 16;
-                word |= __shfl_down_sync(0xffffffffu, s8, 12) << 24;
+                uint32_t word = s8 | (__shfl_down_sync(0xffffffffu, s8, 4) << 8);
+                word |= __shfl_down_sync(0xffffffffu, word, 8) << 16;
+                if ((lane & 15) == 0 && i * 32 < left) *reinterpret_cast<uint32_t*>(sf_row + (j >> 2) * 512u) = word;
+            } else if ((lane & 3) == 0 && i * 32 < left) {
+                sf_row[(j >> 2) * 512u + (j & 3)] = static_cast<uint8_t>(s8);
             }
-            if ((lane & (words ? 15 : 3)) == 0 && vi < vecs) {
-                const long long blk = vi >> 2;
-                const int r = static_cast<int>(blk / k32), j = static_cast<int>(blk - static_cast<long long>(r) * k32);
-                uint8_t* to = SF + (static_cast<size_t>(r >> 7) * k128 + (j >> 2)) * 512 + (r & 31) * 16 + ((r >> 5) & 3) * 4 + (j & 3);
-                if (words) *reinterpret_cast<uint32_t*>(to) = word;
-                else *to = static_cast<uint8_t>(s8);
+            if (i + 1 < kVecs) {
+                j += 8;
+                if (j >= static_cast<uint32_t>(k32)) {
+                    do { j -= k32; ++r; } while (j >= static_cast<uint32_t>(k32));
+                    sf_row = row_at();
+                }
             }
         }
     }
@@ -293,7 +298,7 @@ extern "C" int b200q_quant_rows_mxfp4(const void* X, void* Q, void* SF_blocked, 
 {
     using namespace b200q;
     if (X == nullptr || Q == nullptr || SF_blocked == nullptr) return cudaErrorInvalidValue;
-    if (rows <= 0 || cols <= 0 || cols % 32 != 0) return cudaErrorInvalidValue;
+    if (rows <= 0 || cols <= 0 || cols % 32 != 0 || static_cast<long long>(rows) * (cols / 32) > 0xFFFFFFFFll) return cudaErrorInvalidValue;
     if (!aligned16(X) || (reinterpret_cast<uintptr_t>(Q) & 3u) != 0 || !aligned16(SF_blocked)) return cudaErrorInvalidValue;
     const int sms = num_sms();
     if (sms <= 0) return cudaErrorInvalidDevice;
