@@ -300,13 +300,16 @@ def paged_attention(q, k_cache, v_cache, page_table, cu_q, kv_lens, max_q: int, 
     """Attention of a chunk of new tokens per sequence over a paged cache that holds them already; bf16 like ``q``.
 
     ``q``: bf16 [tokens, heads, head_dim] (slices of a fused projection's output are taken as they are), the chunks of the
-    sequences one after the other: rows ``cu_q[b]`` to ``cu_q[b + 1]`` (int32 [seqs + 1], from 0; lengths may differ, and be
-    zero).  They are the last tokens of the ``kv_lens[b]`` (int32 [seqs]) cached ones.  ``max_q``: a bound of the chunk
+    sequences (at most 8192) one after the other: rows ``cu_q[b]`` to ``cu_q[b + 1]`` (int32 [seqs + 1], from 0; lengths may
+    differ, and be zero).  They are the last tokens of the ``kv_lens[b]`` (int32 [seqs]) cached ones.  ``max_q``: a bound of the chunk
     lengths (it chooses the kernel; a wrong one costs time only).  ``heads`` is a multiple of the cache's kv_heads; query
     head h reads kv head h // (heads // kv_heads).  ``page_table``: int32 [seqs, max_pages]; a token whose page number is not in
     the cache is left out.
     A token at position p sees keys j <= p (``causal``; else all), and with a ``window`` only j > p - window.  A row
-    that sees nothing is zero.  ``scale``: of the scores, 1 / sqrt(head_dim) by default.
+    that sees nothing is zero.  ``scale``: of the scores, 1 / sqrt(head_dim) by default.  What lies in slots that no token of
+    the sequence has may be anything, NaN included.  Tokens that some rows of a chunk see and others do not (those of the
+    chunk itself) reach only the rows that see them, with one exception: in a bf16 cache a value of theirs that is NaN or
+    infinite makes that column NaN in the other rows too.
     ``return_lse``: returns (out, lse), lse fp32 [tokens, heads] the natural log of the sum of exponentials (-inf for a row that
     sees nothing).  Rows of no sequence are zero, or left as they are where ``out`` is given."""
     o, lse = _ext().paged_attention(q, k_cache, v_cache, page_table, cu_q, kv_lens, int(max_q), k_scale, v_scale,

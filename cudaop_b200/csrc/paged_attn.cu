@@ -40,6 +40,8 @@ int b200q_paged_attention(const void* q, const void* k_cache, const void* v_cach
     if (window < 0 || (window > 0 && !causal) || !(softmax_scale == softmax_scale)) return cudaErrorInvalidValue;
     if (q_stride % 8 || q_head_stride % 8 || !aligned16(q) || !aligned16(k_cache) || !aligned16(v_cache) || !aligned16(out) ||
         !aligned16(workspace) || (fp8 && (!aligned16(k_scale) || !aligned16(v_scale)))) return cudaErrorInvalidValue;
+    // the work is counted in shared memory, a word per sequence
+    if (seqs > 8192) return cudaErrorInvalidValue;
     // positions, rows of a chunk and rows of the cache are 32-bit numbers
     const long long most = 0x7FFFFFFFll - 4096;
     if ((static_cast<long long>(max_pages) << shift) > most || static_cast<long long>(tokens) * heads > most ||

@@ -16,7 +16,7 @@
 // A block of no more than 128 rows has no second half: its even tiles go through S_0, O_0 and warps 0-3, its odd tiles through S_1, O_1
 // and warps 4-7, with a running maximum and sum of their own, and warps 0-3 join the two at the end (the same TMEM lanes hold the
 // same rows).  With one half alone the block was one chain of product, softmax, product (24 sequences of up to 16 new on up to 8192 tokens, 32/4
-// heads of 64: 49 us, 32 us so).
+// heads of 64: 49 us, 45 us so).
 // TMEM: S_0 S_1 (128 columns each), O_0 O_1 (D columns each).  The running maximum is raised, and O rescaled in TMEM by the row's
 // own thread, only when it grows by more than 2^4 (exact: the sum uses the same base); after the first tiles that is rare.
 #include "paged_common.cuh"
@@ -47,6 +47,7 @@ struct Cfg {
     static constexpr int kBars = 2 * kSlots + kScaleSlots + 12;
     static constexpr int kSmemBytes = 1024 + kQBytes + kSlots * kSlotBytes + kStaged * kStagedBytes + kScaleSlots * kScaleBytes + kBars * 8 + 32 + 128 * 16;
     static constexpr int kOCol = 256;
+    static_assert(kQBytes + kSlots * kSlotBytes >= 8192 * 4, "a word per sequence");
 };
 
 // p * scale / (power of two above the largest scale) is kept times kRoom = 2^11: at most 2^15, and fp16 starts to lose bits only where
@@ -662,7 +663,6 @@ int launch(const Args& args, cudaStream_t stream)
         if (e != cudaSuccess) return e;
         if (dev < 64) configured[dev] = true;
     }
-    if (static_cast<long long>(a.s.seqs) * 4 > C::kQBytes + C::kSlots * C::kSlotBytes) return cudaErrorInvalidValue;
     if (!tiles_fit(a, kRows, kTile)) return cudaErrorInvalidValue;
     a.block_limit = static_cast<int>((static_cast<long long>(a.max_q) * a.s.group + kRows - 1) / kRows);
     const int ctas = num_sms();

@@ -431,10 +431,11 @@ std::tuple<torch::Tensor, c10::optional<torch::Tensor>> paged_attention(
     check_index(kv_lens, "kv_lens", kI32, 1, k_cache);
     TORCH_CHECK_VALUE(page_table.size(0) == seqs && cu_q.numel() == seqs + 1, "page_table, cu_q and kv_lens must agree on the number of sequences");
     TORCH_CHECK_VALUE(seqs > 0 && page_table.size(1) > 0, "there must be a sequence and a page");
+    TORCH_CHECK_VALUE(seqs <= 8192, "at most 8192 sequences, got ", num(seqs));
     TORCH_CHECK_VALUE(max_q > 0, "max_q must be positive");
     TORCH_CHECK_VALUE(window >= 0 && (window == 0 || causal), "window must not be negative, and needs causal");
     TORCH_CHECK_VALUE(std::isfinite(scale), "scale must be finite");
-    TORCH_CHECK_VALUE(tokens * heads <= INT32_MAX - 4096 && page_table.size(1) <= (INT32_MAX - 4096) / c.page && seqs <= INT32_MAX - 4096,
+    TORCH_CHECK_VALUE(tokens * heads <= INT32_MAX - 4096 && page_table.size(1) <= (INT32_MAX - 4096) / c.page,
                       "sizes pass 32 bits");
     const c10::cuda::CUDAGuard guard(k_cache.device());
     const bool given = out.has_value();

@@ -315,6 +315,46 @@ def test_strided_queries_scale_and_given_output(kernel, n):
     b.check(b.call(q=q))
 
 
+@pytest.mark.parametrize("fp8", [True, False])
+@pytest.mark.parametrize("scale", [-0.2, 0.0, 1e-3])
+def test_scales_that_are_negative_zero_and_small(kernel, scale, fp8):
+    b = Batch([1, 30, 150], [200, 64, 150], 8, 2, 64, 16, fp8)
+    b.check(b.call(scale=scale), scale=scale)
+
+
+@pytest.mark.parametrize("fp8", [True, False])
+def test_groups_larger_than_a_block_of_rows(kernel, fp8):
+    b = Batch([1, 3, 2], [100, 3, 257], 300, 1, 64, 32, fp8)
+    b.check(b.call())
+
+
+@pytest.mark.parametrize("dim,fp8", [(128, True), (64, False)])
+def test_queries_of_very_different_size(kernel, dim, fp8):
+    """Elements of a row, and rows, from 2^-60 to 2^40: an E4M3 cache's fp16 queries are scaled row by row."""
+    b = Batch([40], [300], 4, 1, dim, 16, fp8)
+    g = torch.Generator().manual_seed(8)
+    q = b.q.float() * torch.exp2(torch.randint(-12, 1, b.q.shape, generator=g).float())
+    q[::5] *= 2.0 ** -60
+    q[1::5] *= 2.0 ** 20                                             # (these rows' scores pick one key each)
+    b.q = q.bfloat16()
+    b.check(b.call())
+
+
+def test_lengths_that_contradict_the_tensors_stay_inside_them(kernel):
+    """Starts that go back, pass the end or are negative, lengths beyond the table: rows of such a call are not defined,
+    but nothing is read or written outside the tensors."""
+    b = Batch([20, 20, 20], [100, 100, 100], 4, 2, 64, 16, True)
+    for cu in ([0, 50, 10, 60], [-5, 10, 1000, 2000], [70, 80, 90, 100], [60, 0, 0, 0], [-2 ** 31, 2 ** 31 - 1, 0, 7]):
+        for kv in ([100, 100, 100], [2 ** 31 - 1, -2 ** 31, 5]):
+            guard = torch.full((60 + 64, 4, 64), 9.0, dtype=torch.bfloat16, device="cuda")
+            b.call(cu_q=torch.tensor(cu, dtype=torch.int32).cuda(), kv_lens=torch.tensor(kv, dtype=torch.int32).cuda(), out=guard[32:92])
+            torch.cuda.synchronize()
+            assert (guard[:32] == 9.0).all() and (guard[92:] == 9.0).all()
+    import cudaop_b200 as ops
+    assert ops.status() == 0
+    b.check(b.call())
+
+
 @pytest.mark.parametrize("n,fp8", [(1, True), (1, False), (40, True), (200, False)])
 def test_large_scores_and_equal_runs(kernel, n, fp8):
     """Scores of hundreds: the running maximum moves at every tile; and two runs give the same bits."""
@@ -405,6 +445,29 @@ def test_side_stream_and_graph(n):
     graphs[0][2]["kv_lens"].copy_(torch.tensor(b.kv))
     graphs[0][0].replay()
     b.check(graphs[0][1])
+
+
+@pytest.mark.parametrize("n", [1, 150])
+def test_after_work_that_is_still_running(n):
+    """The cache write, the attention and what reads it in one stream, behind a kernel that takes long."""
+    import cudaop_b200 as ops
+    b = Batch([n, n], [600, 333], 8, 2, 128, 16, True)
+    want = b.call()
+    big = torch.empty(1 << 28, device="cuda")
+    fresh = names(empty_cache(b.pages, 2, 16, 128, True))
+    slots = torch.cat([b.table[s][torch.arange(c) // 16].long() * 16 + torch.arange(c) % 16 for s, c in enumerate(b.kv)]).cuda()
+    k, v = torch.cat(b.k).cuda(), torch.cat(b.v).cuda()
+    args = dict(page_table=b.table.cuda(), cu_q=b.cu.cuda(), kv_lens=torch.tensor(b.kv, dtype=torch.int32).cuda(), max_q=n, return_lse=True)
+    q = b.q.cuda()
+    torch.cuda.synchronize()
+    for _ in range(3):
+        big.normal_()
+        ops.paged_cache_write(k, v, slots, **fresh)
+        got = ops.paged_attention(q, **args, **fresh)
+        copy = got[0].clone()
+        for t in fresh.values():
+            t.view(torch.uint8).fill_(0x7F)
+        assert torch.equal(copy, want[0]) and torch.equal(got[1], want[1])
 
 
 def test_a_layer_of_quantised_inference():

@@ -27,7 +27,7 @@ BAD = [dict(q=None), dict(kc=None), dict(vs=None), dict(cu=None), dict(ws=None),
        dict(ws=P + 8), dict(seqs=0), dict(tokens=0), dict(heads=7), dict(heads=0), dict(kv_heads=0), dict(dim=96), dict(dim=256), dict(page=8),
        dict(page=48), dict(page=256), dict(qs=1020), dict(qh=100), dict(max_q=0), dict(max_pages=0), dict(pages=0), dict(window=-1),
        dict(window=8, causal=0), dict(scale=float("nan")), dict(max_pages=2 ** 27, page=16), dict(pages=2 ** 27, page=16),
-       dict(tokens=2 ** 28, heads=8)]
+       dict(tokens=2 ** 28, heads=8), dict(seqs=8193)]
 
 
 @pytest.mark.parametrize("bad", BAD, ids=str)
