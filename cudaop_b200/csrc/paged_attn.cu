@@ -50,7 +50,7 @@ int b200q_paged_attention(const void* q, const void* k_cache, const void* v_cach
 
     Args a{};
     a.s.cu_q = cu_q; a.s.kv_lens = kv_lens; a.s.table = page_table;
-    a.s.seqs = seqs; a.s.tokens = tokens; a.s.heads = heads; a.s.kv_heads = kv_heads; a.s.group = heads / kv_heads;
+    a.s.seqs = seqs; a.s.tokens = tokens; a.s.heads = heads; a.s.kv_heads = kv_heads; a.s.set_group(heads / kv_heads);
     a.s.max_pages = max_pages; a.s.page_shift = shift; a.s.num_pages = num_pages;
     a.s.causal = causal != 0; a.s.window = window;
     a.q = static_cast<const __nv_bfloat16*>(q); a.q_stride = q_stride; a.q_head = q_head_stride;

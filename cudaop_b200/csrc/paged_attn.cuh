@@ -109,7 +109,7 @@ combine_kernel(const Args a, int rows_per_block)
         }
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
-        const int r = op.r0 + row, t = r / a.s.group;
+        const int r = op.r0 + row, t = a.s.token_of(r);
         const size_t to = static_cast<size_t>(op.token0 + t) * a.s.heads + op.h * a.s.group + r - t * a.s.group;
         const float inv = l == 0.0f ? 0.0f : __frcp_rn(l);
         if constexpr (kPer == 4)

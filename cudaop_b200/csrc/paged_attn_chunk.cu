@@ -125,38 +125,44 @@ attn_chunk_kernel(const Args a)
             const int r_in = (two ? h * 128 : 0) + quad * 32 + lane;          // row inside the block
             const bool half_on = two || todo > h, warp_on = (two ? h * 128 : 0) + quad * 32 < rows;
             const int row = min(r_in, rows - 1);                              // rows behind the block repeat its last one
-            const int tok = (r0 + row) / s.group, head = c.h * s.group + (r0 + row) - tok * s.group;
+            const int tok = s.token_of(r0 + row), head = c.h * s.group + (r0 + row) - tok * s.group;
             const int pos = q.kv - q.n + tok;
             const size_t out_row = static_cast<size_t>(q.q0 + tok) * s.heads + head;
             float row_scale = fabsf(a.scale_log2);
             if (half_on) {
-                // ---- this thread's row of q into shared memory; the sign of the softmax scale goes into it, so that the
-                // factor of the scores is not negative (nor zero)
-                const uint4* qp = reinterpret_cast<const uint4*>(a.q + (q.q0 + tok) * a.q_stride + head * a.q_head);
-                uint4 w[D / 8];
-#pragma unroll
-                for (int i = 0; i < D / 8; ++i) w[i] = __ldg(qp + i);
-                float down = a.scale_log2 > 0.0f ? 1.0f : a.scale_log2 < 0.0f ? -1.0f : 0.0f;
+                // ---- the warp's rows of q into shared memory, a few whole rows at a time (code that runs once a block is bound by
+                // the fetch of its instructions: short loops, not unrolled ones); the sign of the softmax scale goes into them,
+                // so that the factor of the scores is not negative (nor zero)
+                const long long q_row = (q.q0 + tok) * a.q_stride + head * a.q_head;
+                const float sign = a.scale_log2 > 0.0f ? 1.0f : a.scale_log2 < 0.0f ? -1.0f : 0.0f;
                 if (a.scale_log2 == 0.0f) row_scale = 1.0f;
-                if (FP8) {
-                    uint32_t m2 = 0;
+                constexpr int kLanes = D / 8, kAt = 32 / kLanes;              // lanes of a row, rows at a time
+                const int piece = lane % kLanes, sub = lane / kLanes;
+                uint32_t my_e = 127;
+#pragma unroll 8
+                for (int i = 0; i < 32 / kAt; ++i) {
+                    const int rr = i * kAt + sub;
+                    const uint4 w = __ldg(reinterpret_cast<const uint4*>(a.q + __shfl_sync(0xffffffffu, q_row, rr)) + piece);
+                    float down = sign;
+                    if (FP8) {
+                        uint32_t m2 = __vmaxu2(__vmaxu2(w.x & 0x7FFF7FFFu, w.y & 0x7FFF7FFFu), __vmaxu2(w.z & 0x7FFF7FFFu, w.w & 0x7FFF7FFFu));
+                        uint32_t mx = max(m2 & 0xFFFFu, m2 >> 16);
 #pragma unroll
-                    for (int i = 0; i < D / 8; ++i)
-                        m2 = __vmaxu2(__vmaxu2(m2, __vmaxu2(w[i].x & 0x7FFF7FFFu, w[i].y & 0x7FFF7FFFu)), __vmaxu2(w[i].z & 0x7FFF7FFFu, w[i].w & 0x7FFF7FFFu));
-                    const uint32_t e = min(max(max(m2 & 0xFFFFu, m2 >> 16) >> 7, 1u), 253u);
-                    down *= pow2_of_field(254u - e);
-                    row_scale *= pow2_of_field(e);
-                }
-#pragma unroll
-                for (int i = 0; i < D / 8; ++i) {
-                    uint32_t v[4] = {w[i].x, w[i].y, w[i].z, w[i].w};
+                        for (int o = 1; o < kLanes; o <<= 1) mx = max(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+                        const uint32_t e = min(max(mx >> 7, 1u), 253u);       // exponent field of the row's largest element
+                        down *= pow2_of_field(254u - e);
+                        const uint32_t mine = __shfl_sync(0xffffffffu, e, (lane % kAt) * kLanes);
+                        if (lane / kAt == i) my_e = mine;
+                    }
+                    uint32_t v[4] = {w.x, w.y, w.z, w.w};
 #pragma unroll
                     for (int k = 0; k < 4; ++k) {
                         const float lo = __uint_as_float(v[k] << 16) * down, hi = __uint_as_float(v[k] & 0xFFFF0000u) * down;
                         v[k] = FP8 ? pack_f16x2(lo, hi) : pack_bf16x2(lo, hi);
                     }
-                    if (two || h == 0) ptx::st_shared_v4(unit_at(q_base + h * C::kSlotBytes + (i >> 3) * C::kHalfBytes, quad * 32 + lane, i & 7), v[0], v[1], v[2], v[3]);
+                    if (two || h == 0) ptx::st_shared_v4(unit_at(q_base + h * C::kSlotBytes + (piece >> 3) * C::kHalfBytes, quad * 32 + rr, piece & 7), v[0], v[1], v[2], v[3]);
                 }
+                if (FP8) row_scale *= pow2_of_field(my_e);
                 ptx::fence_proxy_async_smem();
                 if (threadIdx.x == 0) { block_info[0] = todo; block_info[1] = two ? 2 : 1; }
                 __syncwarp();
@@ -342,7 +348,7 @@ attn_chunk_kernel(const Args a)
                     constexpr int kPieces = D / 8;                            // 16-byte pieces of a row's place
                     auto flush = [&](int col, bool f32) {
                         __syncwarp();
-#pragma unroll
+#pragma unroll 2
                         for (int i = 0; i < kPieces; ++i) {                   // 32 * kPieces pieces, 32 at a time
                             const int rr = i * (32 / kPieces) + lane / kPieces, piece = lane % kPieces;
                             const uint4 w = ptx::ld_shared_v4(unit_at(place + (piece >> 3) * C::kHalfBytes, quad * 32 + rr, piece & 7));

@@ -198,7 +198,7 @@ attn_split_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
             const int row = min(8 * nt + g, rows - 1);               // rows behind the block repeat its last one
-            const int t = (r0 + row) / s.group;
+            const int t = s.token_of(r0 + row);
             const __nv_bfloat16* qp = a.q + (q.q0 + t) * a.q_stride + (c.h * s.group + (r0 + row) - t * s.group) * a.q_head;
 #pragma unroll
             for (int ks = 0; ks < C::kSteps; ++ks) {
@@ -470,7 +470,7 @@ attn_split_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
                     const int row = 8 * nt + 2 * cc + u;
                     if (begins && ends) {
                         if (row >= rows) continue;
-                        const int t = (r0 + row) / s.group;
+                        const int t = s.token_of(r0 + row);
                         const size_t to = static_cast<size_t>(q.q0 + t) * s.heads + c.h * s.group + (r0 + row) - t * s.group;
                         const float inv = l[nt][u] == 0.0f ? 0.0f : __frcp_rn(l[nt][u]);
 #pragma unroll

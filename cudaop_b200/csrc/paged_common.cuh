@@ -19,6 +19,23 @@ struct Shape {
     int seqs, tokens, heads, kv_heads, group;
     int max_pages, page_shift, num_pages;
     int causal, window;       // window 0 = none; a window implies causal
+    unsigned group_mul, group_shift;        // x / group without a division: see token_of
+
+    // Token of row r of a chunk, r / group, for 0 <= r < 2^31: with s = ceil(log2 group) and mul = ceil(2^(31 + s) / group) the
+    // product r * mul / 2^(31 + s) is off by less than 1 / group (mul * group exceeds 2^(31 + s) by less than 2^s), so its
+    // integer part is the quotient.  A row's code runs once per block and is bound by instruction fetch, where a division
+    // costs twenty of them.
+    __host__ void set_group(int g)
+    {
+        group = g;
+        group_shift = 0;
+        while ((1 << group_shift) < g) ++group_shift;
+        group_mul = static_cast<unsigned>(((1ull << (31 + group_shift)) + g - 1) / g);
+    }
+    __host__ __device__ int token_of(int r) const
+    {
+        return static_cast<int>((static_cast<unsigned long long>(r) * group_mul) >> (31 + group_shift));
+    }
 };
 
 // Lengths as the caller gave them, made safe: whatever the arrays hold, rows stay inside q and keys inside the table.
@@ -43,7 +60,7 @@ struct Range {
 __device__ __forceinline__ Range block_range(const Shape& s, const Seq& q, int i, int rm, int kt)
 {
     const int r0 = i * rm, r1 = min(q.n * s.group, r0 + rm);
-    const int first = q.kv - q.n + r0 / s.group, last = q.kv - q.n + (r1 - 1) / s.group;   // positions of the block's tokens
+    const int first = q.kv - q.n + s.token_of(r0), last = q.kv - q.n + s.token_of(r1 - 1);   // positions of the block's tokens
     Range r;
     r.hi = s.causal ? min(q.cap, last + 1) : q.cap;
     r.lo = s.window > 0 ? max(0, first - s.window + 1) : 0;
