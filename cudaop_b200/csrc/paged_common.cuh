@@ -73,7 +73,8 @@ __device__ __forceinline__ Range block_range(const Shape& s, const Seq& q, int i
 // The work of a call is the list of all tiles: sequence by sequence, kv head by kv head, row block by row block, tile by
 // tile.  The CTAs take equal shares of it (of kMinTiles at least), whatever the lengths are; a long sequence is split over as
 // many CTAs as it takes.  A block whose tiles lie in several CTAs leaves partial results (running maximum, sum,
-// unnormalised output), joined by the combine kernel in CTA order.  Tile counts are 32-bit numbers (the host checks the bound).
+// unnormalised output), joined by the combine kernel in CTA order.  Tile counts are 32-bit numbers: the host refuses calls whose
+// sizes could pass that, and starts that contradict one another (chunks that overlap) and pass it all the same do no work.
 // Tiles a CTA has at least: a part costs a write, a read and a turn of the combine kernel (one sequence of 1500 tokens, 8 kv heads: 13.9 us with
 // 1, 11.5 with 2, 11.3 with 3, 11.7 with 4).
 constexpr int kMinTiles = 3;
@@ -84,6 +85,13 @@ struct Cursor {
     int share, extra;         // tiles of a CTA; the first `extra` CTAs have one more
 };
 
+constexpr int kTooMany = 0x7FFFFFFF;
+__device__ __forceinline__ int add_capped(int a, int b)           // a, b in [0, kTooMany]
+{
+    return static_cast<int>(min(static_cast<unsigned>(a) + static_cast<unsigned>(b), static_cast<unsigned>(kTooMany)));
+}
+__device__ __forceinline__ int capped(long long w) { return static_cast<int>(min(w, static_cast<long long>(kTooMany))); }
+
 // Whole CTA; `prefix` holds seqs words in shared memory (free again after the call, which ends in a barrier).
 // `block_limit`: an upper bound of the row blocks of one sequence.
 __device__ __forceinline__ Cursor find_work(const Shape& s, int rm, int kt, int* prefix, int block_limit, int cta, int ctas)
@@ -93,18 +101,19 @@ __device__ __forceinline__ Cursor find_work(const Shape& s, int rm, int kt, int*
         for (int b = threadIdx.x; b < s.seqs; b += blockDim.x) {
             const Seq q = load_seq(s, b);
             const int blocks = (q.n * s.group + rm - 1) / rm;
-            int w = 0;
+            long long w = 0;
             for (int i = 0; i < blocks; ++i) w += block_range(s, q, i, rm, kt).tiles;
-            prefix[b] = w * s.kv_heads;
+            prefix[b] = capped(w * s.kv_heads);
         }
     } else {                                       // a warp per sequence
         for (int b = warp; b < s.seqs; b += warps) {
             const Seq q = load_seq(s, b);
             const int blocks = (q.n * s.group + rm - 1) / rm;
-            int w = 0;
+            long long w = 0;
             for (int i = lane; i < blocks; i += 32) w += block_range(s, q, i, rm, kt).tiles;
-            w = __reduce_add_sync(0xffffffffu, w);
-            if (lane == 0) prefix[b] = w * s.kv_heads;
+#pragma unroll
+            for (int o = 16; o > 0; o >>= 1) w += __shfl_xor_sync(0xffffffffu, w, o);
+            if (lane == 0) prefix[b] = capped(w * s.kv_heads);
         }
     }
     __syncthreads();
@@ -115,15 +124,15 @@ __device__ __forceinline__ Cursor find_work(const Shape& s, int rm, int kt, int*
 #pragma unroll
             for (int o = 1; o < 32; o <<= 1) {
                 const int u = __shfl_up_sync(0xffffffffu, v, o);
-                if (lane >= o) v += u;
+                if (lane >= o) v = add_capped(v, u);
             }
-            v += run;
+            v = add_capped(v, run);
             if (b0 + lane < s.seqs) prefix[b0 + lane] = v;
             run = __shfl_sync(0xffffffffu, v, 31);
         }
     }
     __syncthreads();
-    const int total = s.seqs > 0 ? prefix[s.seqs - 1] : 0;
+    const int counted = s.seqs > 0 ? prefix[s.seqs - 1] : 0, total = counted == kTooMany ? 0 : counted;
     const int used = min(ctas, (total + kMinTiles - 1) / kMinTiles);
     Cursor c{};
     if (cta < used) {

@@ -355,6 +355,21 @@ def test_lengths_that_contradict_the_tensors_stay_inside_them(kernel):
     b.check(b.call())
 
 
+def test_overlapping_chunks_beyond_the_count_of_tiles_do_nothing(kernel):
+    """4096 sequences that all claim the same 20000 rows and a table of 10^6 tokens: more tiles than 32 bits count."""
+    import cudaop_b200 as ops
+    seqs, T = 4096, 20000
+    cu = torch.zeros(seqs + 1, dtype=torch.int32)
+    cu[1::2] = T
+    cache = names(empty_cache(4, 1, 128, 64, True))
+    out = torch.full((T, 8, 64), 9.0, dtype=torch.bfloat16, device="cuda")
+    table = torch.full((seqs, 8192), -1, dtype=torch.int32, device="cuda")
+    ops.paged_attention(torch.zeros_like(out), page_table=table, cu_q=cu.cuda(), kv_lens=torch.full((seqs,), 2 ** 20, dtype=torch.int32).cuda(),
+                        max_q=T, causal=False, out=out, **cache)
+    torch.cuda.synchronize()
+    assert ops.status() == 0 and (out == 9.0).all()
+
+
 @pytest.mark.parametrize("n,fp8", [(1, True), (1, False), (40, True), (200, False)])
 def test_large_scores_and_equal_runs(kernel, n, fp8):
     """Scores of hundreds: the running maximum moves at every tile; and two runs give the same bits."""
