@@ -307,9 +307,8 @@ def paged_attention(q, k_cache, v_cache, page_table, cu_q, kv_lens, max_q: int, 
     the cache is left out.
     A token at position p sees keys j <= p (``causal``; else all), and with a ``window`` only j > p - window.  A row
     that sees nothing is zero.  ``scale``: of the scores, 1 / sqrt(head_dim) by default.  What lies in slots that no token of
-    the sequence has may be anything, NaN included.  Tokens that some rows of a chunk see and others do not (those of the
-    chunk itself) reach only the rows that see them, with one exception: in a bf16 cache a value of theirs that is NaN or
-    infinite makes that column NaN in the other rows too (in an E4M3 cache only a NaN byte would, and the write stores none).
+    the sequence has may be anything, NaN included, and a token reaches only the rows that see it, whatever its values are.  (An
+    E4M3 cache says NaN in its scales; a NaN byte, which the write never stores, would reach a whole block of rows.)
     ``return_lse``: returns (out, lse), lse fp32 [tokens, heads] the natural log of the sum of exponentials (-inf for a row that
     sees nothing).  Rows of no sequence are zero, or left as they are where ``out`` is given."""
     o, lse = _ext().paged_attention(q, k_cache, v_cache, page_table, cu_q, kv_lens, int(max_q), k_scale, v_scale,

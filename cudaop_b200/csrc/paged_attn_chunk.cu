@@ -45,7 +45,7 @@ struct Cfg {
     static constexpr int kScaleAt = 48;
     static constexpr int kScaleBytes = kScaleAt + (FP8 ? 2 * kTile * 4 : 0);
     static constexpr int kBars = 2 * kSlots + kScaleSlots + 12;
-    static constexpr int kSmemBytes = 1024 + kQBytes + kSlots * kSlotBytes + kStaged * kStagedBytes + kScaleSlots * kScaleBytes + kBars * 8 + 32 + 128 * 16;
+    static constexpr int kSmemBytes = 1024 + kQBytes + kSlots * kSlotBytes + kStaged * kStagedBytes + kScaleSlots * kScaleBytes + kBars * 8 + 64 + 128 * 16;
     static constexpr int kOCol = 256;
     static_assert(kQBytes + kSlots * kSlotBytes >= 8192 * 4, "a word per sequence");
 };
@@ -60,6 +60,13 @@ __device__ __forceinline__ uint32_t pack_f16x2(float lo, float hi)
 {
     const __half2 v = __floats2half2_rn(lo, hi);
     return *reinterpret_cast<const uint32_t*>(&v);
+}
+// two bf16 with those that are not finite set to zero
+__device__ __forceinline__ uint32_t only_finite(uint32_t w)
+{
+    if ((w & 0x7F80u) == 0x7F80u) w &= 0xFFFF0000u;
+    if ((w & 0x7F800000u) == 0x7F800000u) w &= 0x0000FFFFu;
+    return w;
 }
 // 16-byte unit `unit` of row `row` in a [rows][128 bytes] column with the 128-byte swizzle
 __device__ __forceinline__ uint32_t unit_at(uint32_t column, int row, int unit) { return column + row * 128 + ((unit ^ (row & 7)) << 4); }
@@ -87,7 +94,8 @@ attn_chunk_kernel(const Args a)
     const uint32_t joined_bar = more + 8u * 10, read_bar = more + 8u * 11;    // odd tiles' states are there / have been read
     const uint32_t tmem_slot = bars + C::kBars * 8;
     int* block_info = reinterpret_cast<int*>(smem_raw + (tmem_slot + 4 - raw));        // for the products: tiles (0: no more blocks), halves
-    float4* odd_state = reinterpret_cast<float4*>(smem_raw + ((bars + C::kBars * 8 + 32 + 15) / 16 * 16 - raw));       // [128] maximum, sum, poison
+    float4* odd_state = reinterpret_cast<float4*>(smem_raw + ((bars + C::kBars * 8 + 48 + 15) / 16 * 16 - raw));       // [128] maximum, sum, poison
+    int* odd_block = block_info + 3;                                          // [8] by the block's number: it has values that are not finite
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const Shape& s = a.s;
 
@@ -95,6 +103,7 @@ attn_chunk_kernel(const Args a)
     if (threadIdx.x == 0) {
         for (int i = 0; i < C::kSlots; ++i) { ptx::mbar_init(full_bar(i), FP8 ? 4 : 128); ptx::mbar_init(empty_bar(i), 1); }
         for (int i = 0; i < kScaleSlots; ++i) ptx::mbar_init(scale_bar(i), 8);
+        for (int i = 0; i < 8; ++i) odd_block[i] = 0;
         for (int h = 0; h < 2; ++h) { ptx::mbar_init(q_bar(h), 4); ptx::mbar_init(s_bar(h), 1); ptx::mbar_init(p_bar(h, 0), 4); ptx::mbar_init(p_bar(h, 1), 4); ptx::mbar_init(o_bar(h), 1); }
         ptx::mbar_init(joined_bar, 4); ptx::mbar_init(read_bar, 4);
         ptx::fence_mbar_init();
@@ -108,6 +117,16 @@ attn_chunk_kernel(const Args a)
     Seq q{};
     if (c.at < c.end) q = load_seq(s, c.b);
     bool ok = true;
+    // Whether some row of a block does not see a key of the tile that others do.  Values there that are not finite (in a bf16 cache) would
+    // pass the product as 0 * infinity into the rows that do not see them: the loaders set them to zero, note it for the
+    // block, and the rows that do see them get them at the end.
+    auto edge = [&](const Range& r, int i, int tile) {
+        const int first = max(tile * kTile, r.lo), end = min(tile * kTile + kTile, r.hi);
+        const int r1 = min(q.n * s.group, (i + 1) * kRows) - 1;
+        return first < end && ((s.causal && end - 1 > q.kv - q.n + s.token_of(i * kRows)) ||
+                               (s.window > 0 && first <= q.kv - q.n + s.token_of(r1) - s.window));
+    };
+    int block_no = 0;                                                         // blocks so far, the same in all roles
 
     if (warp < 8) {
         // ================================================================================================ softmax
@@ -118,6 +137,7 @@ attn_chunk_kernel(const Args a)
         uint32_t s_phase = 0, o_phase = 0, join_phase = 0;
         int slot = 0;                                                         // of the scale ring
         while (c.at < c.end && ok) {
+            ++block_no;
             const Range r = block_range(s, q, c.i, kRows, kTile);
             const int todo = min(r.tiles - c.tile, c.end - c.at);
             const int r0 = c.i * kRows, rows = min(kRows, q.n * s.group - r0);
@@ -374,6 +394,23 @@ attn_chunk_kernel(const Args a)
 #pragma unroll
                             for (int k = 0; k < 32; ++k) o[k] = __float_as_uint(__uint_as_float(y[k]) * f1 + __uint_as_float(o[k]));
                         }
+                        if (!FP8 && *static_cast<volatile int*>(odd_block + (block_no & 7)) == block_no) {
+#pragma unroll 1
+                            for (int key = (r.tile0 + c.tile) * kTile; key < (r.tile0 + c.tile + todo) * kTile; ++key) {
+                                if (key < r.lo || key >= r.hi || !edge(r, c.i, key / kTile)) continue;
+                                const int page = __ldg(s.table + static_cast<size_t>(c.b) * s.max_pages + (key >> s.page_shift));
+                                if (page < 0 || page >= s.num_pages) continue;
+                                const size_t from = (static_cast<size_t>(page * s.kv_heads + c.h) << s.page_shift) + (key & ((1 << s.page_shift) - 1));
+                                const bool seen = (!s.causal || key <= pos) && (s.window == 0 || key > pos - s.window);
+#pragma unroll
+                                for (int k = 0; k < 32; k += 2) {
+                                    const uint32_t w = __ldg(static_cast<const uint32_t*>(a.v_cache) + (from * D + i + k) / 2);
+                                    const uint32_t odd = w ^ only_finite(w);
+                                    if (seen && (odd & 0xFFFFu)) o[k] = __float_as_uint(__uint_as_float(o[k]) + __uint_as_float(w << 16));
+                                    if (seen && (odd >> 16)) o[k + 1] = __float_as_uint(__uint_as_float(o[k + 1]) + __uint_as_float(w & 0xFFFF0000u));
+                                }
+                            }
+                        }
                         if (whole_block) {
 #pragma unroll
                             for (int k = 0; k < 32; k += 8) {
@@ -426,6 +463,7 @@ attn_chunk_kernel(const Args a)
         uint32_t phase = 0, sphase = 0;
         int stage_in = 0, stage_out = 0;                                      // E4M3: of the staging area's items
         while (c.at < c.end && ok) {
+            ++block_no;
             const Range r = block_range(s, q, c.i, kRows, kTile);
             const int todo = min(r.tiles - c.tile, c.end - c.at);
             const int* table = s.table + static_cast<size_t>(c.b) * s.max_pages;
@@ -536,7 +574,24 @@ attn_chunk_kernel(const Args a)
                             ptx::cp_async_16(unit_at(to + (piece >> 3) * C::kHalfBytes, lw * 32 + i * kRowsAt + sub, piece & 7),
                                              cache + static_cast<size_t>(max(from, 0)) * (2 * D) + piece * 16, from >= 0 ? 16u : 0u);
                         }
-                        ptx::cp_async_arrive(full_bar(slot));                 // as many items in flight as there are slots
+                        if (kv == 1 && edge(r, c.i, r.tile0 + c.tile + t)) {
+                            ptx::cp_async_commit();
+                            ptx::cp_async_wait<0>();
+#pragma unroll 2
+                            for (int i = 0; i < kInstr; ++i) {                // each thread looks at what it copied
+                                const uint32_t at_piece = unit_at(to + (piece >> 3) * C::kHalfBytes, lw * 32 + i * kRowsAt + sub, piece & 7);
+                                const uint4 y = ptx::ld_shared_v4(at_piece);
+                                const uint4 z = make_uint4(only_finite(y.x), only_finite(y.y), only_finite(y.z), only_finite(y.w));
+                                if (((y.x ^ z.x) | (y.y ^ z.y) | (y.z ^ z.z) | (y.w ^ z.w)) != 0u) {
+                                    ptx::st_shared_v4(at_piece, z.x, z.y, z.z, z.w);
+                                    odd_block[block_no & 7] = block_no;
+                                }
+                            }
+                            ptx::fence_proxy_async_smem();
+                            ptx::mbar_arrive(full_bar(slot));                 // (every thread is one of the barrier's arrivals)
+                        } else {
+                            ptx::cp_async_arrive(full_bar(slot));             // as many items in flight as there are slots
+                        }
                     }
                     if (++slot == C::kSlots) { slot = 0; phase ^= 1u; }
                 }

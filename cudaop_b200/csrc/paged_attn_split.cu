@@ -69,6 +69,39 @@ __device__ __forceinline__ uint32_t swizzled(uint32_t base, int row, int byte)
     return base + (a ^ (kBox == 128 ? (a >> 3) & 0x70u : (a >> 3) & 0x30u));
 }
 
+// two bf16 with those that are not finite set to zero
+__device__ __forceinline__ uint32_t only_finite(uint32_t w)
+{
+    if ((w & 0x7F80u) == 0x7F80u) w &= 0xFFFF0000u;
+    if ((w & 0x7F800000u) == 0x7F800000u) w &= 0x0000FFFFu;
+    return w;
+}
+
+// Adds the values of a half tile's 16 keys that are not finite to the rows that see them; `at`: the first of the warp's rows, whose
+// eight 16-byte units are swizzled; a lane has columns of unit g.  Rare, and short rather than fast.
+template <int NT, int STEPS, typename Seen>
+__device__ __forceinline__ void add_not_finite(float (&o)[NT][STEPS][4], int h, uint32_t at, int g, uint32_t valid, Seen seen)
+{
+#pragma unroll 1
+    for (int j = 0; j < 16; ++j) {
+        if (!((valid >> j) & 1u)) continue;
+        const uint4 y = ptx::ld_shared_v4(at + j * 128 + ((g ^ (j & 7)) << 4));
+        const uint32_t w[4] = {y.x, y.y, y.z, y.w};
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            const float v = __uint_as_float(e & 1 ? w[e >> 1] & 0xFFFF0000u : w[e >> 1] << 16);
+            const bool odd = (__float_as_uint(v) & 0x7F800000u) == 0x7F800000u;
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                for (int u = 0; u < 2; ++u)
+#pragma unroll
+                    for (int hh = 0; hh < STEPS / 4; ++hh)
+                        if (hh == h && odd && seen(j, nt, u)) o[nt][4 * hh + (e >> 1)][2 * (e & 1) + u] += v;
+        }
+    }
+}
+
 template <bool FP8>
 __device__ __forceinline__ void mma(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1)
 {
@@ -383,11 +416,26 @@ attn_split_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
                 } else {
 #pragma unroll
                     for (int h = 0; h < C::kHalves; ++h) {
-                        uint32_t w[4][4];
+                        uint32_t w[4][4], top = 0;
 #pragma unroll
                         for (int i = 0; i < 4; ++i) {
                             const uint4 y = ptx::ld_shared_v4(swizzled<128>(vb + h * C::kHalfBytes, vr + (i & 1) + 8 * (i >> 1), g * 16));
                             w[i][0] = in[i] ? y.x : 0u; w[i][1] = in[i] ? y.y : 0u; w[i][2] = in[i] ? y.z : 0u; w[i][3] = in[i] ? y.w : 0u;
+#pragma unroll
+                            for (int j = 0; j < 4; ++j) top = __vmaxu2(top, w[i][j] & 0x7FFF7FFFu);
+                        }
+                        if (__any_sync(0xffffffffu, max(top & 0xFFFFu, top >> 16) >= 0x7F80u)) {
+                            // Values that are not finite: a product would carry them, as 0 * infinity, into the rows that do not see
+                            // their key (and turn an infinity into NaN by the second term of p).  They are added by themselves.
+                            add_not_finite<NT>(o, h, swizzled<128>(vb + h * C::kHalfBytes, warp * 16, 0), g, valid,
+                                               [&](int j, int nt, int u) {
+                                                   const int key = key0 + j;
+                                                   return (!s.causal || key <= pos[nt][u]) && (s.window == 0 || key > pos[nt][u] - s.window);
+                                               });
+#pragma unroll
+                            for (int i = 0; i < 4; ++i)
+#pragma unroll
+                                for (int j = 0; j < 4; ++j) w[i][j] = only_finite(w[i][j]);
                         }
 #pragma unroll
                         for (int j = 0; j < 4; ++j) {

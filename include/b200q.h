@@ -169,8 +169,9 @@ int b200q_paged_cache_read(const void* k_cache, const void* v_cache, const float
  * [seqs + 1]) are the last tokens of the kv_lens[b] (DEVICE int32 [seqs]) cached ones; the token at position p sees keys
  * j <= p (causal != 0), and j > p - window (window > 0, needs causal); rows that see nothing are zero, lse -inf.  max_q: a
  * bound of the chunk lengths (speed only).  Tokens on pages outside the cache are left out.  Rows of no sequence are zeroed
- * (zero_rest != 0) or left.  At most 8192 sequences.  A bf16 value that is not finite, of a token that some rows of a chunk see
- * and others do not, reaches the others as NaN; anything else that a row does not see does not reach it.  Row (token, head) of q is at token * q_stride + head * q_head_stride elements.  `workspace`:
+ * (zero_rest != 0) or left.  At most 8192 sequences.  A token reaches only the rows that see it, whatever its
+ * values are (an E4M3 cache says NaN in its scales; a NaN byte, which the write never stores, would reach a whole block of
+ * rows). Row (token, head) of q is at token * q_stride + head * q_head_stride elements.  `workspace`:
  * caller-owned scratch of b200q_paged_attention_workspace_bytes(head_dim) bytes, 16-byte aligned, no contents needed, not to be
  * shared by calls that may overlap. */
 int b200q_paged_attention(const void* q, const void* k_cache, const void* v_cache, const float* k_scale, const float* v_scale,

@@ -395,6 +395,41 @@ def test_a_nan_key_reaches_the_rows_that_see_it(kernel):
     assert ((out[:4].double().cpu() - want[:4]).abs() <= tol[:4]).all()
 
 
+@pytest.mark.parametrize("window", [0, 40])
+@pytest.mark.parametrize("n,group,dim", [(8, 2, 128), (150, 4, 64), (30, 8, 128)])
+def test_values_that_are_not_finite_reach_the_rows_that_see_them_alone(kernel, n, group, dim, window):
+    """bf16 cache: NaN and infinities in values (and keys) of tokens that some rows see and others do not."""
+    import cudaop_b200 as ops
+    kv = 200
+    b = Batch([n], [kv], 2 * group, 2, dim, 16, False, seed=7)
+    g = torch.Generator().manual_seed(n)
+    odd = {kv - 1: NAN, kv - n // 2: math.inf, kv - n: -math.inf, kv - n + 1: math.inf, 100: NAN, 3: -math.inf}
+    for j, value in odd.items():
+        b.v[0][j, torch.randint(0, 2, (1,), generator=g), torch.randint(0, dim, (3,), generator=g)] = value
+    b.v[0][kv - n + 2, 1] = NAN                                      # a whole row
+    at = torch.arange(kv)
+    slots = b.table[0][at // 16].long() * 16 + at % 16
+    ops.paged_cache_write(b.k[0].cuda(), b.v[0].cuda(), slots.cuda(), **names(b.cache))
+    out, lse = b.call(window=window)
+    torch.cuda.synchronize()
+    assert ops.status() == 0
+    want, wlse, tol, ltol = b.expect(window=window)
+    # what the rows that see a value that is not finite have in its column
+    v = b.v[0].double().repeat_interleave(group, 1)
+    bad = torch.where(torch.isfinite(v), torch.zeros_like(v), v)
+    p, j = torch.arange(n).unsqueeze(1) + kv - n, torch.arange(kv).unsqueeze(0)
+    seen = (j <= p) & ((j > p - window) if window else True)
+    for i in range(n):
+        want[i] += bad[seen[i]].sum(0)
+    out, lse = out.double().cpu(), lse.double().cpu()
+    assert torch.equal(out.isnan(), want.isnan())
+    assert torch.equal(out.isinf(), want.isinf()) and torch.equal(out[want.isinf()], want[want.isinf()])
+    fine = torch.isfinite(want)
+    assert fine.float().mean() > 0.3 and not fine.all()
+    assert ((out - want).abs()[fine] <= tol[fine]).all()
+    assert ((lse - wlse).abs() <= ltol).all()
+
+
 def test_many_sequences_and_a_chunk_bound_that_is_too_small(kernel):
     g = np.random.default_rng(3)
     kv = [int(x) for x in g.integers(1, 90, 700)]
