@@ -9,6 +9,17 @@ int page_shift_of(int page_size);        // paged_cache.cu
 // once, but takes longer to start.  24 sequences of up to 8192 tokens, 8 rows a token, E4M3, heads of 128: 52 / 66 / 111 us with 16 / 32 /
 // 64 rows against 98 us.
 constexpr int kSplitRows = 48;
+// ... and pairs of a block of 16 rows and a tile of 64 keys up to which it is taken whatever the rows are (counted from the sizes
+// of the call, so an upper bound).  Heads 32/8 of 128, E4M3, split-KV against tensor cores: one sequence, 64 new on 512 (1024 pairs)
+// 19 / 33 us, 128 on 512 (2048) 24 / 34, 64 on 2048 (4096) 33 / 35, 256 on 1024 (8192) 54 / 37; 64 sequences, 32 on 64 (2408) 44 / 38.
+constexpr long long kSplitPairs = 2048;
+bool few_pairs(const Args& a)
+{
+    const long long rows = static_cast<long long>(a.max_q) * a.s.group;
+    const long long blocks = a.s.seqs * ((rows + 15) / 16), most = static_cast<long long>(a.s.tokens) * a.s.group / 16 + a.s.seqs;
+    const long long tiles = ((static_cast<long long>(a.s.max_pages) << a.s.page_shift) + 63) / 64;
+    return (blocks < most ? blocks : most) * a.s.kv_heads * tiles <= kSplitPairs;
+}
 int g_impl = 0;                          // 0 by the number of rows, 1 split-KV kernel, 2 tensor-core kernel
 size_t open_bytes() { return (static_cast<size_t>(attn_split_ctas()) * sizeof(Open) + 15) / 16 * 16; }
 }
@@ -63,7 +74,7 @@ int b200q_paged_attention(const void* q, const void* k_cache, const void* v_cach
     if (a.status == nullptr) return cudaErrorInvalidDevice;
     a.open = static_cast<Open*>(workspace);
     a.part = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + open_bytes());
-    const bool chunk = g_impl != 0 ? g_impl == 2 : static_cast<long long>(a.max_q) * a.s.group > kSplitRows;
+    const bool chunk = g_impl != 0 ? g_impl == 2 : static_cast<long long>(a.max_q) * a.s.group > kSplitRows && !few_pairs(a);
     return chunk ? attn_chunk(a, head_dim, fp8 != 0, static_cast<cudaStream_t>(stream)) : attn_split(a, head_dim, fp8 != 0, static_cast<cudaStream_t>(stream));
 }
 
