@@ -5,7 +5,7 @@
 // op/test/arch_primitives/ptx_mma_fp4.cu:49-53,120-130; scale decoder op/test/arch_primitives/ptx_mma_fp6.cu:344-351).
 //
 // Many rows: the CTA-pair block-scaled kernel of gemm_nvfp4_2cta.cu instantiated for this format.
-// Few rows (decode): the product is bound by the bytes of B (K/2 + K/32 per row), so the kernel below is built to
+// Few rows (decode), or few tiles: the product is bound by the bytes of B (K/2 + K/32 per row), so the kernel below is built to
 // stream them.  It computes the transposed tile D[n, m] = sum_k B[n,k] A[m,k]: 128 rows of B fill the 128 lanes of the
 // tensor-core tile, and the rows of A (16 to 128) are its narrow side, so no MMA work is spent on rows that are not there.
 // K is split over the CTAs of a cluster so that even a square projection puts about two CTAs on every SM; the partial
@@ -257,7 +257,10 @@ int b200q_gemm_mxfp4_blocked(const void* A, const void* SFA_blocked, const void*
     if (A == nullptr || SFA_blocked == nullptr || B == nullptr || SFB_blocked == nullptr || C == nullptr) return cudaErrorInvalidValue;
     if (M <= 0 || N <= 0 || K <= 0 || K % 32 != 0) return cudaErrorInvalidValue;
     if (!aligned16(A) || !aligned16(B) || !aligned16(SFA_blocked) || !aligned16(SFB_blocked)) return cudaErrorInvalidValue;
-    if (M <= 128) return mxfp4::few_rows(A, SFA_blocked, B, SFB_blocked, C, M, N, K, stream);
+    // Up to 128 rows, and where the other kernel would have no more than eight tiles of a long K: this one splits K (160 x 512 x
+    // 16384: 8.3 us against 18.5; 256 x 1024 x 16384: 11.2 and 19.5; equal from twelve tiles on; 256 x 512 x 2048: 7.6 and 6.9).
+    const long long pair_tiles = static_cast<long long>((M + 255) / 256) * ((N + 191) / 192);
+    if (M <= 128 || (pair_tiles <= 8 && K >= 4096)) return mxfp4::few_rows(A, SFA_blocked, B, SFB_blocked, C, M, N, K, stream);
     // the width whose last wave of CTA pairs wastes less: tiles of 192 where they fit the same number of waves
     // (256 x 8192 x 8192: 14.4 us with 192 columns, 16.7 with 256; 512 x 8192 x 8192: 22.0 and 17.0)
     const long long tiles_m = (M + 255) / 256, pairs = num_sms() / 2;

@@ -769,6 +769,12 @@ __device__ __forceinline__ uint2 ld_shared_v2(uint32_t smem_addr)
     asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(smem_addr) : "memory");
     return v;
 }
+__device__ __forceinline__ uint32_t ld_shared_u16(uint32_t smem_addr)
+{
+    uint16_t v;
+    asm volatile("ld.shared.u16 %0, [%1];" : "=h"(v) : "r"(smem_addr) : "memory");
+    return v;
+}
 __device__ __forceinline__ float ld_shared_f32(uint32_t smem_addr)
 {
     float v;
