@@ -6,19 +6,22 @@ namespace b200q {
 namespace paged {
 int page_shift_of(int page_size);        // paged_cache.cu
 // Rows per kv head up to which the split-KV kernel is taken.  It reads the keys once per 16 rows, mostly from L2; the tensor-core kernel
-// once, but takes longer to start.  24 sequences of up to 8192 tokens, 8 rows a token, E4M3, heads of 128: 52 / 66 / 111 us with 16 / 32 /
-// 64 rows against 98 us.
+// once, but takes longer to start.  24 sequences of up to 8192 tokens, heads 32/4 of 64, bf16: 38 / 47 / 61 / 74 us with 16 / 32 / 48 / 64
+// rows against 53 us; heads 5/5, E4M3, 42 rows: 36 / 37; heads 8/8 of 128, E4M3, 44 rows: 40 / 41; heads 4/1, 52 rows: 46 / 52.
 constexpr int kSplitRows = 48;
 // ... and pairs of a block of 16 rows and a tile of 64 keys up to which it is taken whatever the rows are (counted from the sizes
 // of the call, so an upper bound).  Heads 32/8 of 128, E4M3, split-KV against tensor cores: one sequence, 64 new on 512 (1024 pairs)
-// 19 / 33 us, 128 on 512 (2048) 24 / 34, 64 on 2048 (4096) 33 / 35, 256 on 1024 (8192) 54 / 37; 64 sequences, 32 on 64 (2408) 44 / 38.
-constexpr long long kSplitPairs = 2048;
+// 18 / 32 us, 128 on 512 (2048) 24 / 33, 64 on 2048 (4096) 32 / 34, 256 on 1024 (8192) 52 / 37; 64 sequences, 32 on 64 (2408) 42 / 38.
+// A window bounds the tiles a block sees: one sequence, 21 new on 4587, window 429, heads 40/5 of 64, bf16: 13.1 / 23.2.
+constexpr long long kSplitPairs = 4096;
 bool few_pairs(const Args& a)
 {
-    const long long rows = static_cast<long long>(a.max_q) * a.s.group;
-    const long long blocks = a.s.seqs * ((rows + 15) / 16), most = static_cast<long long>(a.s.tokens) * a.s.group / 16 + a.s.seqs;
-    const long long tiles = ((static_cast<long long>(a.s.max_pages) << a.s.page_shift) + 63) / 64;
-    return (blocks < most ? blocks : most) * a.s.kv_heads * tiles <= kSplitPairs;
+    long long tiles = ((static_cast<long long>(a.s.max_pages) << a.s.page_shift) + 63) / 64;
+    if (a.s.window > 0) {                            // the 16 rows are at most 16 / group + 1 tokens, rounded up
+        const long long seen = (static_cast<long long>(a.s.window) + (15 + a.s.group) / a.s.group + 62) / 64 + 1;
+        tiles = seen < tiles ? seen : tiles;
+    }
+    return most_blocks(a, 16) * tiles <= kSplitPairs;
 }
 int g_impl = 0;                          // 0 by the number of rows, 1 split-KV kernel, 2 tensor-core kernel
 size_t open_bytes() { return (static_cast<size_t>(attn_split_ctas()) * sizeof(Open) + 15) / 16 * 16; }

@@ -18,6 +18,7 @@ struct Args {
     float scale_log2;                    // softmax scale * log2(e)
     int max_q;                           // the caller's bound of the chunk lengths
     int block_limit;                     // ... in row blocks (only how the work is counted depends on it)
+    int block_most;                      // bound of the call's blocks: row blocks of all sequences, times kv heads
     int zero_rest;                       // rows of no sequence: write zeros (else leave them)
     Open* open;                          // [CTAs]
     float* part;                         // [2 * CTAs][rows * D outputs, then rows x (max, sum)]
@@ -29,6 +30,14 @@ int attn_chunk(const Args& a, int head_dim, bool fp8, cudaStream_t stream);
 size_t attn_chunk_part_bytes(int head_dim);
 int attn_split_ctas();                       // the most CTAs a launch uses
 size_t attn_split_part_bytes(int head_dim);  // the most its parts take
+
+// The most row blocks of a call, over all sequences and kv heads.
+inline long long most_blocks(const Args& a, int rm)
+{
+    const long long each = (static_cast<long long>(a.max_q) * a.s.group + rm - 1) / rm;
+    const long long all = static_cast<long long>(a.s.tokens) * a.s.group / rm + a.s.seqs;
+    return (a.s.seqs * each < all ? a.s.seqs * each : all) * a.s.kv_heads;
+}
 
 // Whether the tiles of a call, however its arrays divide the rows and keys, can be counted in 32 bits.
 inline bool tiles_fit(const Args& a, int rm, int kt)

@@ -111,7 +111,7 @@ attn_chunk_kernel(const Args a)
     }
     if (warp == 12) { ptx::tmem_alloc(tmem_slot, 512); ptx::tmem_relinquish(); }
     ptx::tcgen05_fence_before_sync();
-    Cursor c = find_work(s, kRows, kTile, reinterpret_cast<int*>(smem_raw + (q_base - raw)), a.block_limit, blockIdx.x, gridDim.x);
+    Cursor c = find_work(s, kRows, kTile, reinterpret_cast<int*>(smem_raw + (q_base - raw)), a.block_limit, a.block_most, blockIdx.x, gridDim.x);
     ptx::tcgen05_fence_after_sync();
     const uint32_t tmem = *reinterpret_cast<volatile uint32_t*>(smem_raw + (tmem_slot - raw));
     Seq q{};
@@ -726,6 +726,7 @@ int launch(const Args& args, cudaStream_t stream)
     }
     if (!tiles_fit(a, kRows, kTile)) return cudaErrorInvalidValue;
     a.block_limit = static_cast<int>((static_cast<long long>(a.max_q) * a.s.group + kRows - 1) / kRows);
+    a.block_most = static_cast<int>(most_blocks(a, kRows));          // (tiles_fit bounds it)
     const int ctas = num_sms();
     kernel<<<ctas, kThreads, C::kSmemBytes, stream>>>(a);
     e = cudaGetLastError();

@@ -142,7 +142,7 @@ attn_split_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
         for (int i = 0; i < C::kStages; ++i) { ptx::mbar_init(full_bar(i), 1); ptx::mbar_init(empty_bar(i), kConsumers); }
         ptx::fence_mbar_init();
     }
-    Cursor c = find_work(s, kRows, kTile, reinterpret_cast<int*>(smem_raw + (ring - raw)), a.block_limit, blockIdx.x, gridDim.x);
+    Cursor c = find_work(s, kRows, kTile, reinterpret_cast<int*>(smem_raw + (ring - raw)), a.block_limit, a.block_most, blockIdx.x, gridDim.x);
     if (threadIdx.x == 0) a.open[blockIdx.x].last = -1;
     if (c.at == c.end) return;
     ptx::fence_proxy_async_smem();             // the ring held the prefix sums; the loads that follow are the async proxy's
@@ -574,6 +574,7 @@ int launch(const Args& args, cudaStream_t stream)
     }
     if (!tiles_fit(a, C::kRows, kTile)) return cudaErrorInvalidValue;
     a.block_limit = static_cast<int>((static_cast<long long>(a.max_q) * a.s.group + C::kRows - 1) / C::kRows);
+    a.block_most = static_cast<int>(most_blocks(a, C::kRows));          // (tiles_fit bounds it)
     const int ctas = C::kCtasPerSm * num_sms();
     kernel<<<ctas, kThreads, C::kSmemBytes, stream>>>(tmK, tmV, a);
     e = cudaGetLastError();

@@ -76,7 +76,9 @@ __device__ __forceinline__ Range block_range(const Shape& s, const Seq& q, int i
 // unnormalised output), joined by the combine kernel in CTA order.  Tile counts are 32-bit numbers: the host refuses calls whose
 // sizes could pass that, and starts that contradict one another (chunks that overlap) and pass it all the same do no work.
 // Tiles a CTA has at least: a part costs a write, a read and a turn of the combine kernel (one sequence of 1500 tokens, 8 kv heads: 13.9 us with
-// 1, 11.5 with 2, 11.3 with 3, 11.7 with 4).
+// 1, 11.5 with 2, 11.3 with 3, 11.7 with 4).  But as many CTAs as there are blocks, where the grid has them: a block costs its CTA more
+// than a tile does (one token on 36, heads 32/8 of 128: 11.4 us with three blocks a CTA, 6.5 with one; 40 sequences, up to 4 new on
+// 130: 22.5 and 17.0; tensor-core kernel, one token on 36: 24 and 11.7).
 constexpr int kMinTiles = 3;
 struct Cursor {
     int b, h, i;              // sequence, kv head, row block
@@ -93,8 +95,8 @@ __device__ __forceinline__ int add_capped(int a, int b)           // a, b in [0,
 __device__ __forceinline__ int capped(long long w) { return static_cast<int>(min(w, static_cast<long long>(kTooMany))); }
 
 // Whole CTA; `prefix` holds seqs words in shared memory (free again after the call, which ends in a barrier).
-// `block_limit`: an upper bound of the row blocks of one sequence.
-__device__ __forceinline__ Cursor find_work(const Shape& s, int rm, int kt, int* prefix, int block_limit, int cta, int ctas)
+// `block_limit`: an upper bound of the row blocks of one sequence, `block_most`: of all blocks (row blocks times kv heads).
+__device__ __forceinline__ Cursor find_work(const Shape& s, int rm, int kt, int* prefix, int block_limit, int block_most, int cta, int ctas)
 {
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
     if (block_limit <= 8) {                        // a thread per sequence
@@ -133,7 +135,7 @@ __device__ __forceinline__ Cursor find_work(const Shape& s, int rm, int kt, int*
     }
     __syncthreads();
     const int counted = s.seqs > 0 ? prefix[s.seqs - 1] : 0, total = counted == kTooMany ? 0 : counted;
-    const int used = min(ctas, (total + kMinTiles - 1) / kMinTiles);
+    const int used = min(ctas, max((total + kMinTiles - 1) / kMinTiles, min(total, block_most)));
     Cursor c{};
     if (cta < used) {
         c.share = total / used;
