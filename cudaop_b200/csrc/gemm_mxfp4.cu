@@ -257,16 +257,18 @@ int b200q_gemm_mxfp4_blocked(const void* A, const void* SFA_blocked, const void*
     if (A == nullptr || SFA_blocked == nullptr || B == nullptr || SFB_blocked == nullptr || C == nullptr) return cudaErrorInvalidValue;
     if (M <= 0 || N <= 0 || K <= 0 || K % 32 != 0) return cudaErrorInvalidValue;
     if (!aligned16(A) || !aligned16(B) || !aligned16(SFA_blocked) || !aligned16(SFB_blocked)) return cudaErrorInvalidValue;
-    // Up to 128 rows, and where the other kernel would have no more than eight tiles of a long K: this one splits K (160 x 512 x
-    // 16384: 8.3 us against 18.5; 256 x 1024 x 16384: 11.2 and 19.5; equal from twelve tiles on; 256 x 512 x 2048: 7.6 and 6.9).
-    const long long pair_tiles = static_cast<long long>((M + 255) / 256) * ((N + 191) / 192);
-    if (M <= 128 || (pair_tiles <= 8 && K >= 4096)) return mxfp4::few_rows(A, SFA_blocked, B, SFB_blocked, C, M, N, K, stream);
-    // the width whose last wave of CTA pairs wastes less: tiles of 192 where they fit the same number of waves
-    // (256 x 8192 x 8192: 14.4 us with 192 columns, 16.7 with 256; 512 x 8192 x 8192: 22.0 and 17.0)
-    const long long tiles_m = (M + 255) / 256, pairs = num_sms() / 2;
+    const long long tiles_m = (M + 255) / 256, pairs = num_sms() / 2, tiles = tiles_m * ((N + 127) / 128);
     if (pairs <= 0) return cudaErrorInvalidDevice;
+    // Up to 128 rows, and where the other kernel would have few tiles of a long K: this one splits K (256 x 1024: 7.0 us against 7.7
+    // with K = 4096, 11.3 and 17.0 with 16384; 256 x 2560, 20 tiles: 9.2 and 7.9, 15.0 and 18.9; 600 x 1000 x 2048: 8.0 and 6.5).
+    if (M <= 128 || (K >= 4096 && tiles <= (K >= 16384 ? 20 : 12)))
+        return mxfp4::few_rows(A, SFA_blocked, B, SFB_blocked, C, M, N, K, stream);
+    // Tiles of 128 columns where that leaves each CTA pair one at most (256 x 8192 x 8192: 13.0 us, 14.1 with 192, 16.3 with 256); else
+    // the width whose last wave of CTA pairs wastes less, 192 where it fits the same number of waves (512 x 8192 x 8192: 22.0 us with
+    // 192 columns, 16.5 with 256; 512 x 6568 x 15360: 22.0 and 25.2, 32.3 with 128).
     auto cost = [&](int bn) { return (tiles_m * ((N + bn - 1) / bn) + pairs - 1) / pairs * bn; };
-    return gemm_block_scaled_pair(2, A, SFA_blocked, B, SFB_blocked, C, M, N, K, 1.0f, cost(192) < cost(256) ? 192 : 256, stream);
+    const int bn = tiles <= pairs ? 128 : cost(192) < cost(256) ? 192 : 256;
+    return gemm_block_scaled_pair(2, A, SFA_blocked, B, SFB_blocked, C, M, N, K, 1.0f, bn, stream);
 }
 
 // Both MX formats share the scale layout: one UE8M0 byte per 32 K, 512-byte blocks of 128 rows x 128 K.

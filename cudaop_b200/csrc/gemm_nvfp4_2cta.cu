@@ -60,6 +60,7 @@ struct Cfg {
     static constexpr int kStoreBytes = 8 * 4096;                     // per epilogue warp one 32-row x 64-column bf16 staging buffer
     static constexpr int kStages = (227 * 1024 - 1024 - 256 - kStoreBytes) / kStageBytes > 6 ? 6 : (227 * 1024 - 1024 - 256 - kStoreBytes) / kStageBytes;
     static constexpr int kSmemBytes = kStages * kStageBytes + kStoreBytes + 1024 + 256;
+    static constexpr int kWarpCols = BN <= 128 ? 64 : 128;           // tile columns of an epilogue warp, at most
     static constexpr int kSfCols = 4 * kSfBlocks;                    // TMEM columns of one row block's scales of a stage
     static constexpr int kAccBufs = (2 * BN + kSfCols + kSfCols * kNB <= 512) ? 2 : 1;
     static constexpr int kSfaCol = kAccBufs * BN;
@@ -254,8 +255,8 @@ gemm_nvfp4_2cta_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_con
         // time: bf16 into a 128-byte-swizzled staging buffer -> one TMA store of a 32 x 64 box (full 128-byte
         // lines, clipped at the matrix edge by the tensor map).
         const int q = warp & 3;
-        const int col_begin = ((warp - 2) >> 2) * 128;                       // first tile column of this warp
-        const int nchunks = (min(BN, col_begin + 128) - col_begin) / 64;     // 2, or 1 for the last 64 of a 192-wide tile
+        const int col_begin = ((warp - 2) >> 2) * C::kWarpCols;                       // first tile column of this warp
+        const int nchunks = (min(BN, col_begin + C::kWarpCols) - col_begin) / 64;     // 2, or 1 for the last 64 of a 192-wide tile
         const bool tma_ok = ((static_cast<long long>(p.N) * 2) % 16 == 0) && aligned16(p.C);
         const uint32_t leader_tempty0 = ptx::mapa(tempty_bar(0), 0), leader_tempty1 = ptx::mapa(tempty_bar(1), 0);
         const uint32_t sbuf = store_base + static_cast<uint32_t>(warp - 2) * 4096u;
@@ -309,7 +310,8 @@ gemm_nvfp4_2cta_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_con
                 } else {
                     // Rows that do not start on 16-byte boundaries: through the same staging buffer, then a row at a time, two
                     // neighbouring columns a lane, from the first even address on (a thread writing its own row made 64
-                    // stores of 2 bytes into 32 lines each: MXFP4 300 x 1500 x 1024 took 31.3 us, 9.1 us so; 6.2 us with 1496 columns).
+                    // stores of 2 bytes into 32 lines each: MXFP4 300 x 1500 x 1024 in tiles of
+                    // 192 took 31.3 us, 9.1 us so, 6.2 us with 1496 columns; in tiles of 128 7.3 and 5.8 us).
                     const int valid = min(64, p.N - col0), rows = min(32, p.M - row0);
 #pragma unroll
                     for (int j = 0; j < 8; ++j)
@@ -408,7 +410,7 @@ int gemm_block_scaled_pair(int fmt, const void* Aq, const void* SFA_blocked, con
     if (fmt != kFmtNvfp4 && fmt != kFmtMxfp8 && fmt != kFmtMxfp4) return cudaErrorInvalidValue;
     if (M <= 0 || N <= 0 || K <= 0 || K % (fmt == kFmtNvfp4 ? 64 : 32) != 0) return cudaErrorInvalidValue;
     if (!aligned16(Aq) || !aligned16(Bq) || !aligned16(SFA_blocked) || !aligned16(SFB_blocked)) return cudaErrorInvalidValue;
-    if (bn != 192 && bn != 256) return cudaErrorInvalidValue;
+    if (bn != 192 && bn != 256 && (bn != 128 || fmt != kFmtMxfp4)) return cudaErrorInvalidValue;
     const size_t row_bytes = fmt == kFmtMxfp8 ? static_cast<size_t>(K) : static_cast<size_t>(K) / 2;
     if (row_bytes % 16 != 0) return cudaErrorInvalidValue;
     Params p{};
@@ -429,7 +431,7 @@ int gemm_block_scaled_pair(int fmt, const void* Aq, const void* SFA_blocked, con
         const uint64_t dims_a[3] = {256, k_rows, static_cast<uint64_t>((M + 127) / 128)};
         const uint64_t dims_b[3] = {256, k_rows, static_cast<uint64_t>((N + 127) / 128)};
         const uint32_t box_a[3] = {256, slab_rows, 1};
-        const uint32_t box_b[3] = {256, slab_rows, static_cast<uint32_t>(bn == 192 ? Cfg<192, 0>::kNB : Cfg<256, 0>::kNB)};
+        const uint32_t box_b[3] = {256, slab_rows, static_cast<uint32_t>(bn == 128 ? Cfg<128, 0>::kNB : bn == 192 ? Cfg<192, 0>::kNB : Cfg<256, 0>::kNB)};
         if (encode_tiled(&tmSFA, CU_TENSOR_MAP_DATA_TYPE_UINT8, 3, SFA_blocked, dims_a, strides, box_a, CU_TENSOR_MAP_SWIZZLE_NONE) != CUDA_SUCCESS)
             return cudaErrorInvalidValue;
         if (encode_tiled(&tmSFB, CU_TENSOR_MAP_DATA_TYPE_UINT8, 3, SFB_blocked, dims_b, strides, box_b, CU_TENSOR_MAP_SWIZZLE_NONE) != CUDA_SUCCESS)
@@ -450,7 +452,7 @@ int gemm_block_scaled_pair(int fmt, const void* Aq, const void* SFA_blocked, con
     if (fmt == kFmtMxfp8)
         return bn == 192 ? launch<192, kFmtMxfp8>(tmA, tmB, tmSFA, tmSFB, tmC, p, s) : launch<256, kFmtMxfp8>(tmA, tmB, tmSFA, tmSFB, tmC, p, s);
     if (fmt == kFmtMxfp4)
-        return bn == 192 ? launch<192, kFmtMxfp4>(tmA, tmB, tmSFA, tmSFB, tmC, p, s) : launch<256, kFmtMxfp4>(tmA, tmB, tmSFA, tmSFB, tmC, p, s);
+        return bn == 128 ? launch<128, kFmtMxfp4>(tmA, tmB, tmSFA, tmSFB, tmC, p, s) : bn == 192 ? launch<192, kFmtMxfp4>(tmA, tmB, tmSFA, tmSFB, tmC, p, s) : launch<256, kFmtMxfp4>(tmA, tmB, tmSFA, tmSFB, tmC, p, s);
     return bn == 192 ? launch<192, kFmtNvfp4>(tmA, tmB, tmSFA, tmSFB, tmC, p, s) : launch<256, kFmtNvfp4>(tmA, tmB, tmSFA, tmSFB, tmC, p, s);
 }
 

@@ -74,11 +74,12 @@ def dev(x):
 
 
 # few rows (1..128: the streaming kernel, K in one part and split), many rows (the pair kernel, or the streaming one in tiles of
-# 128 rows where there are few tiles); K ending inside an instruction's step, inside a scale block and inside a slab; rows of
-# the output on every alignment
+# 128 rows where there are few tiles; three tile widths, one tile a CTA pair and several); K ending inside an instruction's step,
+# inside a scale block and inside a slab; rows of the output on every alignment
 @pytest.mark.parametrize("shape", [(1, 1, 32), (1, 130, 64), (3, 300, 96), (16, 128, 2048), (17, 257, 2080), (64, 1000, 4096),
                                    (100, 129, 544), (128, 256, 8192), (129, 300, 288), (200, 72, 4128), (333, 513, 1056),
-                                   (512, 384, 512), (130, 474, 4128), (600, 129, 8192), (257, 1025, 4096), (400, 262, 96), (290, 131, 64)])
+                                   (512, 384, 512), (130, 474, 4128), (600, 129, 8192), (257, 1025, 4096), (400, 262, 96), (290, 131, 64),
+                                   (520, 3301, 96), (520, 4704, 64), (1030, 5003, 64), (1030, 10002, 32)])
 def test_product_against_64_bits(shape):
     import cudaop_b200 as ops
     M, N, K = shape
