@@ -192,7 +192,7 @@ attn_chunk_kernel(const Args a)
             // m: the base of the row's exponents.  For an E4M3 cache p is kept times kRoom / 2^v_exp, 2^v_exp a power of two above the
             // largest value scale so far: sum and output alike, so it cancels, and m - log2 of it is the base that the parts carry.
             float m = -INFINITY, l = 0.0f, poison = 0.0f;
-            uint32_t v_field = 1;
+            uint32_t v_field = kFirstValueField;
             bool fresh = true;                                                // O holds nothing of this block yet
             for (int t = 0; t < todo && ok; ++t) {
                 const uint32_t sc = scales + slot * C::kScaleBytes;

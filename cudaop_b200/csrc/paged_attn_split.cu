@@ -275,7 +275,7 @@ attn_split_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
 #pragma unroll
             for (int i = 0; i < C::kSteps; ++i) o[nt][i][0] = o[nt][i][1] = o[nt][i][2] = o[nt][i][3] = 0.0f;
         }
-        uint32_t v_field = 1;                                        // exponent field of the power of two that p * scale is divided by
+        uint32_t v_field = kFirstValueField;                                        // exponent field of the power of two that p * scale is divided by
 
         for (int t = 0; t < todo; ++t) {
             if (ok) ok = ptx::mbar_wait(full_bar(stage), phase, a.status, 2);

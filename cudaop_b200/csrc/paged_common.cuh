@@ -190,5 +190,10 @@ struct Open {
     int last;                 // CTA that does the block's last tile; -1: nothing open
 };
 
+// E4M3 cache: p * (value scale) is divided by a power of two above the largest scale seen so far, given by its exponent field.  The field
+// starts here rather than at the smallest one: with tiny or zero scales its inverse times the room that fp16 leaves (and, in the
+// tensor-core kernel, 2^that times the sum of a row) would pass 2^128.  2^-63 times the smallest p of fp16 is below any share that counts.
+constexpr uint32_t kFirstValueField = 64;
+
 }  // namespace paged
 }  // namespace b200q

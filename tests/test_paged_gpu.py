@@ -573,6 +573,46 @@ def test_a_layer_of_quantised_inference():
     assert ((whole.double() - y.double()).abs() <= 2.0 ** -7 * whole.double().abs() + 2.0 ** -12).all()
 
 
+# ------------------------------------------------------------------------------------------------------ value scales of an E4M3 cache
+class Scaled(Batch):
+    """A batch whose value scales are given, not those that the write computes: vs[b] is [tokens, kv_heads]."""
+
+    def __init__(self, vs, n, kv, **how):
+        super().__init__(n, kv, fp8=True, **how)
+        self.vs = [s.float() for s in vs]
+        for b, s in enumerate(self.vs):
+            at = torch.arange(s.shape[0])
+            slot = self.table[b][at // self.page].long() * self.page + at % self.page
+            self.cache[3][slot.cuda() // self.page, :, slot.cuda() % self.page] = s.cuda()
+
+    def held(self, b, name):
+        if name == "k":
+            return super().held(b, name)
+        q, _ = quantise_rows(self.v[b])
+        return q.view(torch.float8_e4m3fn).double() * self.vs[b].double().unsqueeze(-1)
+
+
+@pytest.mark.parametrize("dim,page", [(128, 64), (64, 16)])
+@pytest.mark.parametrize("n", [1, 30, 150])
+@pytest.mark.parametrize("s", [0.0, 2.0 ** -126, 2.0 ** -113, 2.0 ** -105])
+@pytest.mark.parametrize("behind", [0, 200])
+def test_value_scales_that_are_zero_or_tiny(kernel, behind, s, n, dim, page):
+    """A cache of zeros read before every slot is written, one quantised elsewhere, rows next to zero: whole tiles of such scales,
+    alone and with tiles of ordinary ones behind them."""
+    kv = [300, 160]
+    vs = [torch.cat([torch.full((k, 2), s), torch.rand(behind, 2, generator=torch.Generator().manual_seed(k)) + 0.01]) for k in kv]
+    b = Scaled(vs, [n, n], [k + behind for k in kv], heads=8, kv_heads=2, dim=dim, page=page)
+    got = b.call()
+    torch.cuda.synchronize()
+    assert torch.isfinite(got[0]).all()
+    out, lse = got
+    want, wlse, tol, ltol = b.expect()
+    # p * scale may round to zero where it is far below 2^-63: half a step of fp16 (2^-25) of at least 2^-74, for each key, times 448
+    tol = tol + 500 * 448 * 2.0 ** -99
+    assert ((out.double().cpu() - want).abs() <= tol).all()
+    assert ((lse.double().cpu() - wlse).abs() <= ltol).all()
+
+
 # ------------------------------------------------------------------------------------------------------ refusals
 def test_refusals():
     import cudaop_b200 as ops
