@@ -28,6 +28,17 @@ bool make_tmap_2d_u8(CUtensorMap* map, const void* gaddr, uint64_t rows, uint64_
 
 int num_sms();
 
+// Tensor memory and clusters.  A CTA that allocates tensor memory waits, without a limit, for CTAs of the same SM to free theirs.  In a
+// cluster those may in turn wait for a peer of their own that is short of tensor memory on another SM: a circle, from any two clustered
+// kernels on two streams.  So whichever of them share an SM must fit its 512 columns together, and shared memory sees to it: a
+// CTA that takes all columns asks for at least kWholeTmemSmem bytes, one that takes half of them for at least kHalfTmemSmem.  Two
+// halves fit an SM (228 KB, 1 KB of each CTA kept by the system); three halves, a half and a whole, or two wholes do not.
+// (CTAs without a cluster end by themselves; waiting for one closes no circle.)
+constexpr int kSmSmem = 228 * 1024, kSystemSmem = 1024;
+constexpr int kWholeTmemSmem = 120 * 1024, kHalfTmemSmem = 108 * 1024, kHalfTmemSmemMost = 113 * 1024;
+static_assert(2 * (kHalfTmemSmemMost + kSystemSmem) <= kSmSmem && 3 * (kHalfTmemSmem + kSystemSmem) > kSmSmem &&
+              kHalfTmemSmem + kWholeTmemSmem + 2 * kSystemSmem > kSmSmem && 2 * (kWholeTmemSmem + kSystemSmem) > kSmSmem, "who shares an SM");
+
 // Tile order of the persistent CTA-pair GEMMs: `group` tile rows walk the N tiles together, so the A rows of a group
 // stay in L2 while B streams past them once per group.  Measured (8192^3 FP8 and NVFP4, the MLP shapes): the best
 // group is the largest power of two whose A rows fit in about 60 MB of the 126 MB L2.

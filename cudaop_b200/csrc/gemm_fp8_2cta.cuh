@@ -43,6 +43,7 @@ struct PairCfg {
     static constexpr int kStoreBytes = 4 * 2 * 2048;                    // per epilogue warp two 32-row x 64-byte staging buffers
     static constexpr int kSmemBytes = kStages * kStageBytes + kStoreBytes + 1024 + 512;    // + alignment slack + barriers and tile ring
     static_assert(kStageBytes % 1024 == 0 && BN % 32 == 0, "tile shape");
+    static_assert(kSmemBytes >= kWholeTmemSmem, "who shares an SM (common.cuh)");
 };
 
 

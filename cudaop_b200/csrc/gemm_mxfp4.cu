@@ -199,16 +199,17 @@ int few_rows(const void* X, const void* SFX, const void* W, const void* SFW, voi
     int splits = 1;
     while (splits < 8 && static_cast<long long>(tiles_n) * tiles_m * splits * 2 <= 2LL * sms && p.slabs >= 4 * splits * 2) splits *= 2;
     const int per_split = (p.slabs + splits - 1) / splits;
-    const int budget = (110 * 1024 - 2048) / p.stage_bytes;
+    constexpr int kRingMost = 108 * 1024;
+    static_assert(kRingMost + 1280 <= kHalfTmemSmemMost && kTmemCols == 256, "who shares an SM");
+    const int budget = kRingMost / p.stage_bytes;
     p.stages = per_split < budget ? per_split : budget;
     if (p.stages > kMaxStages) p.stages = kMaxStages;
     if (p.stages < 1) p.stages = 1;
     // the ring doubles as the exchange buffer of the partial sums
     int ring = p.stages * p.stage_bytes;
     if (splits > 1 && ring < p.mt * kBN * 4) { p.stages = (p.mt * kBN * 4 + p.stage_bytes - 1) / p.stage_bytes; ring = p.stages * p.stage_bytes; }
-    // at least a third of an SM's shared memory: no more than two CTAs, whose tensor memory fits, become resident (a third
-    // one would wait for tensor memory inside its cluster, and clusters could wait for one another in a circle)
-    const int smem = ring + 1280 > 78 * 1024 ? ring + 1280 : 78 * 1024;
+    // enough that no more than two CTAs whose tensor memory fits become resident, of this kernel or of another clustered one (common.cuh)
+    const int smem = ring + 1280 > kHalfTmemSmem ? ring + 1280 : kHalfTmemSmem;
 
     CUtensorMap tmW, tmX, tmSFW, tmSFX;
     const uint64_t row_bytes = static_cast<uint64_t>(K) / 2;
@@ -229,7 +230,7 @@ int few_rows(const void* X, const void* SFX, const void* W, const void* SFW, voi
     cudaError_t e = cudaGetDevice(&dev);
     if (e != cudaSuccess) return e;
     if (dev >= 64 || !configured[dev]) {
-        e = cudaFuncSetAttribute(gemm_mxfp4_few_rows_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 113 * 1024);
+        e = cudaFuncSetAttribute(gemm_mxfp4_few_rows_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kHalfTmemSmemMost);
         if (e != cudaSuccess) return e;
         if (dev < 64) configured[dev] = true;
     }

@@ -65,6 +65,7 @@ struct Cfg {
     static constexpr int kAccBufs = (2 * BN + kSfCols + kSfCols * kNB <= 512) ? 2 : 1;
     static constexpr int kSfaCol = kAccBufs * BN;
     static constexpr int kSfbCol = kSfaCol + kSfCols;
+    static_assert(kSmemBytes >= kWholeTmemSmem, "who shares an SM (common.cuh)");
     static_assert(FMT != kFmtNvfp4 || kLoadBytes % 1024 == 0, "stage alignment");
 };
 

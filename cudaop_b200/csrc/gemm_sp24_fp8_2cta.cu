@@ -34,6 +34,7 @@ constexpr int kStageBytes = kABytes + 2 * kBHalfTile + kMetaBytes;      // 16 + 
 constexpr int kStoreBytes = 4 * 2 * 2048;
 constexpr int kStages = (227 * 1024 - 1024 - 256 - kStoreBytes) / kStageBytes;
 constexpr int kSmemBytes = kStages * kStageBytes + kStoreBytes + 1024 + 256;
+static_assert(kSmemBytes >= kWholeTmemSmem, "who shares an SM (common.cuh)");
 constexpr int kMetaCol = 2 * kBN;                        // metadata columns follow the two accumulators
 static_assert(kStageBytes % 1024 == 0 && kStages >= 2 && kMetaCol + 8 <= 512, "tile shape");
 

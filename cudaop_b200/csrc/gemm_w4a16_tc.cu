@@ -56,8 +56,8 @@ constexpr uint32_t kTmemCols = 512;               // 6 x 64 operand columns + 8 
 constexpr int kSmemUsed = kWStages * kWTileBytes + kASlots * kXTileBytes + kRows * kTok * 4 + kDSlots * kTok * 4 + 1024 + 256;
 // A CTA takes all 512 TMEM columns, so two CTAs must never share an SM: a second one would block in
 // tcgen05.alloc behind the first, and with clusters waiting on their peers that can close a cycle.
-// Asking for more than half of the SM's shared memory rules it out.
-constexpr int kSmemBytes = kSmemUsed > 120 * 1024 ? kSmemUsed : 120 * 1024;
+// Asking for more than half of the SM's shared memory rules it out, for this kernel and for any other clustered one (common.cuh).
+constexpr int kSmemBytes = kSmemUsed > kWholeTmemSmem ? kSmemUsed : kWholeTmemSmem;
 
 struct Params {
     const __nv_bfloat16* X;
