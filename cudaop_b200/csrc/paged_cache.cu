@@ -92,7 +92,7 @@ write_kernel(const __nv_bfloat16* __restrict__ k, const __nv_bfloat16* __restric
     }
 }
 
-// Row r of the output is token r - cu[b] of the sequence b with cu[b] <= r < cu[b + 1].  A token whose page number is outside
+// Row r of the output is token r - cu[b] of the sequence b with cu[b] <= r < cu[b + 1] (a start below zero counts as zero).  A token whose page number is outside
 // the cache reads as zero.  Rows that belong to no sequence are left as they are, or zeroed (zero_rest).
 template <int D, bool FP8>
 __global__ void __launch_bounds__(kThreads)
@@ -113,7 +113,8 @@ read_kernel(const uint8_t* __restrict__ kc, const uint8_t* __restrict__ vc, cons
         }
         long long row = zero_rest ? -1 : -2;
         if (lo < seqs && r >= __ldg(cu + lo)) {
-            const int j = r - __ldg(cu + lo), col = j >> page_shift;
+            // (0 <= j <= r whatever the array holds: r - cu[b] of a start near -2^31 would pass 32 bits and index in front of the table)
+            const int j = r - max(__ldg(cu + lo), 0), col = j >> page_shift;
             const int page = col < max_pages ? __ldg(table + static_cast<size_t>(lo) * max_pages + col) : -1;
             row = page >= 0 && page < num_pages
                       ? ((static_cast<long long>(page) * kv_heads) << page_shift) + (j & ((1 << page_shift) - 1)) : -1;

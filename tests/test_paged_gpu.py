@@ -234,6 +234,17 @@ def test_read_back(dim, page, kv_heads, fp8):
         assert torch.equal(x[:sum(kv)].cpu().float(), y[:sum(kv)].float()) and (x[sum(kv):] == 5.0).all()
 
 
+@pytest.mark.parametrize("start", [-1, -40, -2 ** 31 + 5, -2 ** 31])
+def test_read_back_with_starts_below_zero(start):
+    """A first start below zero counts as zero, as in the attention: the tokens are those from the first one on."""
+    import cudaop_b200 as ops
+    b = Batch([0, 0], [70, 30], heads=2, kv_heads=2, dim=64, page=16, fp8=True)
+    args = dict(page_table=b.table.cuda(), total=100, **names(b.cache))
+    want = ops.paged_cache_read(cu_kv=torch.tensor([0, 70, 100], dtype=torch.int32).cuda(), **args)
+    got = ops.paged_cache_read(cu_kv=torch.tensor([start, 70, 100], dtype=torch.int32).cuda(), **args)
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+
+
 # ------------------------------------------------------------------------------------------------------ attention
 @pytest.mark.parametrize("fp8", [True, False])
 @pytest.mark.parametrize("dim", [64, 128])
