@@ -30,7 +30,13 @@ namespace chunk {
 constexpr int kRows = 256, kTile = 128, kThreads = 512;
 constexpr int kScaleSlots = 4;
 constexpr int kSoftmaxRegs = 200, kLoaderRegs = 72, kMmaRegs = 40;            // 2 * 200 + 72 + 40 = 4 * 128
-constexpr float kLazy = 4.0f;                  // p is at most 2^4
+// The exponents of a tile's value scales, from smallest to largest, up to which the row's n is taken from the largest of them and of its
+// scores: it is then 2^kSpread too high at most, so an operand keeps its bits down to 2^-(25 - kSpread) of the row's largest.  A tile
+// of wider spread is walked twice, key by key.
+constexpr uint32_t kSpread = 12;
+// Power of two, either way, up to which a tile's value scales are not far from one: where all have been so, n - m is as near to 0 as
+// they are (and kLazy more), and 2^(x - n) serves for the row's sum as well.
+constexpr uint32_t kNear = 56;
 
 template <int D, bool FP8>
 struct Cfg {
@@ -41,8 +47,9 @@ struct Cfg {
     static constexpr int kStagedBytes = FP8 ? kTile * D : 0;                  // E4M3 bytes of a tile of keys or values, on their way
     static constexpr int kStaged = D == 64 ? 6 : 3;
     static constexpr int kQBytes = 2 * kSlotBytes;
-    // per tile: mask words, largest value scales, words of the keys whose value scale is not finite (4 each), key scales, value scales
-    static constexpr int kScaleAt = 48;
+    // per tile: mask words, largest and smallest exponent fields of the value scales, words of the keys whose value scale is not
+    // finite (4 each), key scales, value scales
+    static constexpr int kScaleAt = 64;
     static constexpr int kScaleBytes = kScaleAt + (FP8 ? 2 * kTile * 4 : 0);
     static constexpr int kBars = 2 * kSlots + kScaleSlots + 12;
     static constexpr int kSmemBytes = 1024 + kQBytes + kSlots * kSlotBytes + kStaged * kStagedBytes + kScaleSlots * kScaleBytes + kBars * 8 + 64 + 128 * 16;
@@ -50,12 +57,6 @@ struct Cfg {
     static_assert(kQBytes + kSlots * kSlotBytes >= 8192 * 4, "a word per sequence");
 };
 
-// p * scale / (power of two above the largest scale) is kept times kRoom = 2^11: at most 2^15, and fp16 starts to lose bits only where
-// it is below 2^-25 of the largest
-constexpr int kRoomLog2 = 11;
-// log2 of kRoom / 2^(v_field - 127)
-__device__ __forceinline__ float log2_factor(uint32_t v_field) { return static_cast<float>(kRoomLog2 + 127 - static_cast<int>(v_field)); }
-__device__ __forceinline__ float pow2_of_field(uint32_t e) { return __uint_as_float(e << 23); }
 __device__ __forceinline__ uint32_t pack_f16x2(float lo, float hi)
 {
     const __half2 v = __floats2half2_rn(lo, hi);
@@ -70,6 +71,107 @@ __device__ __forceinline__ uint32_t only_finite(uint32_t w)
 }
 // 16-byte unit `unit` of row `row` in a [rows][128 bytes] column with the 128-byte swizzle
 __device__ __forceinline__ uint32_t unit_at(uint32_t column, int row, int unit) { return column + row * 128 + ((unit ^ (row & 7)) << 4); }
+
+// Keys first .. first + 31 that the position of a row lets it see, as bits.
+__device__ __forceinline__ uint32_t visible_keys(int causal, int window, int pos, int first)
+{
+    const int last = causal ? pos - first : 31, from = window > 0 ? pos - window + 1 - first : 0;
+    const uint32_t upto = last < 0 ? 0u : last >= 31 ? 0xFFFFFFFFu : (2u << last) - 1u;
+    return from <= 0 ? upto : from > 31 ? 0u : upto & ~((1u << from) - 1u);
+}
+
+// A row's accumulators times f; the products so far are done.
+template <int D>
+__device__ __forceinline__ void rescale_output(uint32_t t_o, float f)
+{
+    ptx::tcgen05_fence_after_sync();
+#pragma unroll 1
+    for (int i = 0; i < D; i += 16) {
+        uint32_t o[16];
+        ptx::tmem_ld_32x32b_x16(t_o + i, o);
+        ptx::tmem_ld_wait();
+#pragma unroll
+        for (int k = 0; k < 16; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * f);
+        ptx::tmem_st_32x32b_x16(t_o + i, o);
+    }
+}
+
+// P of 64 keys is on its way to tensor memory: once it is there, the products over them can start.
+__device__ __forceinline__ void operands_stored(uint32_t bar)
+{
+    ptx::tmem_st_wait();
+    ptx::tcgen05_fence_before_sync();
+    __syncwarp();
+    if ((threadIdx.x & 31) == 0) ptx::mbar_arrive(bar);
+}
+
+// The softmax of a tile of an E4M3 cache whose value scales are of wide spread, or far from one: walked twice through tensor memory, 32 keys at
+// a time, with an exponential of its own for the sum and for the operand.  (A kernel without this branch takes 1178 us for the prefill chunks
+// that take 1200 with it, inside the loop or, as here, out of line.)
+struct Row {
+    float m, n, l;
+    bool ok;
+};
+template <int D>
+__device__ __noinline__ Row tile_by_key(Row row, uint32_t t_s, uint32_t t_o, uint32_t key_scales, uint32_t masks, float row_scale, int causal, int window,
+                                        int pos, int key0, bool fresh, uint32_t o_bar, uint32_t o_parity, uint32_t p_bar, uint32_t* status)
+{
+    auto scores = [&](int w, float (&x)[32]) {
+        ptx::tmem_ld_32x32b_x32(t_s + 32 * w, reinterpret_cast<uint32_t (&)[32]>(x));
+        ptx::tmem_ld_wait();
+        const uint32_t seen = __float_as_uint(ptx::ld_shared_f32(masks + 4 * w)) & visible_keys(causal, window, pos, key0 + 32 * w);
+#pragma unroll
+        for (int i = 0; i < 32; ++i) {
+            x[i] = x[i] * ptx::ld_shared_f32(key_scales + 4 * (32 * w + i)) * row_scale;
+            if (!((seen >> i) & 1u)) x[i] = -INFINITY;
+        }
+    };
+    auto value_scale = [&](int key) { return ptx::ld_shared_f32(key_scales + 4 * (kTile + key)); };
+    float mn = row.m, nn = -INFINITY;
+#pragma unroll 1
+    for (int w = 0; w < 4; ++w) {
+        float x[32];
+        scores(w, x);
+#pragma unroll
+        for (int i = 0; i < 32; ++i) {
+            mn = fmaxf(mn, x[i]);
+            nn = fmaxf(nn, x[i] + log2_above(field_of(value_scale(32 * w + i))));
+        }
+    }
+    const float om = mn == -INFINITY ? 0.0f : mn;
+    row.l *= ptx::ex2(row.m - om);
+    row.m = mn;
+    float f = 1.0f;
+    if (nn > row.n + kLazy) {
+        f = ptx::ex2(row.n - nn);
+        row.n = nn;
+    }
+    if (!fresh && __any_sync(0xffffffffu, f != 1.0f)) {
+        row.ok = __all_sync(0xffffffffu, ptx::mbar_wait(o_bar, o_parity, status, 3));
+        rescale_output<D>(t_o, f);
+    }
+    const float base = kRoomLog2 - (row.n == -INFINITY ? 0.0f : row.n);
+#pragma unroll 1
+    for (int w = 0; w < 4; ++w) {                                             // (P of 32 keys lies where the scores of 16 were)
+        float x[32];
+        uint32_t p[16];
+        scores(w, x);
+#pragma unroll
+        for (int i = 0; i < 32; i += 2) {
+            float y[2];
+#pragma unroll
+            for (int k = 0; k < 2; ++k) {
+                const float v = value_scale(32 * w + i + k);
+                row.l += ptx::ex2(x[i + k] - om);
+                y[k] = ptx::ex2(x[i + k] + (log2_above(field_of(v)) + base)) * mantissa_of(v);
+            }
+            p[i / 2] = pack_f16x2(y[0], y[1]);
+        }
+        ptx::tmem_st_32x32b_x16(t_s + 16 * w, p);
+        if (w & 1) operands_stored(p_bar + 8u * (w >> 1));
+    }
+    return row;
+}
 
 template <int D, bool FP8>
 __global__ void __launch_bounds__(kThreads, 1)
@@ -189,11 +291,10 @@ attn_chunk_kernel(const Args a)
                 if (lane == 0 && (two || h == 0)) ptx::mbar_arrive(q_bar(h));
             }
             const int pos_lo = __shfl_sync(0xffffffffu, pos, 0), pos_hi = __shfl_sync(0xffffffffu, pos, 31);
-            // m: the base of the row's exponents.  For an E4M3 cache p is kept times kRoom / 2^v_exp, 2^v_exp a power of two above the
-            // largest value scale so far: sum and output alike, so it cancels, and m - log2 of it is the base that the parts carry.
-            float m = -INFINITY, l = 0.0f, poison = 0.0f;
-            uint32_t v_field = kFirstValueField;
+            // m, n: the bases of the row's sum and of its operands (paged_common.cuh)
+            float m = -INFINITY, n = -INFINITY, l = 0.0f, poison = 0.0f;
             bool fresh = true;                                                // O holds nothing of this block yet
+            bool far = false;                                                 // some row of the warp has n far from m
             for (int t = 0; t < todo && ok; ++t) {
                 const uint32_t sc = scales + slot * C::kScaleBytes;
                 const bool mine = two || (t & 1) == h;
@@ -204,117 +305,112 @@ attn_chunk_kernel(const Args a)
                     ptx::tcgen05_fence_after_sync();
                     if (warp_on) {
                         const int key0 = (r.tile0 + c.tile + t) * kTile;
-                        float x[kTile];
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) ptx::tmem_ld_32x32b_x32(t_s + 32 * i, reinterpret_cast<uint32_t (&)[32]>(x[32 * i]));
                         const uint4 mask = ptx::ld_shared_v4(sc);
-                        float v_move = 1.0f;
-                        uint4 odd = make_uint4(0, 0, 0, 0);
-                        if (FP8) {
-                            odd = ptx::ld_shared_v4(sc + 32);
-                            const uint4 top = ptx::ld_shared_v4(sc + 16);
-                            const uint32_t f = max(max(top.x, top.y), max(top.z, top.w));
-                            // two powers of two of room, so that a slightly larger scale does not move the base again
-                            if (f > v_field) {
-                                const uint32_t to = min(f + 2, 253u);
-                                v_move = to - v_field < 127u ? pow2_of_field(127u - (to - v_field)) : 0.0f;
-                                v_field = to;
-                            }
-                        }
-                        ptx::tmem_ld_wait();
-                        if (FP8) {
-#pragma unroll
-                            for (int i = 0; i < kTile; i += 4) {
-                                const uint4 k4 = ptx::ld_shared_v4(sc + C::kScaleAt + 4 * i);
-                                const float2 u = ptx::mul2(make_float2(x[i], x[i + 1]), make_float2(__uint_as_float(k4.x), __uint_as_float(k4.y)));
-                                const float2 v = ptx::mul2(make_float2(x[i + 2], x[i + 3]), make_float2(__uint_as_float(k4.z), __uint_as_float(k4.w)));
-                                x[i] = u.x; x[i + 1] = u.y; x[i + 2] = v.x; x[i + 3] = v.y;
-                            }
-                        }
-                        // keys 32 * w .. + 31 of the tile that this row's position lets it see, as bits
-                        auto visible = [&](int w) {
-                            const int last = s.causal ? pos - key0 - 32 * w : 31, first = s.window > 0 ? pos - s.window + 1 - key0 - 32 * w : 0;
-                            const uint32_t upto = last < 0 ? 0u : last >= 31 ? 0xFFFFFFFFu : (2u << last) - 1u;
-                            return first <= 0 ? upto : first > 31 ? 0u : upto & ~((1u << first) - 1u);
-                        };
-                        const bool whole = (mask.x & mask.y & mask.z & mask.w) == 0xFFFFFFFFu && (!s.causal || key0 + kTile - 1 <= pos_lo) &&
-                                           (s.window == 0 || key0 > pos_hi - s.window);
-                        if (!whole) {
-                            const uint32_t mk[4] = {mask.x, mask.y, mask.z, mask.w};
-#pragma unroll
-                            for (int w = 0; w < 4; ++w) {
-                                const uint32_t seen = mk[w] & visible(w);
-#pragma unroll
-                                for (int i = 0; i < 32; ++i)
-                                    if (!((seen >> i) & 1u)) x[32 * w + i] = -INFINITY;
-                            }
-                        }
-                        if (FP8 && (odd.x | odd.y | odd.z | odd.w) != 0u &&
-                            ((odd.x & visible(0)) | (odd.y & visible(1)) | (odd.z & visible(2)) | (odd.w & visible(3))) != 0u)
-                            poison = __uint_as_float(0x7FC00000u);
-                        float mx[4] = {x[0], x[1], x[2], x[3]};
-#pragma unroll
-                        for (int i = 4; i < kTile - 4; i += 8)
-#pragma unroll
-                            for (int k = 0; k < 4; ++k) mx[k] = ptx::max3(mx[k], x[i + k], x[i + 4 + k]);
-#pragma unroll
-                        for (int k = 0; k < 4; ++k) mx[k] = fmaxf(mx[k], x[kTile - 4 + k]);
-                        const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * row_scale;
-                        float f = v_move;
-                        if (top > m + kLazy || m == -INFINITY) {
-                            const float mn = fmaxf(m, top);
-                            const float fm = ptx::ex2(m - (mn == -INFINITY ? 0.0f : mn));
-                            f *= fm;
-                            m = mn;
-                        }
-                        l *= f;
-                        if (!fresh && __any_sync(0xffffffffu, f != 1.0f)) {
-                            // O of the tiles so far, on the new base
+                        auto visible = [&](int w) { return visible_keys(s.causal, s.window, pos, key0 + 32 * w); };
+                        // O of the tiles so far, on a new base
+                        auto rescale = [&](float f) {
+                            if (fresh || !__any_sync(0xffffffffu, f != 1.0f)) return;
                             ok = __all_sync(0xffffffffu, ptx::mbar_wait(o_bar(h), o_phase ^ 1u, a.status, 3));
-                            ptx::tcgen05_fence_after_sync();
-#pragma unroll 1
-                            for (int i = 0; i < D; i += 16) {
-                                uint32_t o[16];
-                                ptx::tmem_ld_32x32b_x16(t_o + i, o);
-                                ptx::tmem_ld_wait();
-#pragma unroll
-                                for (int k = 0; k < 16; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * f);
-                                ptx::tmem_st_32x32b_x16(t_o + i, o);
-                            }
+                            rescale_output<D>(t_o, f);
+                        };
+                        uint32_t v_top = 0;                                   // exponent field of the largest value scale
+                        bool by_key = false;
+                        if (FP8) {
+                            const uint4 odd = ptx::ld_shared_v4(sc + 48), top4 = ptx::ld_shared_v4(sc + 16), low4 = ptx::ld_shared_v4(sc + 32);
+                            v_top = max(max(top4.x, top4.y), max(top4.z, top4.w));
+                            const uint32_t v_low = min(min(low4.x, low4.y), min(low4.z, low4.w));
+                            by_key = v_top > v_low + kSpread || v_top - (127u - kNear) > 2 * kNear || far;
+                            if ((odd.x | odd.y | odd.z | odd.w) != 0u &&
+                                ((odd.x & visible(0)) | (odd.y & visible(1)) | (odd.z & visible(2)) | (odd.w & visible(3))) != 0u)
+                                poison = __uint_as_float(0x7FC00000u);
                         }
-                        const float base = (m == -INFINITY ? 0.0f : -m) + (FP8 ? log2_factor(v_field) : 0.0f);
-                        const float2 rs2 = make_float2(row_scale, row_scale), b2 = make_float2(base, base);
-                        float2 sum[2] = {make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f)};
+                        if (FP8 && __builtin_expect(by_key, 0)) {
+                            // value scales of wide spread, or far from one
+                            const Row to = tile_by_key<D>(Row{m, n, l, ok}, t_s, t_o, sc + C::kScaleAt, sc, row_scale, s.causal, s.window, pos, key0, fresh,
+                                                          o_bar(h), o_phase ^ 1u, p_bar(h, 0), a.status);
+                            m = to.m; n = to.n; l = to.l; ok = to.ok;
+                            far = __any_sync(0xffffffffu, fabsf(n - m) > kNear + 2 * kLazy);
+                        } else {
+                            float x[kTile];
 #pragma unroll
-                        for (int g = 0; g < kTile; g += 64) {
-                            uint32_t p[32];
+                            for (int i = 0; i < 4; ++i) ptx::tmem_ld_32x32b_x32(t_s + 32 * i, reinterpret_cast<uint32_t (&)[32]>(x[32 * i]));
+                            ptx::tmem_ld_wait();
+                            if (FP8) {
 #pragma unroll
-                            for (int i = 0; i < 64; i += 4) {
-                                float2 u = ptx::fma2(make_float2(x[g + i], x[g + i + 1]), rs2, b2);
-                                float2 v = ptx::fma2(make_float2(x[g + i + 2], x[g + i + 3]), rs2, b2);
-                                u = make_float2(ptx::ex2(u.x), ptx::ex2(u.y));
-                                v = make_float2(ptx::ex2(v.x), ptx::ex2(v.y));
-                                sum[0] = ptx::add2(sum[0], u);
-                                sum[1] = ptx::add2(sum[1], v);
-                                if (FP8) {
-                                    const uint4 y = ptx::ld_shared_v4(sc + C::kScaleAt + 4 * kTile + 4 * (g + i));
-                                    u = ptx::mul2(u, make_float2(__uint_as_float(y.x), __uint_as_float(y.y)));
-                                    v = ptx::mul2(v, make_float2(__uint_as_float(y.z), __uint_as_float(y.w)));
-                                    p[i / 2] = pack_f16x2(u.x, u.y);
-                                    p[i / 2 + 1] = pack_f16x2(v.x, v.y);
-                                } else {
-                                    p[i / 2] = pack_bf16x2(u.x, u.y);
-                                    p[i / 2 + 1] = pack_bf16x2(v.x, v.y);
+                                for (int i = 0; i < kTile; i += 4) {
+                                    const uint4 k4 = ptx::ld_shared_v4(sc + C::kScaleAt + 4 * i);
+                                    const float2 u = ptx::mul2(make_float2(x[i], x[i + 1]), make_float2(__uint_as_float(k4.x), __uint_as_float(k4.y)));
+                                    const float2 v = ptx::mul2(make_float2(x[i + 2], x[i + 3]), make_float2(__uint_as_float(k4.z), __uint_as_float(k4.w)));
+                                    x[i] = u.x; x[i + 1] = u.y; x[i + 2] = v.x; x[i + 3] = v.y;
                                 }
                             }
-                            ptx::tmem_st_32x32b_x32(t_s + g / 2, p);
-                            ptx::tmem_st_wait();
-                            ptx::tcgen05_fence_before_sync();
-                            __syncwarp();
-                            if (lane == 0) ptx::mbar_arrive(p_bar(h, g / 64));      // the products over these keys can start
+                            const bool whole = (mask.x & mask.y & mask.z & mask.w) == 0xFFFFFFFFu && (!s.causal || key0 + kTile - 1 <= pos_lo) &&
+                                               (s.window == 0 || key0 > pos_hi - s.window);
+                            if (!whole) {
+                                const uint32_t mk[4] = {mask.x, mask.y, mask.z, mask.w};
+#pragma unroll
+                                for (int w = 0; w < 4; ++w) {
+                                    const uint32_t seen = mk[w] & visible(w);
+#pragma unroll
+                                    for (int i = 0; i < 32; ++i)
+                                        if (!((seen >> i) & 1u)) x[32 * w + i] = -INFINITY;
+                                }
+                            }
+                            float mx[4] = {x[0], x[1], x[2], x[3]};
+#pragma unroll
+                            for (int i = 4; i < kTile - 4; i += 8)
+#pragma unroll
+                                for (int k = 0; k < 4; ++k) mx[k] = ptx::max3(mx[k], x[i + k], x[i + 4 + k]);
+#pragma unroll
+                            for (int k = 0; k < 4; ++k) mx[k] = fmaxf(mx[k], x[kTile - 4 + k]);
+                            const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * row_scale;
+                            float f = 1.0f;
+                            if (top > m + kLazy || m == -INFINITY) {
+                                const float mn = fmaxf(m, top);
+                                f = ptx::ex2(m - (mn == -INFINITY ? 0.0f : mn));
+                                m = mn;
+                            }
+                            l *= f;
+                            if (FP8) {
+                                // (the keys' own scales are at most 2^kSpread below the largest)
+                                const float nn = top + log2_above(v_top);
+                                const bool up = nn > n + kLazy;
+                                f = up ? ptx::ex2(n - nn) : 1.0f;
+                                if (up) n = nn;
+                            }
+                            rescale(f);
+                            // E4M3: 2^kRoomLog2 2^(x - n), for the operand and, times 2^(n - m), for the sum: n - m is small in this branch
+                            const float om = m == -INFINITY ? 0.0f : m, on = n == -INFINITY ? 0.0f : n, base = FP8 ? kRoomLog2 - on : -om;
+                            const float2 rs2 = make_float2(row_scale, row_scale), b2 = make_float2(base, base);
+                            float2 sum[2] = {make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f)};
+#pragma unroll
+                            for (int g = 0; g < kTile; g += 64) {
+                                uint32_t p[32];
+#pragma unroll
+                                for (int i = 0; i < 64; i += 4) {
+                                    float2 u = ptx::fma2(make_float2(x[g + i], x[g + i + 1]), rs2, b2);
+                                    float2 v = ptx::fma2(make_float2(x[g + i + 2], x[g + i + 3]), rs2, b2);
+                                    u = make_float2(ptx::ex2(u.x), ptx::ex2(u.y));
+                                    v = make_float2(ptx::ex2(v.x), ptx::ex2(v.y));
+                                    sum[0] = ptx::add2(sum[0], u);
+                                    sum[1] = ptx::add2(sum[1], v);
+                                    if (FP8) {
+                                        const uint4 y = ptx::ld_shared_v4(sc + C::kScaleAt + 4 * kTile + 4 * (g + i));
+                                        u = ptx::mul2(u, make_float2(__uint_as_float(y.x), __uint_as_float(y.y)));
+                                        v = ptx::mul2(v, make_float2(__uint_as_float(y.z), __uint_as_float(y.w)));
+                                        p[i / 2] = pack_f16x2(u.x, u.y);
+                                        p[i / 2 + 1] = pack_f16x2(v.x, v.y);
+                                    } else {
+                                        p[i / 2] = pack_bf16x2(u.x, u.y);
+                                        p[i / 2 + 1] = pack_bf16x2(v.x, v.y);
+                                    }
+                                }
+                                ptx::tmem_st_32x32b_x32(t_s + g / 2, p);
+                                operands_stored(p_bar(h, g / 64));
+                            }
+                            sum[0] = ptx::add2(sum[0], sum[1]);
+                            l += (sum[0].x + sum[0].y) * (FP8 ? ptx::ex2(on - om - kRoomLog2) : 1.0f);
                         }
-                        sum[0] = ptx::add2(sum[0], sum[1]);
-                        l += sum[0].x + sum[0].y;
                     } else if (lane == 0) {
                         ptx::mbar_arrive(p_bar(h, 0));
                         ptx::mbar_arrive(p_bar(h, 1));
@@ -334,13 +430,13 @@ attn_chunk_kernel(const Args a)
                 ok = __all_sync(0xffffffffu, ptx::mbar_wait(o_bar(h), o_phase ^ 1u, a.status, 3));
                 ptx::tcgen05_fence_after_sync();
                 const bool begins = c.tile == 0, ends = c.tile + todo == r.tiles;
-                if (FP8) m -= log2_factor(v_field);
                 const int part = 2 * blockIdx.x + (begins ? 1 : 0);
                 float* po = a.part + static_cast<size_t>(part) * kRows * (D + 2);
                 const bool whole_block = begins && ends, joins = !two && todo > 1;
-                float f0 = 1.0f, f1 = 0.0f;
+                const float own = FP8 ? n : m;                                // what O stands on
+                float to1 = -INFINITY;                                        // ... of the odd tiles, where they are joined
                 if (joins && h == 1) {
-                    odd_state[quad * 32 + lane] = make_float4(m, l, poison, 0.0f);
+                    odd_state[quad * 32 + lane] = make_float4(m, l, poison, own);
                     ptx::tcgen05_fence_before_sync();
                     __syncwarp();
                     if (lane == 0) ptx::mbar_arrive(joined_bar);
@@ -350,16 +446,26 @@ attn_chunk_kernel(const Args a)
                     ptx::tcgen05_fence_after_sync();
                     const float4 st = odd_state[quad * 32 + lane];
                     const float mn = fmaxf(m, st.x), base = mn == -INFINITY ? 0.0f : mn;
-                    f0 = ptx::ex2(m - base);
-                    f1 = ptx::ex2(st.x - base);
-                    l = l * f0 + st.y * f1;
+                    l = l * ptx::ex2(m - base) + st.y * ptx::ex2(st.x - base);
                     m = mn;
+                    to1 = st.w;
                     poison += st.z;
                 }
                 if (joins) join_phase ^= 1u;
                 const float inv = !whole_block ? 1.0f : l == 0.0f ? 0.0f : __frcp_rn(l);
-                f0 *= inv;
-                f1 *= inv;
+                // O of this half and of the other on the common base; E4M3: in two steps, since 2^(n - m) alone may lie outside the
+                // range of the numbers
+                const float base = m == -INFINITY ? 0.0f : m;
+                float f0 = 1.0f, f1 = 0.0f, g0 = 1.0f, g1 = 0.0f;
+                if (FP8) {
+                    g0 = ptx::ex2(0.5f * (own - base));
+                    g1 = ptx::ex2(0.5f * (to1 - base));
+                    f0 = g0 * (inv * kRoomInv);
+                    f1 = g1 * (inv * kRoomInv);
+                } else {
+                    f0 = (joins ? ptx::ex2(own - base) : 1.0f) * inv;
+                    f1 = ptx::ex2(to1 - base) * inv;
+                }
                 if (warp_on && (two || h == 0)) {
                     // A thread has a row: written from here, every 16 bytes would be a line of their own.  The rows of q (whose products
                     // are done) lend the warp their place in shared memory, 256 (D = 64: 128) bytes a row, and it writes whole rows.
@@ -386,13 +492,13 @@ attn_chunk_kernel(const Args a)
                         ptx::tmem_ld_32x32b_x32(t_o + i, o);
                         ptx::tmem_ld_wait();
 #pragma unroll
-                        for (int k = 0; k < 32; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * f0 + poison);
+                        for (int k = 0; k < 32; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * (FP8 ? g0 : 1.0f) * f0 + poison);
                         if (joins) {
                             uint32_t y[32];
                             ptx::tmem_ld_32x32b_x32(t_o + D + i, y);
                             ptx::tmem_ld_wait();
 #pragma unroll
-                            for (int k = 0; k < 32; ++k) o[k] = __float_as_uint(__uint_as_float(y[k]) * f1 + __uint_as_float(o[k]));
+                            for (int k = 0; k < 32; ++k) o[k] = __float_as_uint(__uint_as_float(y[k]) * (FP8 ? g1 : 1.0f) * f1 + __uint_as_float(o[k]));
                         }
                         if (!FP8 && *static_cast<volatile int*>(odd_block + (block_no & 7)) == block_no) {
 #pragma unroll 1
@@ -526,12 +632,15 @@ attn_chunk_kernel(const Args a)
                     const uint32_t there = __ballot_sync(0xffffffffu, row >= 0);
                     const uint32_t bits = __float_as_uint(vs) & 0x7FFFFFFFu;
                     const uint32_t odd = __ballot_sync(0xffffffffu, bits >= 0x7F800000u);
-                    if (bits >= 0x7F800000u) vs = 0.0f;
-                    const uint32_t top = __reduce_max_sync(0xffffffffu, bits < 0x7F800000u ? bits : 0u);
+                    // (a scale that is not finite reaches its rows by itself; one below the smallest normal number counts as zero)
+                    const uint32_t field = bits >= 0x7F800000u ? 0u : bits >> 23;
+                    if (field == 0u) vs = 0.0f;
+                    const uint32_t top = __reduce_max_sync(0xffffffffu, field), low = __reduce_min_sync(0xffffffffu, field == 0u ? 255u : field);
                     if (lane == 0) {
                         reinterpret_cast<uint32_t*>(scp)[lw] = there;
-                        reinterpret_cast<uint32_t*>(scp)[4 + lw] = (top >> 23) + 1;
-                        reinterpret_cast<uint32_t*>(scp)[8 + lw] = odd;
+                        reinterpret_cast<uint32_t*>(scp)[4 + lw] = top;
+                        reinterpret_cast<uint32_t*>(scp)[8 + lw] = low;
+                        reinterpret_cast<uint32_t*>(scp)[12 + lw] = odd;
                     }
                     if (FP8) {
                         reinterpret_cast<float*>(scp + C::kScaleAt)[lw * 32 + lane] = ks;

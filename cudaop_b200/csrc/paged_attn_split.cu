@@ -16,13 +16,14 @@
 //
 // Precision.  An E4M3 cache is never rounded again: the bytes become fp16 exactly, a key's scale multiplies the 32-bit
 // product q.k, and a value's scale multiplies p.  The fp16 operands are kept in range by powers of two: a row of q is divided
-// by that of its largest element (an element 2^15 below it starts to lose bits that are below those of the 32-bit sum), and p * scale by that of the largest
-// scale seen so far, which is a running maximum like m.  So p keeps 11 bits.  A bf16 cache needs bf16 operands, which would leave p 8
+// by that of its largest element (an element 2^15 below it starts to lose bits that are below those of the 32-bit sum), and p * scale by that of
+// its own running maximum over the keys that the row sees (paged_common.cuh).  So it keeps 11 bits.  A bf16 cache needs bf16 operands, which would leave p 8
 // bits; it is split in two (its rounding and the rest) and the second product runs twice, which costs nothing here.
 // Sums, maxima and accumulators are 32-bit.  The work is divided over the persistent grid by tiles (paged_common.cuh).
 #include "paged_common.cuh"
 #include "paged_attn.cuh"
 #include "ptx.cuh"
+#include <cfloat>
 
 namespace b200q {
 namespace paged {
@@ -114,9 +115,6 @@ __device__ __forceinline__ uint32_t pack_f16x2(float lo, float hi)
     const __half2 v = __floats2half2_rn(lo, hi);
     return *reinterpret_cast<const uint32_t*>(&v);
 }
-// p * scale / (power of two above the largest scale) is kept times 2^15: fp16 starts to lose bits only where it is below 2^-29
-constexpr float kRoom = 32768.0f;
-__device__ __forceinline__ float pow2_of_field(uint32_t e) { return __uint_as_float(e << 23); }      // 2^(e - 127), 1 <= e <= 254
 
 template <int D, bool FP8, int NT>
 __global__ void __launch_bounds__(kThreads, NT == 1 ? 3 : 2)
@@ -267,15 +265,14 @@ attn_split_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
             if (nt == 0) pos_lo = __shfl_sync(0xffffffffu, p, 0);
             pos_hi = __shfl_sync(0xffffffffu, p, 31);
         }
-        float m[NT][2], l[NT][2], o[NT][C::kSteps][4];
+        float m[NT][2], l[NT][2], n[NT][2], o[NT][C::kSteps][4];
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
-            for (int u = 0; u < 2; ++u) { m[nt][u] = -INFINITY; l[nt][u] = 0.0f; }
+            for (int u = 0; u < 2; ++u) { m[nt][u] = -INFINITY; n[nt][u] = -FLT_MAX; l[nt][u] = 0.0f; }
 #pragma unroll
             for (int i = 0; i < C::kSteps; ++i) o[nt][i][0] = o[nt][i][1] = o[nt][i][2] = o[nt][i][3] = 0.0f;
         }
-        uint32_t v_field = kFirstValueField;                                        // exponent field of the power of two that p * scale is divided by
 
         for (int t = 0; t < todo; ++t) {
             if (ok) ok = ptx::mbar_wait(full_bar(stage), phase, a.status, 2);
@@ -315,26 +312,21 @@ attn_split_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
                 }
                 float ks[2] = {1.0f, 1.0f}, vs[2] = {1.0f, 1.0f};    // of keys g and g + 8
                 const bool there[2] = {((valid >> g) & 1u) != 0, ((valid >> (g + 8)) & 1u) != 0};
-                float v_down = 1.0f, v_move = 1.0f;
+                float ve[2] = {0.0f, 0.0f};                          // log2 of the powers of two above the value scales
                 if (FP8) {
                     const uint32_t at = kb + 2 * C::kTensorBytes + kr * 4;
                     ks[0] = ptx::ld_shared_f32(at); ks[1] = ptx::ld_shared_f32(at + 32);
-                    vs[0] = ptx::ld_shared_f32(at + C::kScaleBytes); vs[1] = ptx::ld_shared_f32(at + C::kScaleBytes + 32);
-                    // field of the smallest power of two above the largest finite scale (scales are not negative)
-                    uint32_t f = 0;
 #pragma unroll
                     for (int k = 0; k < 2; ++k) {
-                        const uint32_t bits = __float_as_uint(vs[k]) & 0x7FFFFFFFu;
-                        if (there[k] && bits < 0x7F800000u) f = max(f, bits);
+                        const float v = ptx::ld_shared_f32(at + C::kScaleBytes + 32 * k);
+                        ve[k] = log2_above(field_of(v));
+                        vs[k] = mantissa_of(v);
                     }
-                    f = min((__reduce_max_sync(0xffffffffu, f) >> 23) + 1, 253u);
-                    if (f > v_field) { v_move = f - v_field < 127u ? pow2_of_field(127u - (f - v_field)) : 0.0f; v_field = f; }
-                    v_down = pow2_of_field(254u - v_field) * kRoom;
                 }
                 // keys that are not there for the whole block, that come after a row, or that have left its window
                 const bool whole = valid == 0xFFFFu && (!s.causal || key0 + 15 <= pos_lo) && (s.window == 0 || key0 > pos_hi - s.window);
                 uint32_t pb[NT][2], pl[NT][2];
-                bool moved = FP8 && v_move != 1.0f;
+                bool moved = false;
                 float f[NT][2];
 #pragma unroll
                 for (int nt = 0; nt < NT; ++nt) {
@@ -357,20 +349,19 @@ attn_split_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
                         mn = ptx::max_nan(mn, m[nt][u]);
                         const float base = mn == -INFINITY ? 0.0f : mn;      // a row that has seen nothing yet
                         const float fm = ptx::ex2(m[nt][u] - base);
-                        f[nt][u] = fm * v_move;
-                        moved |= mn != m[nt][u];
+                        f[nt][u] = fm;
+                        moved |= !FP8 && mn != m[nt][u];
                         p[u] = ptx::ex2(x[nt][u] - base);
                         p[2 + u] = ptx::ex2(x[nt][2 + u] - base);
                         l[nt][u] = l[nt][u] * fm + (p[u] + p[2 + u]);
                         m[nt][u] = mn;
+                        if (FP8) {                                   // from here on x + e
+                            x[nt][u] += ve[0];
+                            x[nt][2 + u] += ve[1];
+                            moved |= fmaxf(x[nt][u], x[nt][2 + u]) > n[nt][u] + kLazy;
+                        }
                     }
-                    if (FP8) {
-                        // a masked key's p is 0: its product with a scale that is not finite must be 0 as well
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) p[i] = !whole && p[i] == 0.0f ? 0.0f : p[i] * (vs[i >> 1] * v_down);
-                        pb[nt][0] = ptx::movmatrix_trans(pack_f16x2(p[0], p[1]));
-                        pb[nt][1] = ptx::movmatrix_trans(pack_f16x2(p[2], p[3]));
-                    } else {
+                    if (!FP8) {
 #pragma unroll
                         for (int k = 0; k < 2; ++k) {
                             const uint32_t hi = pack_bf16x2(p[2 * k], p[2 * k + 1]);
@@ -380,10 +371,37 @@ attn_split_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
                     }
                 }
                 if (__any_sync(0xffffffffu, moved)) {
+                    if (FP8) {
+#pragma unroll
+                        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                            for (int u = 0; u < 2; ++u) {
+                                float nn = fmaxf(x[nt][u], x[nt][2 + u]);
+#pragma unroll
+                                for (int w = 4; w <= 16; w <<= 1) nn = fmaxf(nn, __shfl_xor_sync(0xffffffffu, nn, w));
+                                nn = fmaxf(nn, n[nt][u]);
+                                f[nt][u] = nn == n[nt][u] ? 1.0f : ptx::ex2(n[nt][u] - nn);
+                                n[nt][u] = nn;
+                            }
+                    }
 #pragma unroll
                     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
                         for (int i = 0; i < C::kSteps; ++i) { o[nt][i][0] *= f[nt][0]; o[nt][i][1] *= f[nt][1]; o[nt][i][2] *= f[nt][0]; o[nt][i][3] *= f[nt][1]; }
+                }
+                if (FP8) {
+#pragma unroll
+                    for (int nt = 0; nt < NT; ++nt) {
+                        float p[4];
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            p[i] = ptx::ex2(x[nt][i] + (kRoomLog2 - n[nt][i & 1])) * vs[i >> 1];
+                            // a key that the row does not see: its scale may be anything
+                            if (!whole && x[nt][i] == -INFINITY) p[i] = 0.0f;
+                        }
+                        pb[nt][0] = ptx::movmatrix_trans(pack_f16x2(p[0], p[1]));
+                        pb[nt][1] = ptx::movmatrix_trans(pack_f16x2(p[2], p[3]));
+                    }
                 }
                 // values: columns of chunk g in rows 2cc, 2cc + 1, 2cc + 8, 2cc + 9; what is not there counts as zero, whatever it is
                 const int vr = warp * 16 + 2 * cc;
@@ -465,7 +483,6 @@ attn_split_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
                 if (g == 0) state_p[warp * kRows + 8 * nt + 2 * cc + u] = make_float2(m[nt][u], l[nt][u]);
             }
         ptx::named_barrier(1, 32 * kConsumers);
-        const float v_up = FP8 ? pow2_of_field(v_field) * (1.0f / kRoom) : 1.0f;
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -477,9 +494,13 @@ attn_split_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
                 const float base = mm == -INFINITY ? 0.0f : mm;
 #pragma unroll
                 for (int w = 0; w < kConsumers; ++w) ll += st[w].y * ptx::ex2(st[w].x - base);
-                const float fw = ptx::ex2(m[nt][u] - base) * v_up;
+                // E4M3: from the units of n, in two steps, since 2^(n - base) alone may lie outside the range of the numbers
+                const float fw = FP8 ? ptx::ex2(0.5f * (n[nt][u] - base)) : ptx::ex2(m[nt][u] - base), fw2 = fw * kRoomInv;
 #pragma unroll
-                for (int i = 0; i < C::kSteps; ++i) { o[nt][i][u] *= fw; o[nt][i][2 + u] *= fw; }
+                for (int i = 0; i < C::kSteps; ++i) {
+                    o[nt][i][u] *= fw; o[nt][i][2 + u] *= fw;
+                    if (FP8) { o[nt][i][u] *= fw2; o[nt][i][2 + u] *= fw2; }
+                }
                 m[nt][u] = mm;
                 l[nt][u] = ll;
             }

@@ -190,10 +190,24 @@ struct Open {
     int last;                 // CTA that does the block's last tile; -1: nothing open
 };
 
-// E4M3 cache: p * (value scale) is divided by a power of two above the largest scale seen so far, given by its exponent field.  The field
-// starts here rather than at the smallest one: with tiny or zero scales its inverse times the room that fp16 leaves (and, in the
-// tensor-core kernel, 2^that times the sum of a row) would pass 2^128.  2^-63 times the smallest p of fp16 is below any share that counts.
-constexpr uint32_t kFirstValueField = 64;
+// E4M3 cache: the second product takes p_j s_j (s_j the scale of value j) in fp16.  Each row keeps two running maxima, both in units of
+// log2: m of its scores x_j, on which its sum of 2^(x_j - m) stands, and n of x_j + e_j with 2^e_j the power of two above s_j, on which
+// its operands and its accumulators stand: the product's operand is 2^(x_j - n) s_j 2^kRoomLog2.  So what fp16 keeps depends on what the row itself uses
+// of its values, not on the scales of keys that it does not see, has left behind or gives no weight.  n is raised only when
+// it grows by more than kLazy, so an operand is below 2^(kRoomLog2 + kLazy) = 2^15; it loses bits where it is below 2^-14, that is
+// 2^-25 of n's key.  Scales below the smallest normal number (the write makes none) count as zero.
+constexpr int kRoomLog2 = 11;
+constexpr float kRoomInv = 1.0f / 2048.0f;
+constexpr float kLazy = 4.0f;
+__device__ __forceinline__ float pow2_of_field(uint32_t e) { return __uint_as_float(e << 23); }      // 2^(e - 127), 1 <= e <= 254
+__device__ __forceinline__ uint32_t field_of(float x) { return (__float_as_uint(x) >> 23) & 255u; }
+__device__ __forceinline__ float log2_above(uint32_t field) { return static_cast<float>(static_cast<int>(field) - 126); }   // e_j
+// s / 2^e_j: 0.5 to 1 in magnitude, 0 for a zero; infinities and NaN as they are
+__device__ __forceinline__ float mantissa_of(float s)
+{
+    const uint32_t b = __float_as_uint(s), f = field_of(s);
+    return f == 255u ? s : f == 0u ? 0.0f : __uint_as_float((b & 0x807FFFFFu) | 0x3F000000u);
+}
 
 }  // namespace paged
 }  // namespace b200q

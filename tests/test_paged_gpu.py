@@ -624,6 +624,113 @@ def test_value_scales_that_are_zero_or_tiny(kernel, behind, s, n, dim, page):
     assert ((lse.double().cpu() - wlse).abs() <= ltol).all()
 
 
+def shares(b, causal=True, window=0):
+    """Per sequence, from the definition in 64 bits: the weights [heads, n, keys] of the softmax."""
+    group = b.heads // b.kv_heads
+    for s, (n, kv) in enumerate(zip(b.n, b.kv)):
+        q, k = b.q[int(b.cu[s]):int(b.cu[s]) + n].double(), b.held(s, "k").repeat_interleave(group, 1)
+        p, j = torch.arange(n).unsqueeze(1) + kv - n, torch.arange(kv).unsqueeze(0)
+        seen = (j <= p) | (not causal)
+        if window:
+            seen &= j > p - window
+        x = torch.einsum("nhd,khd->hnk", q, k) * b.dim ** -0.5
+        yield s, torch.softmax(torch.where(seen, x, torch.full_like(x, -math.inf)), 2)
+
+
+def check_scaled(b, **how):
+    """Against 64 bits, with a bound made of what each row itself uses: the share of p |v| that it sees, and the loss of fp16."""
+    import cudaop_b200 as ops
+    out, lse = b.call(**how)
+    torch.cuda.synchronize()
+    assert ops.status() == 0
+    want, wlse, tol, ltol = b.expect(**how)
+    # p * scale is held in fp16 times 2^11 / 2^n: half a step of its small numbers, 2^-25, is 2^-36 2^n for each key; 2^n is at most
+    # 2^13 times the largest p * scale that the row sees (2^12 of spread, and up to 2 from the scale to the power of two above it).
+    # The tensor-core kernel may hold a first part on a base that is 2^4 below.
+    extra = []
+    for s, w in shares(b, **how):
+        vs = b.vs[s].double().repeat_interleave(b.heads // b.kv_heads, 1)
+        top = (w * vs.t().unsqueeze(1)).amax(2)                      # [heads, n]
+        codes = quantise_rows(b.v[s])[0].view(torch.float8_e4m3fn).double().abs().sum(0).repeat_interleave(b.heads // b.kv_heads, 0)
+        extra.append(2.0 ** -23 * top.t().unsqueeze(2) * codes)
+    tol = (tol - 1e-30) + torch.cat(extra) + 2.0 ** -133             # (... and half a step of bf16's smallest numbers)
+    err = (out.double().cpu() - want).abs()
+    assert (err <= tol).all(), f"out: {(err / tol).max():.3f} of the bound"
+    assert ((lse.double().cpu() - wlse).abs() <= ltol).all()
+
+
+@pytest.mark.parametrize("dim,page", [(128, 64), (64, 16)])
+@pytest.mark.parametrize("n", [1, 30, 150])
+@pytest.mark.parametrize("s", [2.0 ** -126, 2.0 ** -113, 2.0 ** -70, 2.0 ** 100])
+def test_value_scales_far_from_one_keep_their_bits(kernel, s, n, dim, page):
+    """All scales near the same power of two: relative errors are those of ordinary ones."""
+    g = torch.Generator().manual_seed(n)
+    check_scaled(Scaled([s * (1 + torch.rand(k, 2, generator=g)) for k in (300, 160)], [n, n], [300, 160], heads=8, kv_heads=2, dim=dim, page=page))
+
+
+@pytest.mark.parametrize("dim,page", [(128, 64), (64, 16)])
+@pytest.mark.parametrize("n", [1, 30, 150])
+@pytest.mark.parametrize("how", ["keys", "tiles", "tiles, down", "zeros between"])
+def test_value_scales_of_wide_spread(kernel, how, n, dim, page):
+    """Scales from 2^-40 to 2^40 key by key, and from 2^-126 to 2^60 and back tile by tile."""
+    g = torch.Generator().manual_seed(n)
+    kv = [600, 400]
+    vs = []
+    for k in kv:
+        if how == "keys":
+            s = torch.exp2(torch.randint(-40, 41, (k, 2), generator=g).float())
+        elif how == "zeros between":
+            s = torch.rand(k, 2, generator=g) * (torch.rand(k, 2, generator=g) < 0.5)
+        else:
+            e = torch.tensor([-126.0, 0.0, 60.0, -50.0, 3.0])[torch.arange(k) // 128]
+            s = torch.exp2(e.flip(0) if how == "tiles, down" else e).unsqueeze(1).repeat(1, 2)
+        vs.append(s)
+    check_scaled(Scaled(vs, [n, n], kv, heads=8, kv_heads=2, dim=dim, page=page))
+
+
+@pytest.mark.parametrize("dim,page", [(128, 64), (64, 16)])
+@pytest.mark.parametrize("n,window", [(8, 0), (8, 40), (150, 0), (150, 100), (300, 130)])
+@pytest.mark.parametrize("up", [45, 100])
+def test_a_huge_value_reaches_the_rows_that_see_it_alone(kernel, up, n, window, dim, page):
+    """One finite token whose value scale is 2^45 (2^100) times the others': rows in front of it, and rows whose window it has
+    left, are as exact as without it; so are rows that give it next to no weight."""
+    kv = 400
+    vs = torch.rand(kv, 2, generator=torch.Generator().manual_seed(n)) + 0.5
+    vs[kv - n // 2, 0] *= 2.0 ** up                                  # new itself: hidden from the first half of the rows
+    vs[kv - n - 5, 1] *= 2.0 ** up                                   # with a window of 100 or 130: seen by the first rows only
+    check_scaled(Scaled([vs], [n], [kv], heads=8, kv_heads=2, dim=dim, page=page), window=window)
+
+
+@pytest.mark.parametrize("dim,page", [(128, 64), (64, 16)])
+@pytest.mark.parametrize("n", [1, 30, 150])
+def test_a_huge_value_of_next_to_no_weight(kernel, n, dim, page):
+    import cudaop_b200 as ops
+    kv, at = 400, 200
+    vs = torch.rand(kv, 2, generator=torch.Generator().manual_seed(n)) + 0.5
+    vs[at] *= 2.0 ** 45
+    b = Scaled([vs], [n], [kv], heads=8, kv_heads=2, dim=dim, page=page)
+    b.q = b.q.abs()
+    b.k[0][at] = -64.0 * dim ** -0.5                                 # scores near -50 for every row: a weight near 2^-75, times 2^45
+    slot = int(b.table[0, at // page]) * page + at % page
+    ops.paged_cache_write(b.k[0][at:at + 1].cuda(), b.v[0][at:at + 1].cuda(), torch.tensor([slot]).cuda(), **names(b.cache))
+    b.cache[3][slot // page, :, slot % page] = vs[at].cuda()
+    check_scaled(b)
+
+
+def test_a_nan_scale_of_a_key_reaches_the_rows_that_see_it(kernel):
+    """NaN in a key's scale: rows that see the token are NaN, lse included, rows in front of it as if it were not there."""
+    for n, at in ((8, 60), (150, 100)):
+        b = Batch([n], [at + 4 if n == 8 else 170], 4, 1, 128, 16, True)
+        kv = b.kv[0]
+        b.cache[2][int(b.table[0, at // 16]), :, at % 16] = NAN
+        out, lse = b.call()
+        front = at - (kv - n)
+        assert out[front:].isnan().all() and lse[front:].isnan().all()
+        want, wlse, tol, ltol = b.expect()
+        assert ((out[:front].double().cpu() - want[:front]).abs() <= tol[:front]).all()
+        assert ((lse[:front].double().cpu() - wlse[:front]).abs() <= ltol[:front]).all()
+
+
 # ------------------------------------------------------------------------------------------------------ refusals
 def test_refusals():
     import cudaop_b200 as ops
