@@ -9,7 +9,6 @@
 #include <torch/extension.h>
 
 #include <ATen/cuda/CUDAContext.h>
-#include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDAException.h>
 #include <c10/cuda/CUDAGuard.h>
 
@@ -64,7 +63,7 @@ constexpr auto kI32 = c10::ScalarType::Int;
 
 torch::Tensor out_like(const torch::Tensor& ref, std::vector<int64_t> shape, c10::ScalarType dt)
 {
-    return at::detail::empty_cuda(shape, dt, ref.device(), c10::nullopt);     // torch::empty without the dispatcher's way there
+    return torch::empty(shape, ref.options().dtype(dt));
 }
 
 }  // namespace

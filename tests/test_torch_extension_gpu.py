@@ -96,3 +96,34 @@ def test_launches_on_the_current_stream():
     side.synchronize()
     assert torch.equal(got, want)
     torch.cuda.synchronize()
+
+
+def test_outputs_are_allocated_where_dispatch_modes_see_it():
+    """A mode that watches torch's allocations sees those of the operators, and one that has memory filled fills them."""
+    import cudaop_b200 as ops
+    from torch.utils._python_dispatch import TorchDispatchMode
+
+    class Watch(TorchDispatchMode):
+        def __init__(self):
+            super().__init__()
+            self.empty = []
+
+        def __torch_dispatch__(self, func, types, args=(), kwargs=None):
+            out = func(*args, **(kwargs or {}))
+            if "empty" in str(func):
+                self.empty.append((tuple(out.shape), out.dtype))
+            return out
+
+    a = torch.zeros((16, 64), dtype=torch.uint8, device="cuda")
+    x = torch.zeros((4, 64), dtype=torch.bfloat16, device="cuda")
+    cache = torch.zeros((3, 2, 16, 64), dtype=torch.bfloat16, device="cuda")
+    ints = [torch.tensor(t, dtype=torch.int32, device="cuda") for t in ([[0, 2]], [0, 1], [20])]
+    with Watch() as seen:
+        ops.gemm_fp8(a, a, 1.0, 1.0)
+        ops.quant_rows_e4m3(x)
+        ops.quant_rows_mxfp4(x)
+        ops.paged_attention(x.view(1, 4, 64), cache, cache, *ints, 1)
+    for want in (((16, 16), torch.bfloat16), ((4,), torch.float32), ((4, 32), torch.uint8), ((1, 4, 64), torch.bfloat16)):
+        assert want in seen.empty, (want, seen.empty)
+    torch.cuda.synchronize()
+    assert ops.status() == 0
