@@ -365,6 +365,12 @@ void check_index(const torch::Tensor& t, const char* name, c10::ScalarType dt, i
     same_place(kc, t, name);
 }
 
+// A table without columns has no page for any token, as one whose page numbers are all -1.
+torch::Tensor with_a_column(const torch::Tensor& page_table)
+{
+    return page_table.size(1) > 0 ? page_table : torch::full({page_table.size(0), 1}, -1, page_table.options());
+}
+
 void paged_cache_write(torch::Tensor k, torch::Tensor v, torch::Tensor slots, torch::Tensor k_cache, torch::Tensor v_cache,
                        c10::optional<torch::Tensor> k_scale, c10::optional<torch::Tensor> v_scale)
 {
@@ -407,10 +413,11 @@ std::tuple<torch::Tensor, torch::Tensor> paged_cache_read(torch::Tensor k_cache,
         v = out_like(k_cache, {total, c.kv_heads, c.dim}, kBF16);
     }
     if (total == 0) return {k, v};
-    if (seqs == 0 || page_table.size(1) == 0) {                    // no token has a page
-        if (!k_out.has_value() || seqs > 0) { k.zero_(); v.zero_(); }
+    if (seqs == 0) {                                               // every row is one of no sequence
+        if (!k_out.has_value()) { k.zero_(); v.zero_(); }
         return {k, v};
     }
+    page_table = with_a_column(page_table);
     raise_on(b200q_paged_cache_read(k_cache.data_ptr(), v_cache.data_ptr(), c.ks, c.vs, page_table.data_ptr<int>(), cu_kv.data_ptr<int>(),
                                     k.data_ptr(), v.data_ptr(), (int)seqs, (int)total, c.kv_heads, c.dim, (int)page_table.size(1), c.pages, c.page,
                                     c.fp8, !k_out.has_value(), stream_of(k_cache)), "b200q_paged_cache_read");
@@ -429,7 +436,6 @@ std::tuple<torch::Tensor, c10::optional<torch::Tensor>> paged_attention(
     check_index(page_table, "page_table", kI32, 2, k_cache); check_index(cu_q, "cu_q", kI32, 1, k_cache);
     check_index(kv_lens, "kv_lens", kI32, 1, k_cache);
     TORCH_CHECK_VALUE(page_table.size(0) == seqs && cu_q.numel() == seqs + 1, "page_table, cu_q and kv_lens must agree on the number of sequences");
-    TORCH_CHECK_VALUE(seqs > 0 && page_table.size(1) > 0, "there must be a sequence and a page");
     TORCH_CHECK_VALUE(seqs <= 8192, "at most 8192 sequences, got ", num(seqs));
     TORCH_CHECK_VALUE(max_q > 0, "max_q must be positive");
     TORCH_CHECK_VALUE(window >= 0 && (window == 0 || causal), "window must not be negative, and needs causal");
@@ -450,6 +456,12 @@ std::tuple<torch::Tensor, c10::optional<torch::Tensor>> paged_attention(
     c10::optional<torch::Tensor> lse;
     if (return_lse) lse = given ? torch::full({tokens, heads}, -INFINITY, k_cache.options().dtype(kF32)) : out_like(k_cache, {tokens, heads}, kF32);
     if (tokens == 0) return {o, lse};
+    if (seqs == 0) {                                               // every row is one of no sequence
+        if (!given) o.zero_();
+        if (return_lse) lse->fill_(-INFINITY);
+        return {o, lse};
+    }
+    page_table = with_a_column(page_table);
     auto ws = out_like(k_cache, {(int64_t)b200q_paged_attention_workspace_bytes(c.dim)}, kU8);
     raise_on(b200q_paged_attention(q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), c.ks, c.vs, page_table.data_ptr<int>(),
                                    cu_q.data_ptr<int>(), kv_lens.data_ptr<int>(), o.data_ptr(), lse.has_value() ? lse->data_ptr<float>() : nullptr,

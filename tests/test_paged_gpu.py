@@ -731,6 +731,44 @@ def test_a_nan_scale_of_a_key_reaches_the_rows_that_see_it(kernel):
         assert ((lse[:front].double().cpu() - wlse[:front]).abs() <= ltol[:front]).all()
 
 
+# ------------------------------------------------------------------------------------------------------ nothing to attend to
+def test_no_sequences_and_tables_without_columns():
+    """An empty batch is not an error, for the attention as for the read-back: every row is one of no sequence.  With a table
+    without columns the sequences' rows see nothing, and only the rows of no sequence stay as they are in what is given."""
+    import cudaop_b200 as ops
+    cache = names(empty_cache(3, 2, 16, 64, True))
+
+    def ints(*x, shape=None):
+        return torch.tensor(x, dtype=torch.int32, device="cuda").view(shape or (len(x),))
+    q = torch.ones(5, 4, 64, dtype=torch.bfloat16, device="cuda")
+    for table in (ints(shape=(0, 0)), ints(shape=(0, 3))):
+        out, lse = ops.paged_attention(q, page_table=table, cu_q=ints(0), kv_lens=ints(), max_q=1, return_lse=True, **cache)
+        assert out.shape == q.shape and (out == 0).all() and lse.shape == (5, 4) and (lse == -math.inf).all()
+        given = torch.full_like(q, 3.0)
+        out, lse = ops.paged_attention(q, page_table=table, cu_q=ints(0), kv_lens=ints(), max_q=1, return_lse=True, out=given, **cache)
+        assert (given == 3.0).all() and (lse == -math.inf).all()
+        assert ops.paged_attention(q[:0], page_table=table, cu_q=ints(0), kv_lens=ints(), max_q=1, **cache).shape == (0, 4, 64)
+        k, v = ops.paged_cache_read(page_table=table, cu_kv=ints(0), total=4, **cache)
+        assert k.shape == (4, 2, 64) and (k == 0).all() and (v == 0).all()
+        kv = [torch.full((4, 2, 64), 3.0, dtype=torch.bfloat16, device="cuda") for _ in range(2)]
+        ops.paged_cache_read(page_table=table, cu_kv=ints(0), total=4, k_out=kv[0], v_out=kv[1], **cache)
+        assert (kv[0] == 3.0).all() and (kv[1] == 3.0).all()
+    table = ints(shape=(2, 0))
+    given = torch.full_like(q, 3.0)
+    out, lse = ops.paged_attention(q, page_table=table, cu_q=ints(0, 1, 3), kv_lens=ints(1, 7), max_q=2, return_lse=True, out=given, **cache)
+    assert (given[:3] == 0).all() and (given[3:] == 3.0).all() and (lse == -math.inf).all()
+    out, lse = ops.paged_attention(q, page_table=table, cu_q=ints(0, 1, 3), kv_lens=ints(1, 7), max_q=2, return_lse=True, **cache)
+    assert (out == 0).all() and (lse == -math.inf).all()
+    kv = [torch.full((4, 2, 64), 3.0, dtype=torch.bfloat16, device="cuda") for _ in range(2)]
+    ops.paged_cache_read(page_table=table, cu_kv=ints(0, 1, 3), total=4, k_out=kv[0], v_out=kv[1], **cache)
+    for t in kv:
+        assert (t[:3] == 0).all() and (t[3:] == 3.0).all()
+    k, v = ops.paged_cache_read(page_table=table, cu_kv=ints(0, 1, 3), total=4, **cache)
+    assert (k == 0).all() and (v == 0).all()
+    torch.cuda.synchronize()
+    assert ops.status() == 0
+
+
 # ------------------------------------------------------------------------------------------------------ refusals
 def test_refusals():
     import cudaop_b200 as ops
