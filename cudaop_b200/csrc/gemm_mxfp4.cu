@@ -262,7 +262,9 @@ int b200q_gemm_mxfp4_blocked(const void* A, const void* SFA_blocked, const void*
     if (pairs <= 0) return cudaErrorInvalidDevice;
     // Up to 128 rows, and where the other kernel would have few tiles of a long K: this one splits K (256 x 1024: 7.0 us against 7.7
     // with K = 4096, 11.3 and 17.0 with 16384; 256 x 2560, 20 tiles: 9.2 and 7.9, 15.0 and 18.9; 600 x 1000 x 2048: 8.0 and 6.5).
-    if (M <= 128 || (K >= 4096 && tiles <= (K >= 16384 ? 20 : 12)))
+    // Its grid has a row of clusters per 128 columns, which ends at 65535; the other kernel is persistent.
+    constexpr int kMostN = 65535 * mxfp4::kBN;
+    if ((M <= 128 && N <= kMostN) || (K >= 4096 && tiles <= (K >= 16384 ? 20 : 12)))
         return mxfp4::few_rows(A, SFA_blocked, B, SFB_blocked, C, M, N, K, stream);
     // Tiles of 128 columns where that leaves each CTA pair one at most (256 x 8192 x 8192: 13.0 us, 14.1 with 192, 16.3 with 256); else
     // the width whose last wave of CTA pairs wastes less, 192 where it fits the same number of waves (512 x 8192 x 8192: 22.0 us with

@@ -206,6 +206,28 @@ def test_weights_quantised_right_before_their_product():
         check_product(out, ca, sa, cb, sb)
 
 
+@pytest.mark.parametrize("M", [3, 128])
+def test_more_columns_than_a_grid_has_rows_of_clusters(M):
+    """N beyond 65535 tiles of 128 columns, with few rows of A."""
+    import cudaop_b200 as ops
+    N, K = 65535 * 128 + 200, 32
+    g = torch.Generator(device="cuda").manual_seed(M)
+    a, sa, _, _ = case(M, 1, K, M)
+    bq = torch.randint(0, 256, (N, K // 2), generator=g, dtype=torch.uint8, device="cuda")
+    sb = torch.randint(121, 134, (N, 1), generator=g, dtype=torch.uint8, device="cuda")
+    out = ops.gemm_mxfp4(dev(pack(a)), dev(sa), bq, sb)
+    va = torch.from_numpy(values(a, sa)).cuda()
+    grid = torch.from_numpy(np.concatenate([GRID, -GRID])).cuda()
+    worst = 0.0
+    for n0 in range(0, N, 1 << 20):
+        codes = torch.stack((bq[n0:n0 + (1 << 20)] & 15, bq[n0:n0 + (1 << 20)] >> 4), 2).flatten(1).int()
+        vb = grid[codes] * torch.exp2(sb[n0:n0 + (1 << 20)].double() - 127)
+        want = va @ vb.T
+        bound = 2.0 ** -8 * want.abs() + 3 * 2.0 ** -22 * (va.abs() @ vb.abs().T) + 1e-300
+        worst = max(worst, float(((out[:, n0:n0 + (1 << 20)].double() - want).abs() / bound).max()))
+    assert ops.status() == 0 and worst <= 1.0, worst
+
+
 def test_refusals():
     import cudaop_b200 as ops
     a = torch.zeros((128, 48), dtype=torch.uint8, device="cuda")
