@@ -284,7 +284,8 @@ attn_chunk_kernel(const Args a)
                     }
                     if (two || h == 0) ptx::st_shared_v4(unit_at(q_base + h * C::kSlotBytes + (piece >> 3) * C::kHalfBytes, quad * 32 + rr, piece & 7), v[0], v[1], v[2], v[3]);
                 }
-                if (FP8) row_scale *= pow2_of_field(my_e);
+                // (not zero, which would make a hidden key's -infinity NaN: tiny rows times a tiny softmax scale)
+                if (FP8) row_scale = fmaxf(row_scale * pow2_of_field(my_e), __uint_as_float(1u));
                 ptx::fence_proxy_async_smem();
                 if (threadIdx.x == 0) { block_info[0] = todo; block_info[1] = two ? 2 : 1; }
                 __syncwarp();

@@ -731,6 +731,16 @@ def test_a_nan_scale_of_a_key_reaches_the_rows_that_see_it(kernel):
         assert ((lse[:front].double().cpu() - wlse[:front]).abs() <= ltol[:front]).all()
 
 
+@pytest.mark.parametrize("dim,fp8", [(128, True), (64, True), (128, False)])
+@pytest.mark.parametrize("scale", [1e-6, 1e-8, -1e-12, 1e-30, 1e-38])
+def test_rows_of_zeros_and_next_to_zero_with_a_small_scale(kernel, scale, dim, fp8):
+    """The power of two of a row times the softmax scale may leave the range of the numbers: all visible keys count alike."""
+    b = Batch([30, 150], [64, 300], 8, 2, dim, 16, fp8)
+    b.q[::3] = 0
+    b.q[1::3] = (b.q[1::3].float() * 2.0 ** -120).bfloat16()
+    b.check(b.call(scale=scale), scale=scale)
+
+
 # ------------------------------------------------------------------------------------------------------ nothing to attend to
 def test_no_sequences_and_tables_without_columns():
     """An empty batch is not an error, for the attention as for the read-back: every row is one of no sequence.  With a table
