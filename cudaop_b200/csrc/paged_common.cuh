@@ -63,7 +63,7 @@ __device__ __forceinline__ Range block_range(const Shape& s, const Seq& q, int i
     const int first = q.kv - q.n + s.token_of(r0), last = q.kv - q.n + s.token_of(r1 - 1);   // positions of the block's tokens
     Range r;
     r.hi = s.causal ? min(q.cap, last + 1) : q.cap;
-    r.lo = s.window > 0 ? max(0, first - s.window + 1) : 0;
+    r.lo = s.window > 0 && first >= s.window ? first - s.window + 1 : 0;       // (a negative position less a large window would pass 32 bits)
     if (r.lo >= r.hi) { r.lo = 0; r.hi = 0; }
     r.tile0 = r.lo / kt;
     r.tiles = max(1, (r.hi + kt - 1) / kt - r.tile0);

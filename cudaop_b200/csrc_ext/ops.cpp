@@ -467,7 +467,7 @@ std::tuple<torch::Tensor, c10::optional<torch::Tensor>> paged_attention(
                                    cu_q.data_ptr<int>(), kv_lens.data_ptr<int>(), o.data_ptr(), lse.has_value() ? lse->data_ptr<float>() : nullptr,
                                    (int)seqs, (int)tokens, (int)heads, c.kv_heads, c.dim, q.stride(0), q.stride(1),
                                    (int)std::min<int64_t>(max_q, tokens), (int)page_table.size(1), c.pages, c.page, c.fp8, (float)scale, causal,
-                                   (int)std::min<int64_t>(window, INT32_MAX / 2), !given, ws.data_ptr(), stream_of(k_cache)),
+                                   (int)std::min<int64_t>(window, INT32_MAX), !given, ws.data_ptr(), stream_of(k_cache)),
              "b200q_paged_attention");
     return {o, lse};
 }

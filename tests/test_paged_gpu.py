@@ -741,6 +741,26 @@ def test_rows_of_zeros_and_next_to_zero_with_a_small_scale(kernel, scale, dim, f
     b.check(b.call(scale=scale), scale=scale)
 
 
+@pytest.mark.parametrize("dim,fp8", [(128, True), (64, False)])
+@pytest.mark.parametrize("window", [2 ** 30, 2 ** 31 - 1, 2 ** 62])
+def test_windows_that_hide_nothing(kernel, window, dim, fp8):
+    """The largest windows, with chunks that are longer than what is cached (their first positions are negative)."""
+    import cudaop_b200 as ops
+    b = Batch([40, 3, 300], [7, 100, 290], 8, 2, dim, 16, fp8)
+    want = b.call()
+    got = b.call(window=window)
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+    if window < 2 ** 31:                                             # ... and through the C ABI
+        L = ops.lib()
+        q, table, cu, lens = b.q.cuda(), b.table.cuda(), b.cu.cuda(), torch.tensor(b.kv, dtype=torch.int32).cuda()
+        out = torch.zeros_like(q)
+        ws = torch.empty(L.b200q_paged_attention_workspace_bytes(dim), dtype=torch.uint8, device="cuda")
+        at = [t if t is None else t.data_ptr() for t in (q, *b.cache, table, cu, lens, out, None)]
+        assert L.b200q_paged_attention(*at, 3, q.shape[0], 8, 2, dim, q.stride(0), q.stride(1), 300, table.shape[1], b.pages, 16, fp8,
+                                       dim ** -0.5, 1, window, 1, ws.data_ptr(), torch.cuda.current_stream().cuda_stream) == 0
+        assert torch.equal(out, want[0])
+
+
 # ------------------------------------------------------------------------------------------------------ nothing to attend to
 def test_no_sequences_and_tables_without_columns():
     """An empty batch is not an error, for the attention as for the read-back: every row is one of no sequence.  With a table
