@@ -761,6 +761,41 @@ def test_windows_that_hide_nothing(kernel, window, dim, fp8):
         assert torch.equal(out, want[0])
 
 
+# ------------------------------------------------------------------------------------------------------ bits of the probabilities
+@pytest.mark.parametrize("n", [1, 20])
+@pytest.mark.parametrize("dim,fp8", [(128, True), (64, True), (128, False), (64, False)])
+def test_bits_of_the_probabilities(kernel, dim, fp8, n):
+    """Two kinds of keys, half of them with p = 1 and half with a p that differs by row, and values of opposite sign that nearly cancel
+    in some columns: there the rounding of the output is small, and that of p shows undiluted, since all its errors agree."""
+    import cudaop_b200 as ops
+    kv, heads, scale = 200, 16, 0.25
+    b = Batch([n], [kv], heads, 1, dim, 16, fp8, seed=2)
+    g = torch.Generator().manual_seed(n)
+    b.q = torch.zeros(n, heads, dim, dtype=torch.bfloat16)
+    b.q[:, :, 0] = (0.25 + 8 * torch.rand(n, heads, generator=g)).bfloat16()       # one product a score: exact in 32 bits
+    b.k[0].zero_()
+    b.k[0][1::2, :, 0] = -1.0
+    b.v[0][0::2] = 1.0
+    b.v[0][1::2] = -torch.exp2(torch.linspace(-0.5, 3.5, dim)).bfloat16()
+    at = torch.arange(kv)
+    ops.paged_cache_write(b.k[0].cuda(), b.v[0].cuda(), (b.table[0][at // 16].long() * 16 + at % 16).cuda(), **names(b.cache))
+    out, _ = b.call(causal=False, scale=scale)
+    torch.cuda.synchronize()
+    k, v = b.held(0, "k")[:, 0], b.held(0, "v")[:, 0]
+    x = torch.einsum("nhd,kd->nhk", b.q.double(), k) * scale
+    p = torch.exp(x - x.amax(2, keepdim=True))
+    want, share = (p @ v) / p.sum(2, keepdim=True), (p @ v.abs()) / p.sum(2, keepdim=True)
+    # p: fp16 for an E4M3 cache; for a bf16 cache two bf16 in the split-KV kernel (half a step of what half a step leaves), one in the
+    # tensor-core kernel.  Everything else is 32-bit: the score's three roundings (|x| <= 4 in units of log2), 2^x (2^-22), sums of 200
+    bits = 2.0 ** -11 if fp8 else 2.0 ** -8 if kernel == "chunk" else 2.0 ** -16
+    bound = 2.0 ** -8 * want.abs() + (bits + 2.0 ** -17) * share
+    err = (out.double().cpu() - want).abs()
+    assert (err <= bound).all(), float((err / bound).max())
+    if fp8 or kernel != "chunk":                                     # one bf16 would not pass
+        rough = (p.bfloat16().double() @ v) / p.sum(2, keepdim=True)
+        assert ((rough - want).abs() > 2 * (2.0 ** -8 * want.abs() + (bits + 2.0 ** -17) * share)).any()
+
+
 # ------------------------------------------------------------------------------------------------------ nothing to attend to
 def test_no_sequences_and_tables_without_columns():
     """An empty batch is not an error, for the attention as for the read-back: every row is one of no sequence.  With a table
