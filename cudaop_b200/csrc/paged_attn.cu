@@ -5,25 +5,33 @@
 namespace b200q {
 namespace paged {
 int page_shift_of(int page_size);        // paged_cache.cu
-// Rows per kv head up to which the split-KV kernel is taken.  It reads the keys once per 16 rows, mostly from L2; the tensor-core kernel
-// once, but takes longer to start.  24 sequences of up to 8192 tokens, heads 32/4 of 64, bf16: 38 / 47 / 61 / 74 us with 16 / 32 / 48 / 64
-// rows against 53 us; heads 5/5, E4M3, 42 rows: 36 / 37; heads 8/8 of 128, E4M3, 44 rows: 40 / 41; heads 4/1, 52 rows: 46 / 52.
-constexpr int kSplitRows = 48;
-// ... and pairs of a block of 16 rows and a tile of 64 keys up to which it is taken whatever the rows are (counted from the sizes
-// of the call, so an upper bound).  Heads 32/8 of 128, E4M3, split-KV against tensor cores: one sequence, 64 new on 512 (1024 pairs)
-// 18 / 32 us, 128 on 512 (2048) 24 / 33, 64 on 2048 (4096) 32 / 34, 256 on 1024 (8192) 52 / 37; 64 sequences, 32 on 64 (2408) 42 / 38.
-// A window bounds the tiles a block sees: one sequence, 21 new on 4587, window 429, heads 40/5 of 64, bf16: 13.1 / 23.2.
-constexpr long long kSplitPairs = 4096;
-bool few_pairs(const Args& a)
+// Which kernel.  The split-KV kernel reads the keys once per 16 rows, mostly from L2; the tensor-core kernel once, but takes longer to start.
+// Figures are split-KV / tensor cores in us; chunks of equal length on the given lengths, 8 kv heads of 128, 32 heads unless said.
+//
+// E4M3 cache (p has 11 bits in both).  Up to 32 rows per kv head the split-KV kernel: 64 sequences of 1024 tokens, 16 / 24 / 32 / 40 / 48 rows:
+// 62/118, 106/120, 108/121, 153/120, 156/120; 256 of 256: 89/170, 155/180, 164/181, 232/183, 239/181; 24 of up to 8192, heads 32/4: 48/78,
+// 91/88, 87/89, 103/70, 140/93.  With more rows where the call is small, counted in blocks of 16 rows and tiles of 64 keys from its sizes (an
+// upper bound), a block costing about as much as eight tiles: one sequence, 64 new on 512 (2048) 20/33, 128 on 512 (4096) 26/34, 64 on
+// 2048 (5120) 35/35, 128 on 1024 (6144) 41/39, 256 on 1024 (12288) 59/37; 8 sequences, 16 on 256 (3072) 19/15; 64, 32 on 64 (36864) 88/39.
+//
+// bf16 cache.  The split-KV kernel holds p in two bf16 terms, the tensor-core kernel in one (8 bits), so it is kept for longer than its time alone
+// would have it: 64 sequences of 1024 tokens, 32 / 40 / 48 rows: 119/104, 169/104, 170/105, heads of 64 68/68, 96/68, 97/68; 64 sequences, 32 on
+// 64 (4096 pairs of a block and a tile): 79/38; one sequence, 256 on 1024 (8192): 56/37.
+constexpr int kSplitRowsE4m3 = 32, kSplitRowsBf16 = 48;
+constexpr long long kSplitWork = 4096;
+bool split_kernel(const Args& a, bool fp8)
 {
+    if (static_cast<long long>(a.max_q) * a.s.group <= (fp8 ? kSplitRowsE4m3 : kSplitRowsBf16)) return true;
     long long tiles = ((static_cast<long long>(a.s.max_pages) << a.s.page_shift) + 63) / 64;
-    if (a.s.window > 0) {                            // the 16 rows are at most 16 / group + 1 tokens, rounded up
+    // A window bounds the tiles a block sees (one sequence, 21 new on 4587, window 429, heads 40/5 of 64, bf16: 13/23): the 16 rows are at
+    // most 16 / group + 1 tokens, rounded up.
+    if (a.s.window > 0) {
         const long long seen = (static_cast<long long>(a.s.window) + (15 + a.s.group) / a.s.group + 62) / 64 + 1;
         tiles = seen < tiles ? seen : tiles;
     }
-    return most_blocks(a, 16) * tiles <= kSplitPairs;
+    return most_blocks(a, 16) * (tiles + (fp8 ? 8 : 0)) <= kSplitWork;
 }
-int g_impl = 0;                          // 0 by the number of rows, 1 split-KV kernel, 2 tensor-core kernel
+int g_impl = 0;                          // 0 by the rule above, 1 split-KV kernel, 2 tensor-core kernel
 size_t open_bytes() { return (static_cast<size_t>(attn_split_ctas()) * sizeof(Open) + 15) / 16 * 16; }
 }
 }
@@ -77,8 +85,8 @@ int b200q_paged_attention(const void* q, const void* k_cache, const void* v_cach
     if (a.status == nullptr) return cudaErrorInvalidDevice;
     a.open = static_cast<Open*>(workspace);
     a.part = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + open_bytes());
-    const bool chunk = g_impl != 0 ? g_impl == 2 : static_cast<long long>(a.max_q) * a.s.group > kSplitRows && !few_pairs(a);
-    return chunk ? attn_chunk(a, head_dim, fp8 != 0, static_cast<cudaStream_t>(stream)) : attn_split(a, head_dim, fp8 != 0, static_cast<cudaStream_t>(stream));
+    const bool split = g_impl != 0 ? g_impl == 1 : split_kernel(a, fp8 != 0);
+    return split ? attn_split(a, head_dim, fp8 != 0, static_cast<cudaStream_t>(stream)) : attn_chunk(a, head_dim, fp8 != 0, static_cast<cudaStream_t>(stream));
 }
 
 int b200q_paged_set_impl(int impl)
