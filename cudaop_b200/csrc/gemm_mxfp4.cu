@@ -95,6 +95,7 @@ gemm_mxfp4_few_rows_kernel(const __grid_constant__ CUtensorMap tmW, const __grid
             if (!ok) __nanosleep(200000);                        // let loads in flight land before the CTA leaves
         }
     } else if (warp == 1) {
+        ptx::pdl_wait();                                         // (the kernel before this one does not count against the waits' limit)
         if (ptx::elect_one()) {
             const uint32_t idesc = ptx::umma_idesc_block_scaled(1, 1, kBN, p.mt, 0, 0, 1);
             const uint32_t tsfw = tmem_base + 128, tsfx = tsfw + 8;
@@ -127,6 +128,7 @@ gemm_mxfp4_few_rows_kernel(const __grid_constant__ CUtensorMap tmW, const __grid
     } else {
         // accumulator lane = row of B (output column), accumulator column = row of A (output row): for one output row a
         // warp stores 32 neighbouring columns
+        ptx::pdl_wait();
         const int q = warp & 3;
         const int n = n0 + q * 32 + lane;
         const bool ok = ptx::mbar_wait(done_bar, 0, p.status, 4);

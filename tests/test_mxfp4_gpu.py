@@ -249,3 +249,24 @@ def test_refusals():
     with pytest.raises(RuntimeError):
         ops.quant_rows_mxfp4(torch.zeros((0, 64), dtype=torch.bfloat16, device="cuda"))
     torch.cuda.synchronize()
+
+
+def test_the_kernel_before_does_not_count_against_the_wait_limit():
+    """A product launched beside a quantiser that runs longer than the limit of the device's waits."""
+    import cudaop_b200 as ops
+    L = ops.lib()
+    a, sa, b, sb = case(5, 300, 2080, 9)
+    args = [dev(pack(a)), dev(sa), dev(pack(b)), dev(sb)]
+    blocks = [args[0], ops.mxfp8_swizzle_sf(args[1], 2080), args[2], ops.mxfp8_swizzle_sf(args[3], 2080)]
+    want = ops.gemm_mxfp4(*blocks, blocked=True)
+    big = torch.zeros((1 << 17, 1 << 14), dtype=torch.bfloat16, device="cuda")
+    torch.cuda.synchronize()
+    assert L.b200q_set_wait_limit_ms(0, 1) == 0
+    try:
+        for _ in range(3):
+            ops.quant_rows_mxfp4(big)
+            got = ops.gemm_mxfp4(*blocks, blocked=True)
+            torch.cuda.synchronize()
+            assert ops.status() == 0 and torch.equal(got, want)
+    finally:
+        L.b200q_set_wait_limit_ms(0, 2000)
