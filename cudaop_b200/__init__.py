@@ -290,7 +290,7 @@ def paged_cache_write(k, v, slots, k_cache, v_cache, k_scale=None, v_scale=None)
 def paged_cache_read(k_cache, v_cache, page_table, cu_kv, total: int, k_scale=None, v_scale=None, k_out=None, v_out=None):
     """Sequences of a paged cache back to bf16: (k, v), each [total, kv_heads, head_dim], row ``cu_kv[b] + j`` being token j
     of sequence b.  ``page_table``: int32 [seqs, max_pages]; ``cu_kv``: int32 [seqs + 1]; ``total``: rows of the output
-    (normally ``cu_kv[-1]``).  A token whose page number is not in the cache (say -1) reads as zero.  Rows of no sequence
+    (normally ``cu_kv[-1]``).  The starts ascend from 0 (one below counts as 0).  A token whose page number is not in the cache (say -1) reads as zero.  Rows of no sequence
     are zero, or left as they are where ``k_out`` and ``v_out`` are given."""
     return _ext().paged_cache_read(k_cache, v_cache, page_table, cu_kv, int(total), k_scale, v_scale, k_out, v_out)
 
@@ -302,7 +302,7 @@ def paged_attention(q, k_cache, v_cache, page_table, cu_q, kv_lens, max_q: int, 
     ``q``: bf16 [tokens, heads, head_dim] (slices of a fused projection's output are taken as they are), the chunks of the
     sequences (at most 8192) one after the other: rows ``cu_q[b]`` to ``cu_q[b + 1]`` (int32 [seqs + 1], from 0; lengths may
     differ, and be zero).  They are the last tokens of the ``kv_lens[b]`` (int32 [seqs]) cached ones.  ``max_q``: a bound of the chunk
-    lengths (it chooses the kernel; a wrong one costs time only).  ``heads`` is a multiple of the cache's kv_heads; query
+    lengths (it chooses the kernel; a wrong one costs time, and over a bf16 cache may change the bits of the probabilities).  ``heads`` is a multiple of the cache's kv_heads; query
     head h reads kv head h // (heads // kv_heads).  ``page_table``: int32 [seqs, max_pages]; a token whose page number is not in
     the cache is left out.
     A token at position p sees keys j <= p (``causal``; else all), and with a ``window`` only j > p - window.  A row
@@ -310,7 +310,10 @@ def paged_attention(q, k_cache, v_cache, page_table, cu_q, kv_lens, max_q: int, 
     the sequence has may be anything, NaN included, and a token reaches only the rows that see it, whatever its values are.  (An
     E4M3 cache says NaN in its scales; a NaN byte, which the write never stores, would reach a whole block of rows.)
     ``return_lse``: returns (out, lse), lse fp32 [tokens, heads] the natural log of the sum of exponentials (-inf for a row that
-    sees nothing).  Rows of no sequence are zero, or left as they are where ``out`` is given."""
+    sees nothing).  Rows of no sequence are zero, or left as they are where ``out`` is given.
+    Scores, sums and accumulators have 32 bits.  The probabilities enter the product with the values in 11 bits (times the
+    value's scale) over an E4M3 cache; over a bf16 cache in 16 bits up to 48 rows (tokens of a chunk times query heads of a kv
+    head) and in small calls, in 8 bits else.  Value scales below 2^-126, which the write does not make, count as zero."""
     o, lse = _ext().paged_attention(q, k_cache, v_cache, page_table, cu_q, kv_lens, int(max_q), k_scale, v_scale,
                                     float(q.shape[-1] ** -0.5 if scale is None else scale), bool(causal), int(window), bool(return_lse), out)
     return (o, lse) if return_lse else o

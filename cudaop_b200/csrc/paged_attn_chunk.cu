@@ -57,18 +57,6 @@ struct Cfg {
     static_assert(kQBytes + kSlots * kSlotBytes >= 8192 * 4, "a word per sequence");
 };
 
-__device__ __forceinline__ uint32_t pack_f16x2(float lo, float hi)
-{
-    const __half2 v = __floats2half2_rn(lo, hi);
-    return *reinterpret_cast<const uint32_t*>(&v);
-}
-// two bf16 with those that are not finite set to zero
-__device__ __forceinline__ uint32_t only_finite(uint32_t w)
-{
-    if ((w & 0x7F80u) == 0x7F80u) w &= 0xFFFF0000u;
-    if ((w & 0x7F800000u) == 0x7F800000u) w &= 0x0000FFFFu;
-    return w;
-}
 // 16-byte unit `unit` of row `row` in a [rows][128 bytes] column with the 128-byte swizzle
 __device__ __forceinline__ uint32_t unit_at(uint32_t column, int row, int unit) { return column + row * 128 + ((unit ^ (row & 7)) << 4); }
 

@@ -70,14 +70,6 @@ __device__ __forceinline__ uint32_t swizzled(uint32_t base, int row, int byte)
     return base + (a ^ (kBox == 128 ? (a >> 3) & 0x70u : (a >> 3) & 0x30u));
 }
 
-// two bf16 with those that are not finite set to zero
-__device__ __forceinline__ uint32_t only_finite(uint32_t w)
-{
-    if ((w & 0x7F80u) == 0x7F80u) w &= 0xFFFF0000u;
-    if ((w & 0x7F800000u) == 0x7F800000u) w &= 0x0000FFFFu;
-    return w;
-}
-
 // Adds the values of a half tile's 16 keys that are not finite to the rows that see them; `at`: the first of the warp's rows, whose
 // eight 16-byte units are swizzled; a lane has columns of unit g.  Rare, and short rather than fast.
 template <int NT, int STEPS, typename Seen>
@@ -108,12 +100,6 @@ __device__ __forceinline__ void mma(float (&d)[4], uint32_t a0, uint32_t a1, uin
 {
     if (FP8) ptx::mma_f16_16816(d, a0, a1, a2, a3, b0, b1);
     else ptx::mma_bf16_16816(d, a0, a1, a2, a3, b0, b1);
-}
-
-__device__ __forceinline__ uint32_t pack_f16x2(float lo, float hi)
-{
-    const __half2 v = __floats2half2_rn(lo, hi);
-    return *reinterpret_cast<const uint32_t*>(&v);
 }
 
 template <int D, bool FP8, int NT>

@@ -209,5 +209,18 @@ __device__ __forceinline__ float mantissa_of(float s)
     return f == 255u ? s : f == 0u ? 0.0f : __uint_as_float((b & 0x807FFFFFu) | 0x3F000000u);
 }
 
+__device__ __forceinline__ uint32_t pack_f16x2(float lo, float hi)
+{
+    const __half2 v = __floats2half2_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t*>(&v);
+}
+// two bf16 with those that are not finite set to zero
+__device__ __forceinline__ uint32_t only_finite(uint32_t w)
+{
+    if ((w & 0x7F80u) == 0x7F80u) w &= 0xFFFF0000u;
+    if ((w & 0x7F800000u) == 0x7F800000u) w &= 0x0000FFFFu;
+    return w;
+}
+
 }  // namespace paged
 }  // namespace b200q

@@ -158,7 +158,7 @@ int b200q_paged_cache_write(const void* k, const void* v, const long long* slots
                             long long k_head_stride, long long v_head_stride, int num_pages, int page_size, int fp8, void* stream);
 
 /* Read back: k, v [total, kv_heads, head_dim] bf16, row cu_kv[b] + j = token j of sequence b (page_table: DEVICE int32
- * [seqs, max_pages], cu_kv: DEVICE int32 [seqs + 1]).  Tokens on pages outside the cache read as zero; rows of no
+ * [seqs, max_pages], cu_kv: DEVICE int32 [seqs + 1], ascending; a start below 0 counts as 0).  Tokens on pages outside the cache read as zero; rows of no
  * sequence are zeroed (zero_rest != 0) or left. */
 int b200q_paged_cache_read(const void* k_cache, const void* v_cache, const float* k_scale, const float* v_scale,
                            const int* page_table, const int* cu_kv, void* k, void* v, int seqs, int total, int kv_heads, int head_dim,
@@ -168,10 +168,12 @@ int b200q_paged_cache_read(const void* k_cache, const void* v_cache, const float
  * optionally lse[tokens, heads] (fp32, natural log; NULL for none).  The rows cu_q[b] .. cu_q[b + 1] of q (DEVICE int32
  * [seqs + 1]) are the last tokens of the kv_lens[b] (DEVICE int32 [seqs]) cached ones; the token at position p sees keys
  * j <= p (causal != 0), and j > p - window (window > 0, needs causal); rows that see nothing are zero, lse -inf.  max_q: a
- * bound of the chunk lengths (speed only).  Tokens on pages outside the cache are left out.  Rows of no sequence are zeroed
+ * bound of the chunk lengths (it chooses the kernel).  Tokens on pages outside the cache are left out.  Rows of no sequence are zeroed
  * (zero_rest != 0) or left.  At most 8192 sequences.  A token reaches only the rows that see it, whatever its
  * values are (an E4M3 cache says NaN in its scales; a NaN byte, which the write never stores, would reach a whole block of
- * rows). Row (token, head) of q is at token * q_stride + head * q_head_stride elements.  `workspace`:
+ * rows).  Value scales below 2^-126 count as zero.  Probabilities enter the product with the values in 11 bits (E4M3
+ * cache), 16 bits (bf16 cache, split-KV kernel) or 8 bits (bf16 cache, tensor-core kernel); everything else has 32 bits.
+ * Row (token, head) of q is at token * q_stride + head * q_head_stride elements.  `workspace`:
  * caller-owned scratch of b200q_paged_attention_workspace_bytes(head_dim) bytes, 16-byte aligned, no contents needed, not to be
  * shared by calls that may overlap. */
 int b200q_paged_attention(const void* q, const void* k_cache, const void* v_cache, const float* k_scale, const float* v_scale,
