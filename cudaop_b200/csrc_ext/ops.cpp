@@ -31,6 +31,8 @@ void check_cuda_2d(const torch::Tensor& t, const char* name, std::initializer_li
     TORCH_CHECK_VALUE(t.dim() == dim, name, " must have ", num(dim), " dimensions, got ", num(t.dim()));
     TORCH_CHECK_VALUE(t.is_cuda(), name, " must be a CUDA tensor");
     TORCH_CHECK_VALUE(t.is_contiguous(), name, " must be contiguous");
+    // the rows and columns of a matrix are 32-bit numbers from here on
+    if (dim == 2) TORCH_CHECK_VALUE(t.size(0) <= INT32_MAX && t.size(1) <= INT32_MAX, name, " has too many rows or columns for 32-bit numbers");
     bool ok = false;
     for (auto d : dtypes) ok = ok || t.scalar_type() == d;
     TORCH_CHECK_VALUE(ok, name, " has dtype ", c10::toString(t.scalar_type()), ", which this operator does not take");
@@ -237,6 +239,7 @@ torch::Tensor gemm_mxfp4(torch::Tensor aq, torch::Tensor sfa, torch::Tensor bq, 
     check_cuda_2d(aq, "aq", {kU8}); check_cuda_2d(bq, "bq", {kU8});
     const int64_t M = aq.size(0), N = bq.size(0), K = 2 * aq.size(1);
     TORCH_CHECK_VALUE(aq.size(1) == bq.size(1) && K % 32 == 0, "shape mismatch (K must match and be a multiple of 32)");
+    TORCH_CHECK_VALUE(K <= INT32_MAX, "K is too large for a 32-bit number");
     const c10::cuda::CUDAGuard guard(aq.device());
     auto c = out_like(aq, {M, N}, kBF16);
     if (blocked) {

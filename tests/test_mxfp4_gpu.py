@@ -270,3 +270,22 @@ def test_the_kernel_before_does_not_count_against_the_wait_limit():
             assert ops.status() == 0 and torch.equal(got, want)
     finally:
         L.b200q_set_wait_limit_ms(0, 2000)
+
+
+def test_sizes_that_pass_32_bits_are_refused():
+    """Cut to 32 bits, 2^32 + 64 columns would be 64, and all behind them stay unwritten."""
+    import cudaop_b200 as ops
+    x = torch.empty((1, 2 ** 32 + 64), dtype=torch.bfloat16, device="cuda")
+    with pytest.raises(ValueError):
+        ops.quant_rows_mxfp4(x)
+    with pytest.raises(ValueError):
+        ops.quant_rows_e4m3(x)
+    del x
+    for half in (2 ** 30 + 16, 2 ** 31 + 16):                        # K = 2^31 + 32 and 2^32 + 32
+        a = torch.empty((1, half), dtype=torch.uint8, device="cuda")
+        s = torch.empty((1, 2 * half // 32), dtype=torch.uint8, device="cuda")
+        with pytest.raises(ValueError):
+            ops.gemm_mxfp4(a, s, a, s)
+        del a, s
+    torch.cuda.synchronize()
+    assert ops.status() == 0
