@@ -12,7 +12,7 @@ int page_shift_of(int page_size);        // paged_cache.cu
 // 62/118, 106/120, 108/121, 153/120, 156/120; 256 of 256: 89/170, 155/180, 164/181, 232/183, 239/181; 24 of up to 8192, heads 32/4: 48/78,
 // 91/88, 87/89, 103/70, 140/93.  With more rows where the call is small, counted in blocks of 16 rows and tiles of 64 keys from its sizes (an
 // upper bound), a block costing about as much as eight tiles: one sequence, 64 new on 512 (2048) 20/33, 128 on 512 (4096) 26/34, 64 on
-// 2048 (5120) 35/35, 128 on 1024 (6144) 41/39, 256 on 1024 (12288) 59/37; 8 sequences, 16 on 256 (3072) 19/15; 64, 32 on 64 (36864) 88/39.
+// 2048 (5120) 35/35, 128 on 1024 (6144) 41/39, 256 on 1024 (12288) 59/37; 8 sequences, 16 on 256 tokens 19/15; 64, 32 on 64 (36864) 88/39.
 //
 // bf16 cache.  The split-KV kernel holds p in two bf16 terms, the tensor-core kernel in one (8 bits), so it is kept for longer than its time alone
 // would have it: 64 sequences of 1024 tokens, 32 / 40 / 48 rows: 119/104, 169/104, 170/105, heads of 64 68/68, 96/68, 97/68; 64 sequences, 32 on
