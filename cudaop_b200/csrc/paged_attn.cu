@@ -16,7 +16,7 @@ int page_shift_of(int page_size);        // paged_cache.cu
 //
 // bf16 cache.  The split-KV kernel holds p in two bf16 terms, the tensor-core kernel in one (8 bits), so it is kept for longer than its time alone
 // would have it: 64 sequences of 1024 tokens, 32 / 40 / 48 rows: 119/104, 169/104, 170/105, heads of 64 68/68, 96/68, 97/68; 64 sequences, 32 on
-// 64 (4096 pairs of a block and a tile): 79/38; one sequence, 256 on 1024 (8192): 56/37.
+// 64 (4096 pairs of a block and a tile): 79/37; one sequence, 128 on 1024 (4096): 36/34, 256 on 1024 (8192): 61/36.
 constexpr int kSplitRowsE4m3 = 32, kSplitRowsBf16 = 48;
 constexpr long long kSplitWork = 4096;
 bool split_kernel(const Args& a, bool fp8)
